@@ -174,6 +174,22 @@ def _register_fakes() -> None:
         return (q.new_empty((b, h, t, d)), q.new_empty((b, h, t, d)), q.new_empty((b, h, t, d)),
                 q.new_empty((b, h, t, d)) if need_gdout else q.new_empty((0,)))
 
+    @torch.library.register_fake("ttt::layer_norm")
+    def _ln(x, w, b, eps, need_stats):
+        stats = x.new_empty((2, x.numel() // x.shape[-1] if need_stats else 0), dtype=torch.float32)
+        return x.new_empty(x.shape), stats[0], stats[1]
+
+    @torch.library.register_fake("ttt::layer_norm_bwd")
+    def _ln_bwd(dy, x, w, mean, rstd, need_dx, need_dw, need_db, p_type):
+        d = x.shape[-1]
+        return (x.new_empty(x.shape if need_dx else (0,)), x.new_empty((d if need_dw else 0,), dtype=p_type),
+                x.new_empty((d if need_db else 0,), dtype=p_type))
+
+    @torch.library.register_fake("ttt::layer_norm_bwd2")
+    def _ln_bwd2(dy, x, w, mean, rstd, ux, uw, ub):
+        gw = x.new_empty((0,)) if w is None else w.new_empty(w.shape)
+        return x.new_empty(x.shape), x.new_empty(x.shape), gw
+
     @torch.library.register_fake("ttt::error_word")
     def _err(device):
         return torch.empty((1,), dtype=torch.int32, device=device)
@@ -490,6 +506,25 @@ def attn_bwd2_noalloc(q, k, v, dout, lse2, delta, uq, uk, uv, causal: bool, scal
         if _SYNC_CHECK:
             check_device_errors(q.device)
     return gq, gk, gv, gdout
+
+
+# ---------------------------------------------------------------- layer norm (include/ttt_ops.h)
+def layer_norm(x, w, b, eps: float, need_stats: bool):
+    """y, mean, rstd (fp32 [rows]; empty unless need_stats) over rows of x's last dimension."""
+    load_torch_ops()
+    return _op(torch.ops.ttt.layer_norm, x, w, b, eps, need_stats)
+
+
+def layer_norm_bwd(dy, x, w, mean, rstd, need, p_type):
+    """dx, dw, db; need = (dx, dw, db) wanted (an output that is not is empty)."""
+    load_torch_ops()
+    return _op(torch.ops.ttt.layer_norm_bwd, dy, x, w, mean, rstd, *map(bool, need), p_type)
+
+
+def layer_norm_bwd2(dy, x, w, mean, rstd, ux, uw, ub):
+    """Gradients (gdy, gx, gw) of <dx, ux> + <dw, uw> + <db, ub>; a probe given as None is zero."""
+    load_torch_ops()
+    return _op(torch.ops.ttt.layer_norm_bwd2, dy, x, w, mean, rstd, ux, uw, ub)
 
 
 # ---------------------------------------------------------------- passes over materialized P

@@ -1,6 +1,5 @@
 """Build libttt_attn.so (the sm_100a kernels + C ABI) in-tree with nvcc, and
-libttt_torch.so (the ttt::fwd / ttt::bwd / ttt::bwd2 PyTorch operators over
-that C ABI) with g++ against the installed torch.
+libttt_torch.so (the ttt::* PyTorch operators over that C ABI) with g++ against the installed torch.
 
 The libraries are written to ``testtimeideas_b200/_lib/`` and object files to
 ``testtimeideas_b200/_build/``; both are git-ignored build products. Usage::
@@ -25,11 +24,11 @@ INCLUDE = PKG.parent / "include"
 BUILD = PKG / "_build"
 LIBDIR = PKG / "_lib"
 LIB = LIBDIR / "libttt_attn.so"
-TORCH_SRC = CSRC / "torch_ops.cpp"
+TORCH_SRCS = [CSRC / "torch_ops.cpp", CSRC / "torch_model_ops.cpp"]
 TORCH_LIB = LIBDIR / "libttt_torch.so"
 
 SOURCES = ["capi.cu", "attn_fwd.cu", "attn_bwd_qm.cu", "attn_bwd_km.cu", "misc.cu", "noalloc.cu", "attn_from_p.cu",
-           "attn_pwrite.cu"]
+           "attn_pwrite.cu", "norm.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-Xptxas", "-warn-spills"]
@@ -94,11 +93,11 @@ def cuda_home() -> Path:
 
 
 def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
-    """Compile torch_ops.cpp into libttt_torch.so, linked against libttt_attn.so
+    """Compile the operator files into libttt_torch.so, linked against libttt_attn.so
     (found next to it through an $ORIGIN run path) and torch's libraries."""
     import torch
 
-    deps = [TORCH_SRC, LIB, *sorted(INCLUDE.glob("*.h"))]
+    deps = [*TORCH_SRCS, LIB, CSRC / "torch_common.h", *sorted(INCLUDE.glob("*.h"))]
     if not force and TORCH_LIB.exists() and all(d.stat().st_mtime <= TORCH_LIB.stat().st_mtime for d in deps):
         return TORCH_LIB
     torch_dir = Path(torch.__file__).resolve().parent
@@ -107,12 +106,12 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     tmp = TORCH_LIB.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           *[f"-I{p}" for p in incs], str(TORCH_SRC), "-o", str(tmp),
+           *[f"-I{p}" for p in incs], *map(str, TORCH_SRCS), "-o", str(tmp),
            f"-L{torch_dir / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
            f"-L{LIBDIR}", "-lttt_attn", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_dir / 'lib'}"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for {TORCH_SRC.name}:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+        raise RuntimeError(f"g++ failed for {TORCH_LIB.name}:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
     if verbose and r.stderr.strip():
         print(r.stderr, file=sys.stderr)
     os.replace(tmp, TORCH_LIB)

@@ -24,6 +24,7 @@
 #include <mutex>
 #include <tuple>
 
+#include "torch_common.h"
 #include "ttt_attn.h"
 
 namespace {
@@ -37,6 +38,10 @@ std::mutex g_mu;
 // Never destroyed: tensors held past interpreter shutdown must not be freed
 // after the CUDA runtime has gone.
 std::map<int, DeviceWords>* g_words = new std::map<int, DeviceWords>();
+
+}  // namespace
+
+namespace ttt_torch {
 
 // The device's error word, created (and its mirror registered) on first use;
 // the device must be current.
@@ -65,6 +70,14 @@ void raise_if_pending(int dev, at::Tensor& word) {
 void check(int status, const char* op) {
   TORCH_CHECK(status == TTT_OK, "libttt_attn: ", ttt_attn_status_string(status), " (status ", status, ") in ", op);
 }
+
+}  // namespace ttt_torch
+
+namespace {
+
+using ttt_torch::check;
+using ttt_torch::error_word_for;
+using ttt_torch::raise_if_pending;
 
 // x, or a contiguous copy when its layout cannot feed a TMA tensor map (d
 // stride != 1, a b/h/t stride not a positive multiple of 8 elements, or a base
