@@ -79,7 +79,11 @@ EXPORTED = ("ttt_attn_fwd", "ttt_attn_bwd", "ttt_attn_bwd2", "ttt_attn_t_pad", "
             "ttt_attn_selftest_wait")
 ERR_WORD_TIMEOUT = 0x40000000  # TTT_ERR_WORD_TIMEOUT
 SELFTEST_WAIT_SITE = 0xFE
+ERR_WORD_TARGET = 0x10000000  # TTT_ERR_WORD_TARGET
 NOALLOC_MAX_ROWS = 1 << 20  # TTT_ATTN_NOALLOC_MAX_ROWS
+# Every symbol include/ttt_ops.h declares.
+EXPORTED_OPS = ("ttt_norm_fwd", "ttt_norm_bwd", "ttt_norm_bwd2", "ttt_norm_work_bytes", "ttt_lce_fwd", "ttt_lce_bwd",
+                "ttt_lce_bwd2", "ttt_lce_state_bytes", "ttt_lce_work_bytes")
 KERNEL_KINDS = ("fwd", "delta", "bwd_kv", "bwd_q", "bwd2_stats", "bwd2_q", "bwd2_kv", "from_p")
 
 _lib = None
@@ -190,6 +194,20 @@ def _register_fakes() -> None:
         gw = x.new_empty((0,)) if w is None else w.new_empty(w.shape)
         return x.new_empty(x.shape), x.new_empty(x.shape), gw
 
+    @torch.library.register_fake("ttt::linear_ce")
+    def _lce(h, w, targets, mask, reduction, ignore_index):
+        loss = h.new_empty(targets.shape if reduction == 0 else (), dtype=torch.float32)
+        return loss, h.new_empty((_lce_state_bytes(targets.numel()),), dtype=torch.uint8)
+
+    @torch.library.register_fake("ttt::linear_ce_bwd")
+    def _lce_bwd(dloss, h, w, state, reduction, need_dh, need_dw):
+        return h.new_empty(h.shape if need_dh else (0,)), w.new_empty(w.shape if need_dw else (0,))
+
+    @torch.library.register_fake("ttt::linear_ce_bwd2")
+    def _lce_bwd2(dloss, h, w, state, reduction, uh, uw, need_gdloss, need_gh, need_gw):
+        return (dloss.new_empty(dloss.shape if need_gdloss else (0,), dtype=torch.float32),
+                h.new_empty(h.shape if need_gh else (0,)), w.new_empty(w.shape if need_gw else (0,)))
+
     @torch.library.register_fake("ttt::error_word")
     def _err(device):
         return torch.empty((1,), dtype=torch.int32, device=device)
@@ -245,6 +263,11 @@ def error_word(device: torch.device) -> torch.Tensor:
     return w
 
 
+def _target_message(code: int, dev) -> str:
+    return (f"libttt_attn: a linear cross entropy on {dev} met a target outside the vocabulary (error word "
+            f"0x{code:08x}, row {code & 0xffffff}); results of the calls since then are invalid")
+
+
 def raise_pending(device: torch.device | None = None) -> None:
     """Raise KernelError if a kernel on `device` has reported a failed bounded wait
     to the host mirror; no synchronization. Clears both words (the device word in
@@ -257,6 +280,8 @@ def raise_pending(device: torch.device | None = None) -> None:
         if code == 0:
             return
         _err_words[idx].zero_()
+    if code & ERR_WORD_TARGET:
+        raise KernelError(_target_message(code, f"cuda:{idx}"))
     raise KernelError(f"libttt_attn kernel gave up on a bounded wait on cuda:{idx} (error word 0x{code:08x}); "
                       "results of the calls since then are invalid")
 
@@ -274,6 +299,8 @@ def check_device_errors(device: torch.device | None = None) -> None:
         if code != 0:
             w.zero_()
             torch.cuda.synchronize(dev)
+    if code & ERR_WORD_TARGET:
+        raise KernelError(_target_message(code, dev))
     if code != 0:
         raise KernelError(f"libttt_attn kernel timeout on {dev} (error word 0x{code:08x})")
 
@@ -525,6 +552,44 @@ def layer_norm_bwd2(dy, x, w, mean, rstd, ux, uw, ub):
     """Gradients (gdy, gx, gw) of <dx, ux> + <dw, uw> + <db, ub>; a probe given as None is zero."""
     load_torch_ops()
     return _op(torch.ops.ttt.layer_norm_bwd2, dy, x, w, mean, rstd, ux, uw, ub)
+
+
+# ---------------------------------------------------------------- linear cross entropy (include/ttt_ops.h)
+LCE_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _lce_state_bytes(n: int) -> int:
+    """ttt_lce_state_bytes: the head, four arrays of n rows padded to 128 and one of n, each in 256-byte parts."""
+    up = lambda b: (b + 255) // 256 * 256  # noqa: E731
+    return 256 + 4 * up((n + 127) // 128 * 128 * 4) + up(n * 4)
+
+
+def linear_ce(h, w, targets, mask, reduction: str, ignore_index: int):
+    """loss (fp32; targets' shape for "none", else a scalar) and the state of the gradients."""
+    load_torch_ops()
+    loss, state = _op(torch.ops.ttt.linear_ce, h, w, targets, mask, LCE_REDUCTIONS[reduction], ignore_index)
+    if _SYNC_CHECK:
+        check_device_errors(h.device)
+    return loss, state
+
+
+def linear_ce_bwd(dloss, h, w, state, reduction: str, need):
+    """dh, dw; need = (dh, dw) wanted (an output that is not is empty)."""
+    load_torch_ops()
+    out = _op(torch.ops.ttt.linear_ce_bwd, dloss, h, w, state, LCE_REDUCTIONS[reduction], *map(bool, need))
+    if _SYNC_CHECK:
+        check_device_errors(h.device)
+    return out
+
+
+def linear_ce_bwd2(dloss, h, w, state, reduction: str, uh, uw, need):
+    """Gradients (gdloss, gh, gw) of <dh, uh> + <dw, uw>; a probe given as None is zero,
+    need = (gdloss, gh, gw) wanted."""
+    load_torch_ops()
+    out = _op(torch.ops.ttt.linear_ce_bwd2, dloss, h, w, state, LCE_REDUCTIONS[reduction], uh, uw, *map(bool, need))
+    if _SYNC_CHECK:
+        check_device_errors(h.device)
+    return out
 
 
 # ---------------------------------------------------------------- passes over materialized P

@@ -28,7 +28,8 @@ TORCH_SRCS = [CSRC / "torch_ops.cpp", CSRC / "torch_model_ops.cpp"]
 TORCH_LIB = LIBDIR / "libttt_torch.so"
 
 SOURCES = ["capi.cu", "attn_fwd.cu", "attn_bwd_qm.cu", "attn_bwd_km.cu", "misc.cu", "noalloc.cu", "attn_from_p.cu",
-           "attn_pwrite.cu", "norm.cu"]
+           "attn_pwrite.cu", "norm.cu",
+           "lce.cu", "lce_gemm.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-Xptxas", "-warn-spills"]

@@ -442,6 +442,27 @@ class Fork {
 
 }  // namespace
 
+namespace ttt {
+
+// For the operators of ttt_ops.h (lce.cu): the registered mirror, and a 2-D
+// 16-bit tensor map with 128-byte swizzle, elements outside read as zero.
+int32_t* registered_error_mirror() { return error_mirror(); }
+
+bool encode_2d(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64_t rows, int64_t stride, int box_cols,
+               int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base),
+            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace ttt
+
 extern "C" {
 
 int ttt_attn_t_pad(int t) { return (t + 127) / 128 * 128; }

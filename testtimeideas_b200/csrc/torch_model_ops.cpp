@@ -1,5 +1,5 @@
-// PyTorch operators over include/ttt_ops.h: ttt::layer_norm* (forward, gradient
-// and gradient of the gradient). Like torch_ops.cpp: argument checks, output
+// PyTorch operators over include/ttt_ops.h: ttt::layer_norm* and ttt::linear_ce*
+// (forward, gradient and gradient of the gradient). Like torch_ops.cpp: argument checks, output
 // and work space allocation (PyTorch's caching allocator, on the current device
 // and stream) and the call into the C ABI.
 #include <ATen/ATen.h>
@@ -188,6 +188,178 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_layer_norm_bwd2(const at::Tens
   return {gdy, gx, gw};
 }
 
+// ---------------------------------------------------------------- linear cross entropy
+// w as the kernels read it: unit column stride, a row stride that is a multiple of
+// 8 elements, 16-byte aligned; else a copy with padded rows.
+at::Tensor weight_rows(const at::Tensor& w) {
+  const bool ok = w.stride(1) == 1 && (reinterpret_cast<uintptr_t>(w.data_ptr()) & 15u) == 0 &&
+                  (w.size(0) == 1 || (w.stride(0) >= w.size(1) && w.stride(0) % 8 == 0)) &&
+                  (w.size(0) > 1 || w.size(1) % 8 == 0);
+  if (ok) return w;
+  at::Tensor buf = at::empty({w.size(0), (w.size(1) + 7) / 8 * 8}, w.options());
+  at::Tensor r = buf.narrow(1, 0, w.size(1));
+  r.copy_(w);
+  return r;
+}
+
+ttt_lce_problem lce_problem(const at::Tensor& h, const at::Tensor& w, int64_t reduction, int64_t ignore_index) {
+  TORCH_CHECK(h.is_cuda() && w.is_cuda(), "ttt linear cross entropy needs CUDA tensors");
+  const auto t = h.scalar_type();
+  TORCH_CHECK(t == at::kHalf || t == at::kBFloat16, "ttt linear cross entropy takes fp16 or bf16 tensors, got ", t);
+  TORCH_CHECK(w.scalar_type() == t, "linear cross entropy: hidden and weight must share one dtype, got ", t, " and ",
+              w.scalar_type());
+  TORCH_CHECK(w.device() == h.device(), "linear cross entropy: hidden and weight must be on one device");
+  TORCH_CHECK(h.dim() >= 1 && w.dim() == 2 && h.size(-1) == w.size(1) && w.size(0) >= 1 && w.size(1) >= 1,
+              "linear cross entropy: expected hidden [..., dim] and weight [vocab, dim], got ", h.sizes(), " and ",
+              w.sizes());
+  ttt_lce_problem pb{};
+  pb.dim = static_cast<int32_t>(w.size(1));
+  pb.n = h.numel() / pb.dim;
+  pb.vocab = w.size(0);
+  TORCH_CHECK(pb.dim <= 65536 && pb.n <= (1 << 24) && pb.vocab <= (1 << 24),
+              "linear cross entropy takes at most 2^24 rows, 2^24 vocabulary entries and 65536 columns");
+  pb.dtype = type_code(t);
+  TORCH_CHECK(reduction >= 0 && reduction <= 2, "linear cross entropy: unknown reduction ", reduction);
+  pb.reduction = static_cast<int32_t>(reduction);
+  pb.ignore_index = ignore_index;
+  return pb;
+}
+
+at::Tensor lce_work(const ttt_lce_problem& pb, int pass, const at::Tensor& like) {
+  return scratch(ttt_lce_work_bytes(&pb, pass), like);
+}
+
+std::tuple<at::Tensor, at::Tensor> op_linear_ce(const at::Tensor& h_, const at::Tensor& w_, const at::Tensor& targets_,
+                                                const OptTensor& mask_, int64_t reduction, int64_t ignore_index) {
+  ttt_lce_problem pb = lce_problem(h_, w_, reduction, ignore_index);
+  TORCH_CHECK(targets_.device() == h_.device() && at::isIntegralType(targets_.scalar_type(), false),
+              "linear cross entropy: targets must be integers on hidden's device");
+  TORCH_CHECK(targets_.sizes() == h_.sizes().slice(0, h_.dim() - 1),
+              "linear cross entropy: targets must have hidden's leading shape ", h_.sizes().slice(0, h_.dim() - 1),
+              ", got ", targets_.sizes());
+  c10::cuda::CUDAGuard guard(h_.device());
+  at::Tensor word = error_word_for(h_.get_device());
+  raise_if_pending(h_.get_device(), word);
+  at::Tensor mask;
+  if (mask_.has_value()) {
+    TORCH_CHECK(mask_->device() == h_.device() && mask_->sizes() == targets_.sizes(),
+                "linear cross entropy: mask must have the targets' shape and device, got ", mask_->sizes());
+    const bool u8 = mask_->scalar_type() == at::kBool;
+    mask = (u8 ? *mask_ : mask_->to(at::kFloat)).contiguous();
+    pb.mask_kind = u8 ? TTT_LCE_MASK_U8 : TTT_LCE_MASK_F32;
+  }
+  const at::Tensor h = as_rows(h_, pb.dim), w = weight_rows(w_);
+  const at::Tensor targets = targets_.to(at::kLong).contiguous();
+  const auto f32 = h_.options().dtype(at::kFloat);
+  at::Tensor loss = reduction == TTT_LCE_NONE ? at::empty(targets_.sizes(), f32) : at::empty({}, f32);
+  at::Tensor state = at::empty({ttt_lce_state_bytes(&pb)}, h_.options().dtype(at::kByte));
+  at::Tensor work = lce_work(pb, 0, h_);
+  ttt_lce_fwd_args a{};
+  a.pb = pb;
+  a.h = h.numel() > 0 ? h.data_ptr() : nullptr;
+  a.h_stride = h.stride(0);
+  a.w = w.data_ptr();
+  a.w_stride = w.stride(0);
+  a.targets = pb.n > 0 ? targets.data_ptr<int64_t>() : nullptr;
+  a.mask = mask.defined() ? mask.data_ptr() : nullptr;
+  // an empty loss has no storage; the entry point wants an address
+  a.loss = loss.numel() > 0 ? loss.data_ptr<float>() : reinterpret_cast<float*>(word.data_ptr());
+  a.state = state.numel() > 0 ? state.data_ptr() : nullptr;
+  a.err = word.data_ptr<int32_t>();
+  a.work = ptr(work);
+  a.work_bytes = work.defined() ? work.numel() : 0;
+  check(ttt_lce_fwd(&a, stream()), "ttt::linear_ce");
+  return {loss, state};
+}
+
+// dloss as the entry points read it: fp32, one value or one per row.
+at::Tensor lce_upstream(const at::Tensor& dloss, const at::Tensor& h, const ttt_lce_problem& pb) {
+  TORCH_CHECK(dloss.device() == h.device() && dloss.numel() == (pb.reduction == TTT_LCE_NONE ? pb.n : 1),
+              "linear cross entropy: dloss must have the loss's shape, got ", dloss.sizes());
+  return dloss.to(at::kFloat).contiguous();
+}
+void check_state(const at::Tensor& state, const ttt_lce_problem& pb) {
+  TORCH_CHECK(state.is_cuda() && state.scalar_type() == at::kByte && state.numel() == ttt_lce_state_bytes(&pb),
+              "linear cross entropy: state must be the forward's");
+}
+
+std::tuple<at::Tensor, at::Tensor> op_linear_ce_bwd(const at::Tensor& dloss_, const at::Tensor& h_,
+                                                    const at::Tensor& w_, const at::Tensor& state, int64_t reduction,
+                                                    bool need_dh, bool need_dw) {
+  const ttt_lce_problem pb = lce_problem(h_, w_, reduction, 0);
+  c10::cuda::CUDAGuard guard(h_.device());
+  at::Tensor word = error_word_for(h_.get_device());
+  raise_if_pending(h_.get_device(), word);
+  check_state(state, pb);
+  const at::Tensor h = as_rows(h_, pb.dim), w = weight_rows(w_), dloss = lce_upstream(dloss_, h_, pb);
+  at::Tensor dh = need_dh ? at::empty(h_.sizes(), h_.options()) : at::empty({0}, h_.options());
+  at::Tensor dw = need_dw ? at::empty(w_.sizes(), w_.options()) : at::empty({0}, w_.options());
+  at::Tensor work = lce_work(pb, 1, h_);
+  ttt_lce_bwd_args a{};
+  a.pb = pb;
+  a.h = h.numel() > 0 ? h.data_ptr() : nullptr;
+  a.h_stride = h.stride(0);
+  a.w = w.data_ptr();
+  a.w_stride = w.stride(0);
+  a.state = state.data_ptr();
+  a.dloss = pb.n > 0 || reduction != TTT_LCE_NONE ? dloss.data_ptr<float>() : reinterpret_cast<float*>(word.data_ptr());
+  a.dh = need_dh && pb.n > 0 ? dh.data_ptr() : nullptr;
+  a.dw = need_dw ? dw.data_ptr() : nullptr;
+  a.err = word.data_ptr<int32_t>();
+  a.work = ptr(work);
+  a.work_bytes = work.defined() ? work.numel() : 0;
+  check(ttt_lce_bwd(&a, stream()), "ttt::linear_ce_bwd");
+  return {dh, dw};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> op_linear_ce_bwd2(const at::Tensor& dloss_, const at::Tensor& h_,
+                                                                 const at::Tensor& w_, const at::Tensor& state,
+                                                                 int64_t reduction, const OptTensor& uh_,
+                                                                 const OptTensor& uw_, bool need_gdloss, bool need_gh,
+                                                                 bool need_gw) {
+  const ttt_lce_problem pb = lce_problem(h_, w_, reduction, 0);
+  c10::cuda::CUDAGuard guard(h_.device());
+  at::Tensor word = error_word_for(h_.get_device());
+  raise_if_pending(h_.get_device(), word);
+  check_state(state, pb);
+  const at::Tensor h = as_rows(h_, pb.dim), w = weight_rows(w_), dloss = lce_upstream(dloss_, h_, pb);
+  at::Tensor uh, uw;
+  if (uh_.has_value()) {
+    TORCH_CHECK(uh_->sizes() == h_.sizes() && uh_->device() == h_.device(),
+                "linear cross entropy: uh must have hidden's shape and device");
+    uh = as_rows(uh_->to(h_.scalar_type()), pb.dim);
+  }
+  if (uw_.has_value()) {
+    TORCH_CHECK(uw_->sizes() == w_.sizes() && uw_->device() == h_.device(),
+                "linear cross entropy: uw must have the weight's shape and device");
+    uw = weight_rows(uw_->to(w_.scalar_type()));
+  }
+  at::Tensor gd = need_gdloss ? at::empty(dloss_.sizes(), dloss.options()) : at::empty({0}, dloss.options());
+  at::Tensor gh = need_gh ? at::empty(h_.sizes(), h_.options()) : at::empty({0}, h_.options());
+  at::Tensor gw = need_gw ? at::empty(w_.sizes(), w_.options()) : at::empty({0}, w_.options());
+  at::Tensor work = lce_work(pb, 2, h_);
+  ttt_lce_bwd2_args a{};
+  a.pb = pb;
+  a.h = h.numel() > 0 ? h.data_ptr() : nullptr;
+  a.h_stride = h.stride(0);
+  a.w = w.data_ptr();
+  a.w_stride = w.stride(0);
+  a.uh = uh.defined() && pb.n > 0 ? uh.data_ptr() : nullptr;
+  a.uh_stride = uh.defined() ? uh.stride(0) : 0;
+  a.uw = uw.defined() ? uw.data_ptr() : nullptr;
+  a.uw_stride = uw.defined() ? uw.stride(0) : 0;
+  a.state = state.data_ptr();
+  a.dloss = pb.n > 0 || reduction != TTT_LCE_NONE ? dloss.data_ptr<float>() : reinterpret_cast<float*>(word.data_ptr());
+  a.gh = need_gh && pb.n > 0 ? gh.data_ptr() : nullptr;
+  a.gw = need_gw ? gw.data_ptr() : nullptr;
+  a.gdloss = need_gdloss && gd.numel() > 0 ? gd.data_ptr<float>() : nullptr;
+  a.err = word.data_ptr<int32_t>();
+  a.work = ptr(work);
+  a.work_bytes = work.defined() ? work.numel() : 0;
+  check(ttt_lce_bwd2(&a, stream()), "ttt::linear_ce_bwd2");
+  return {gd, gh, gw};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(ttt, m) {
@@ -199,10 +371,20 @@ TORCH_LIBRARY_FRAGMENT(ttt, m) {
         "bool need_db, ScalarType p_type) -> (Tensor dx, Tensor dw, Tensor db)");
   m.def("layer_norm_bwd2(Tensor dy, Tensor x, Tensor? w, Tensor mean, Tensor rstd, Tensor? ux, Tensor? uw, "
         "Tensor? ub) -> (Tensor gdy, Tensor gx, Tensor gw)");
+  // reduction: 0 none, 1 mean, 2 sum; state (bytes) is what the gradients need of the forward.
+  m.def("linear_ce(Tensor h, Tensor w, Tensor targets, Tensor? mask, int reduction, int ignore_index) -> "
+        "(Tensor loss, Tensor state)");
+  m.def("linear_ce_bwd(Tensor dloss, Tensor h, Tensor w, Tensor state, int reduction, bool need_dh, bool need_dw) -> "
+        "(Tensor dh, Tensor dw)");
+  m.def("linear_ce_bwd2(Tensor dloss, Tensor h, Tensor w, Tensor state, int reduction, Tensor? uh, Tensor? uw, "
+        "bool need_gdloss, bool need_gh, bool need_gw) -> (Tensor gdloss, Tensor gh, Tensor gw)");
 }
 
 TORCH_LIBRARY_IMPL(ttt, CUDA, m) {
   m.impl("layer_norm", &op_layer_norm);
   m.impl("layer_norm_bwd", &op_layer_norm_bwd);
   m.impl("layer_norm_bwd2", &op_layer_norm_bwd2);
+  m.impl("linear_ce", &op_linear_ce);
+  m.impl("linear_ce_bwd", &op_linear_ce_bwd);
+  m.impl("linear_ce_bwd2", &op_linear_ce_bwd2);
 }

@@ -25,7 +25,7 @@
 #include <tuple>
 
 #include "torch_common.h"
-#include "ttt_attn.h"
+#include "ttt_ops.h"
 
 namespace {
 
@@ -63,6 +63,9 @@ void raise_if_pending(int dev, at::Tensor& word) {
   word.zero_();
   char hex[16];
   std::snprintf(hex, sizeof(hex), "0x%08x", static_cast<unsigned>(code));
+  TORCH_CHECK((code & TTT_ERR_WORD_TARGET) == 0, "libttt_attn: a linear cross entropy on cuda:", dev,
+              " met a target outside the vocabulary (error word ", hex, ", row ", code & 0xffffff,
+              "); results of the calls since then are invalid");
   TORCH_CHECK(false, "libttt_attn kernel gave up on a bounded wait on cuda:", dev, " (error word ", hex,
               "); results of the calls since then are invalid");
 }

@@ -115,3 +115,96 @@ class LayerNorm(nn.LayerNorm):
         if len(self.normalized_shape) != 1:
             raise ValueError(f"LayerNorm normalizes one dimension, got {self.normalized_shape}")
         return layer_norm(x, self.weight, self.bias, self.eps)
+
+
+# ---------------------------------------------------------------- linear cross entropy
+class _LinearCEBwdFn(torch.autograd.Function):
+    """The gradient as a differentiable op: (dloss, h, w) -> (dh, dw)."""
+
+    @staticmethod
+    def forward(ctx, dloss, h, w, state, reduction, need):
+        dh, dw = _lib.linear_ce_bwd(dloss, h, w, state, reduction, need)
+        ctx.save_for_backward(dloss, h, w, state)
+        ctx.reduction = reduction
+        ctx.set_materialize_grads(False)
+        return dh, dw
+
+    @staticmethod
+    def backward(ctx, uh, uw):
+        dloss, h, w, state = ctx.saved_tensors
+        if uh is None and uw is None:
+            return (None,) * 6
+        need = tuple(ctx.needs_input_grad[:3])
+        with torch.no_grad():
+            grads = _lib.linear_ce_bwd2(dloss, h, w, state, ctx.reduction, uh, uw, need)
+            grads = tuple(g if n else None for g, n in zip(grads, need))
+        return (*_last(grads, (dloss, h, w, uh, uw)), None, None, None)
+
+
+class LinearCrossEntropyFn(torch.autograd.Function):
+    """apply(h, w, targets, mask, reduction, ignore_index): see linear_cross_entropy."""
+
+    @staticmethod
+    def forward(ctx, h, w, targets, mask, reduction: str, ignore_index: int):
+        loss, state = _lib.linear_ce(h, w, targets, mask, reduction, ignore_index)
+        ctx.save_for_backward(h, w, state)
+        ctx.reduction = reduction
+        ctx.set_materialize_grads(False)
+        return loss
+
+    @staticmethod
+    def backward(ctx, dloss):
+        if dloss is None:
+            return (None,) * 6
+        h, w, state = ctx.saved_tensors
+        need = tuple(ctx.needs_input_grad[:2])
+        fn = _LinearCEBwdFn.apply if torch.is_grad_enabled() else _lib.linear_ce_bwd
+        dh, dw = fn(dloss, h, w, state, ctx.reduction, need)
+        return (dh if need[0] else None, dw if need[1] else None, None, None, None, None)
+
+
+def _linear_ce_math(h, w, targets, mask, reduction, ignore_index):
+    """The same value in PyTorch (CPU tensors)."""
+    weight = torch.ones_like(targets, dtype=h.dtype) if mask is None else mask.to(h.dtype)
+    keep = (weight != 0) & (targets != ignore_index)
+    if bool(((targets < 0) | (targets >= w.shape[0]))[keep].any()):
+        raise ValueError(f"linear cross entropy: a target is outside the vocabulary of {w.shape[0]}")
+    h = torch.where(keep[..., None], h, torch.zeros((), dtype=h.dtype, device=h.device))
+    t = torch.where(keep, targets, torch.zeros_like(targets))
+    z = torch.matmul(h, w.transpose(0, 1))
+    ce = torch.logsumexp(z, -1) - z.gather(-1, t[..., None])[..., 0]
+    ce = torch.where(keep, ce * weight, torch.zeros_like(ce))
+    if reduction == "none":
+        return ce
+    if reduction == "sum":
+        return ce.sum()
+    return ce.sum() / (max(targets.numel(), 1) if mask is None else weight.sum().clamp_min(1.0))
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                         mask: Optional[torch.Tensor] = None, *, reduction: str = "mean",
+                         ignore_index: int = -100) -> torch.Tensor:
+    """Token cross entropy of the logits ``hidden @ weight.T``, which are never stored.
+
+    hidden: [..., dim]; weight: [vocab, dim] (both fp16 or both bf16 on CUDA);
+    targets: integers, hidden's leading shape; mask: the targets' shape, bool or
+    weights m (a position with m = 0 is left out). The position's loss is m times
+    its cross entropy, 0 where the target is ``ignore_index``; the result is fp32
+    (on CPU hidden's dtype):
+
+    * "none": the positions' losses;  * "sum": their sum;
+    * "mean": their sum over max(1, sum of the mask), or over the number of
+      positions without a mask, as ``ttt_model.compute_loss`` divides (ignored
+      targets count). A loss over no position at all is 0.
+
+    Positions left out are not read: what ``hidden`` holds there changes nothing,
+    and their gradient is exactly 0. A target outside the vocabulary raises: at
+    once on CPU, at the next call of this library (or check_device_errors) on
+    CUDA. Differentiable twice in hidden, weight and the upstream gradient."""
+    if reduction not in _lib.LCE_REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_lib.LCE_REDUCTIONS)}, got {reduction!r}")
+    if not _kernel_path(hidden):
+        return _linear_ce_math(hidden, weight, targets, mask, reduction, ignore_index)
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return LinearCrossEntropyFn.apply(hidden, weight, targets, mask, reduction, int(ignore_index))
+    return _lib.linear_ce(hidden, weight, targets, mask, reduction, int(ignore_index))[0]
