@@ -536,22 +536,13 @@ def attn_bwd2_noalloc(q, k, v, dout, lse2, delta, uq, uk, uv, causal: bool, scal
 
 
 # ---------------------------------------------------------------- layer norm (include/ttt_ops.h)
-def layer_norm(x, w, b, eps: float, need_stats: bool):
-    """y, mean, rstd (fp32 [rows]; empty unless need_stats) over rows of x's last dimension."""
+def layer_norm_ad(x, w, b, eps: float):
+    """Layer norm over rows of x's last dimension, differentiable twice (ttt::layer_norm and its gradients)."""
     load_torch_ops()
-    return _op(torch.ops.ttt.layer_norm, x, w, b, eps, need_stats)
-
-
-def layer_norm_bwd(dy, x, w, mean, rstd, need, p_type):
-    """dx, dw, db; need = (dx, dw, db) wanted (an output that is not is empty)."""
-    load_torch_ops()
-    return _op(torch.ops.ttt.layer_norm_bwd, dy, x, w, mean, rstd, *map(bool, need), p_type)
-
-
-def layer_norm_bwd2(dy, x, w, mean, rstd, ux, uw, ub):
-    """Gradients (gdy, gx, gw) of <dx, ux> + <dw, uw> + <db, ub>; a probe given as None is zero."""
-    load_torch_ops()
-    return _op(torch.ops.ttt.layer_norm_bwd2, dy, x, w, mean, rstd, ux, uw, ub)
+    y = _op(torch.ops.ttt.layer_norm_ad.default, x, w, b, eps)
+    if _SYNC_CHECK:
+        check_device_errors(x.device)
+    return y
 
 
 # ---------------------------------------------------------------- linear cross entropy (include/ttt_ops.h)
@@ -564,32 +555,14 @@ def _lce_state_bytes(n: int) -> int:
     return 256 + 4 * up((n + 127) // 128 * 128 * 4) + up(n * 4)
 
 
-def linear_ce(h, w, targets, mask, reduction: str, ignore_index: int):
-    """loss (fp32; targets' shape for "none", else a scalar) and the state of the gradients."""
+def linear_ce_ad(h, w, targets, mask, reduction: str, ignore_index: int):
+    """The linear cross entropy, differentiable twice (ttt::linear_ce and its gradients):
+    fp32, targets' shape for "none", else a scalar."""
     load_torch_ops()
-    loss, state = _op(torch.ops.ttt.linear_ce, h, w, targets, mask, LCE_REDUCTIONS[reduction], ignore_index)
+    loss = _op(torch.ops.ttt.linear_ce_ad.default, h, w, targets, mask, LCE_REDUCTIONS[reduction], ignore_index)
     if _SYNC_CHECK:
         check_device_errors(h.device)
-    return loss, state
-
-
-def linear_ce_bwd(dloss, h, w, state, reduction: str, need):
-    """dh, dw; need = (dh, dw) wanted (an output that is not is empty)."""
-    load_torch_ops()
-    out = _op(torch.ops.ttt.linear_ce_bwd, dloss, h, w, state, LCE_REDUCTIONS[reduction], *map(bool, need))
-    if _SYNC_CHECK:
-        check_device_errors(h.device)
-    return out
-
-
-def linear_ce_bwd2(dloss, h, w, state, reduction: str, uh, uw, need):
-    """Gradients (gdloss, gh, gw) of <dh, uh> + <dw, uw>; a probe given as None is zero,
-    need = (gdloss, gh, gw) wanted."""
-    load_torch_ops()
-    out = _op(torch.ops.ttt.linear_ce_bwd2, dloss, h, w, state, LCE_REDUCTIONS[reduction], uh, uw, *map(bool, need))
-    if _SYNC_CHECK:
-        check_device_errors(h.device)
-    return out
+    return loss
 
 
 # ---------------------------------------------------------------- passes over materialized P

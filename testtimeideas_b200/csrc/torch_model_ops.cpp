@@ -2,9 +2,16 @@
 // (forward, gradient and gradient of the gradient). Like torch_ops.cpp: argument checks, output
 // and work space allocation (PyTorch's caching allocator, on the current device
 // and stream) and the call into the C ABI.
+//
+// ttt::layer_norm_ad and ttt::linear_ce_ad are what the public functions call:
+// autograd Functions over those operators, in C++ because the norms' kernels take
+// a few microseconds and Python Functions cost about 30 us a node. The backward of
+// each is itself a Function with a closed-form backward, as the attention's is,
+// and computes only the gradients that the running backward asks for.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <optional>
@@ -360,6 +367,204 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_linear_ce_bwd2(const at::Tenso
   return {gd, gh, gw};
 }
 
+// ---------------------------------------------------------------- autograd
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+at::Tensor defined_or(const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); }
+OptTensor opt(const at::Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
+template <class Sig>
+auto raw_op(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
+}
+auto& raw_layer_norm() {
+  static auto op = raw_op<decltype(op_layer_norm)>("ttt::layer_norm");
+  return op;
+}
+auto& raw_layer_norm_bwd() {
+  static auto op = raw_op<decltype(op_layer_norm_bwd)>("ttt::layer_norm_bwd");
+  return op;
+}
+auto& raw_layer_norm_bwd2() {
+  static auto op = raw_op<decltype(op_layer_norm_bwd2)>("ttt::layer_norm_bwd2");
+  return op;
+}
+auto& raw_linear_ce() {
+  static auto op = raw_op<decltype(op_linear_ce)>("ttt::linear_ce");
+  return op;
+}
+auto& raw_linear_ce_bwd() {
+  static auto op = raw_op<decltype(op_linear_ce_bwd)>("ttt::linear_ce_bwd");
+  return op;
+}
+auto& raw_linear_ce_bwd2() {
+  static auto op = raw_op<decltype(op_linear_ce_bwd2)>("ttt::linear_ce_bwd2");
+  return op;
+}
+
+// An output of a second gradient, tied to the tensors it was computed from by a
+// backward that raises, so that a third derivative is refused rather than wrong.
+struct LastFn : torch::autograd::Function<LastFn> {
+  static at::Tensor forward(AutogradContext*, const at::Tensor& out, const OptTensor&, const OptTensor&,
+                            const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&) {
+    return out.view_as(out);
+  }
+  static variable_list backward(AutogradContext*, const variable_list&) {
+    TORCH_CHECK(false, "the second gradient of this op is not differentiable (a third derivative was requested)");
+  }
+};
+// Marks the defined ones of `outs`, in place; up to six inputs, any of them undefined.
+void mark_last(variable_list& outs, variable_list inputs) {
+  if (!at::GradMode::is_enabled()) return;
+  inputs.resize(6);
+  for (at::Tensor& o : outs)
+    if (o.defined())
+      o = LastFn::apply(o, opt(inputs[0]), opt(inputs[1]), opt(inputs[2]), opt(inputs[3]), opt(inputs[4]),
+                        opt(inputs[5]));
+}
+
+// (dy, x, w) -> (dx, dw, db); `need` has a bit per output.
+struct LayerNormBwdFn : torch::autograd::Function<LayerNormBwdFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& dy, const at::Tensor& x, const OptTensor& w,
+                               const at::Tensor& mean, const at::Tensor& rstd, int64_t need, int64_t p_type) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({dy, x, defined_or(w), mean, rstd});
+    ctx->set_materialize_grads(false);
+    auto [dx, dw, db] = raw_layer_norm_bwd().call(dy, x, w, mean, rstd, (need & 1) != 0, (need & 2) != 0,
+                                                  (need & 4) != 0, static_cast<at::ScalarType>(p_type));
+    return {dx, dw, db};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& up) {
+    const variable_list v = ctx->get_saved_variables();
+    variable_list g(7);
+    if (!up[0].defined() && !up[1].defined() && !up[2].defined()) return g;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(g[0], g[1], g[2]) =
+          raw_layer_norm_bwd2().call(v[0], v[1], opt(v[2]), v[3], v[4], opt(up[0]), opt(up[1]), opt(up[2]));
+      g[0] = g[0].to(v[0].scalar_type());
+      if (!v[2].defined()) g[2] = at::Tensor();
+    }
+    mark_last(g, {v[0], v[1], v[2], up[0], up[1], up[2]});
+    return g;
+  }
+};
+
+struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& w, const OptTensor& b,
+                            double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, mean, rstd] = raw_layer_norm().call(x, w, b, eps, true);
+    ctx->save_for_backward({x, defined_or(w), mean, rstd});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["p_type"] = static_cast<int64_t>((w.has_value() ? *w : (b.has_value() ? *b : x)).scalar_type());
+    ctx->saved_data["has_b"] = b.has_value();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& up) {
+    variable_list g(4);
+    if (!up[0].defined()) return g;
+    const variable_list v = ctx->get_saved_variables();
+    const int64_t p_type = ctx->saved_data["p_type"].toInt();
+    // needs_input_grad counts the tensors that were given: x, then w and b where present
+    const bool has_w = v[1].defined(), has_b = ctx->saved_data["has_b"].toBool();
+    int64_t need = ctx->needs_input_grad(0) ? 1 : 0;
+    if (has_w && ctx->needs_input_grad(1)) need |= 2;
+    if (has_b && ctx->needs_input_grad(has_w ? 2 : 1)) need |= 4;
+    variable_list out;
+    if (at::GradMode::is_enabled()) {
+      out = LayerNormBwdFn::apply(up[0], v[0], opt(v[1]), v[2], v[3], need, p_type);
+    } else {
+      auto [dx, dw, db] = raw_layer_norm_bwd().call(up[0], v[0], opt(v[1]), v[2], v[3], (need & 1) != 0,
+                                                    (need & 2) != 0, (need & 4) != 0,
+                                                    static_cast<at::ScalarType>(p_type));
+      out = {dx, dw, db};
+    }
+    for (int i = 0; i < 3; ++i)
+      if (need & (1 << i)) g[i] = out[i];
+    return g;
+  }
+};
+
+bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+at::Tensor op_layer_norm_ad(const at::Tensor& x, const OptTensor& w_, const OptTensor& b_, double eps) {
+  const at::Tensor w = defined_or(w_), b = defined_or(b_);
+  if (wants_grad({&x, &w, &b})) return LayerNormFn::apply(x, w_, b_, eps);
+  return std::get<0>(raw_layer_norm().call(x, w_, b_, eps, false));
+}
+
+// (dloss, h, w) -> (dh, dw); `need` has a bit per output.
+struct LinearCEBwdFn : torch::autograd::Function<LinearCEBwdFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& dloss, const at::Tensor& h, const at::Tensor& w,
+                               const at::Tensor& state, int64_t reduction, int64_t need) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({dloss, h, w, state});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["reduction"] = reduction;
+    auto [dh, dw] = raw_linear_ce_bwd().call(dloss, h, w, state, reduction, (need & 1) != 0, (need & 2) != 0);
+    return {dh, dw};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& up) {
+    const variable_list v = ctx->get_saved_variables();
+    variable_list g(6);
+    if (!up[0].defined() && !up[1].defined()) return g;
+    bool need[3];
+    for (int i = 0; i < 3; ++i) need[i] = ctx->needs_input_grad(i);
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(g[0], g[1], g[2]) = raw_linear_ce_bwd2().call(v[0], v[1], v[2], v[3],
+                                                             ctx->saved_data["reduction"].toInt(), opt(up[0]),
+                                                             opt(up[1]), need[0], need[1], need[2]);
+      for (int i = 0; i < 3; ++i)
+        if (!need[i]) g[i] = at::Tensor();
+    }
+    mark_last(g, {v[0], v[1], v[2], up[0], up[1]});
+    return g;
+  }
+};
+
+struct LinearCEFn : torch::autograd::Function<LinearCEFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& targets,
+                            const OptTensor& mask, int64_t reduction, int64_t ignore_index) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [loss, state] = raw_linear_ce().call(h, w, targets, mask, reduction, ignore_index);
+    ctx->save_for_backward({h, w, state});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["reduction"] = reduction;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& up) {
+    variable_list g(6);
+    if (!up[0].defined()) return g;
+    const variable_list v = ctx->get_saved_variables();
+    const int64_t reduction = ctx->saved_data["reduction"].toInt();
+    const int64_t need = (ctx->needs_input_grad(0) ? 1 : 0) | (ctx->needs_input_grad(1) ? 2 : 0);
+    variable_list out;
+    if (at::GradMode::is_enabled()) {
+      out = LinearCEBwdFn::apply(up[0], v[0], v[1], v[2], reduction, need);
+    } else {
+      auto [dh, dw] = raw_linear_ce_bwd().call(up[0], v[0], v[1], v[2], reduction, (need & 1) != 0, (need & 2) != 0);
+      out = {dh, dw};
+    }
+    for (int i = 0; i < 2; ++i)
+      if (need & (1 << i)) g[i] = out[i];
+    return g;
+  }
+};
+
+at::Tensor op_linear_ce_ad(const at::Tensor& h, const at::Tensor& w, const at::Tensor& targets, const OptTensor& mask,
+                           int64_t reduction, int64_t ignore_index) {
+  if (wants_grad({&h, &w})) return LinearCEFn::apply(h, w, targets, mask, reduction, ignore_index);
+  return std::get<0>(raw_linear_ce().call(h, w, targets, mask, reduction, ignore_index));
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(ttt, m) {
@@ -378,6 +583,17 @@ TORCH_LIBRARY_FRAGMENT(ttt, m) {
         "(Tensor dh, Tensor dw)");
   m.def("linear_ce_bwd2(Tensor dloss, Tensor h, Tensor w, Tensor state, int reduction, Tensor? uh, Tensor? uw, "
         "bool need_gdloss, bool need_gh, bool need_gw) -> (Tensor gdloss, Tensor gh, Tensor gw)");
+}
+
+TORCH_LIBRARY_FRAGMENT(ttt, m) {
+  // Differentiable (twice) forms of layer_norm and linear_ce.
+  m.def("layer_norm_ad(Tensor x, Tensor? w, Tensor? b, float eps) -> Tensor");
+  m.def("linear_ce_ad(Tensor h, Tensor w, Tensor targets, Tensor? mask, int reduction, int ignore_index) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(ttt, CompositeImplicitAutograd, m) {
+  m.impl("layer_norm_ad", &op_layer_norm_ad);
+  m.impl("linear_ce_ad", &op_linear_ce_ad);
 }
 
 TORCH_LIBRARY_IMPL(ttt, CUDA, m) {
