@@ -13,26 +13,27 @@
 // (the last term and the sign of the one before it come from dr/dx = -r^2 xh / D).
 //
 // All three are bound by memory: 2, 3 and 5 passes over [rows, D]. A row is read
-// once and stays in the registers of the NT threads that own it (a warp up to
-// 1024 elements, a block of 128 or 512 threads above), so mean and variance are
-// two sums over registers, and no statistic is a difference of large sums. The
-// threads of a row own fixed columns, so the parameter gradients are summed in
-// registers over all rows that a block meets; the blocks' sums (fp32) are added
-// in block order by a second small kernel. Everything is computed in fp32 and
-// rounded once on the way out.
+// once and stays, packed as it came, in the registers of the NT threads that own
+// it: eight elements each up to 2048 (16 to 32 above), so that a thread needs few
+// registers and an SM holds enough rows in flight to cover the memory's latency
+// (32 elements a thread took 170 registers and ran at a quarter of the bandwidth).
+// Mean and variance are two sums over registers, and no statistic is a difference
+// of large sums. The threads of a row own fixed columns, so the parameter gradients
+// are summed in registers over all rows that a block meets; the blocks' sums (fp32)
+// are added in block order by a second small kernel, launched ahead of the first
+// one's end. Everything is computed in fp32 and rounded once on the way out.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "ttt_ops.h"
 
 namespace {
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <class T>
 __device__ __forceinline__ T from_f(float v);
 template <>
@@ -48,103 +49,154 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// N consecutive elements starting at p; N * sizeof(T) is 16 bytes or a multiple
-// of it (then p is 16-byte aligned), or N is 1.
-template <class T, int N>
-__device__ __forceinline__ void load_n(const T* p, float* v) {
-  if constexpr (N == 1) {
-    v[0] = to_f(*p);
-  } else {
-    constexpr int PER = 16 / sizeof(T);
-    static_assert(N % PER == 0, "whole 16-byte pieces");
-#pragma unroll
-    for (int q = 0; q < N / PER; ++q) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p + q * PER);
-      T e[PER];
-      *reinterpret_cast<uint4*>(e) = u;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) v[q * PER + j] = to_f(e[j]);
+// EPT elements of a row as they lie in memory, two 16-bit elements to a register.
+template <class T, int EPT>
+struct Pack {
+  uint32_t w[EPT / 2];
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      return __uint_as_float((i & 1) ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16));
+    } else {
+      return __half2float(__ushort_as_half(static_cast<unsigned short>((i & 1) ? w[i >> 1] >> 16 : w[i >> 1])));
     }
   }
-}
-template <class T, int N>
-__device__ __forceinline__ void store_n(T* p, const float* v) {
-  if constexpr (N == 1) {
-    *p = from_f<T>(v[0]);
-  } else {
-    constexpr int PER = 16 / sizeof(T);
-    static_assert(N % PER == 0, "whole 16-byte pieces");
-#pragma unroll
-    for (int q = 0; q < N / PER; ++q) {
-      __align__(16) T e[PER];
-#pragma unroll
-      for (int j = 0; j < PER; ++j) e[j] = from_f<T>(v[q * PER + j]);
-      *reinterpret_cast<uint4*>(p + q * PER) = *reinterpret_cast<const uint4*>(e);
+  // Elements i (even) and i + 1.
+  __device__ __forceinline__ void set2(int i, float lo, float hi) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+      w[i >> 1] = *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+      const __half2 v = __floats2half2_rn(lo, hi);
+      w[i >> 1] = *reinterpret_cast<const uint32_t*>(&v);
     }
   }
+  __device__ __forceinline__ void set_bits(int i, uint32_t bits) {
+    w[i >> 1] = (i & 1) ? (w[i >> 1] & 0xffffu) | (bits << 16) : bits;
+  }
+  __device__ __forceinline__ uint32_t bits(int i) const { return (i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu; }
+};
+template <int EPT>
+struct Pack<float, EPT> {
+  uint32_t w[EPT];
+  __device__ __forceinline__ float at(int i) const { return __uint_as_float(w[i]); }
+  __device__ __forceinline__ void set2(int i, float lo, float hi) {
+    w[i] = __float_as_uint(lo);
+    w[i + 1] = __float_as_uint(hi);
+  }
+  __device__ __forceinline__ void set_bits(int i, uint32_t bits) { w[i] = bits; }
+  __device__ __forceinline__ uint32_t bits(int i) const { return w[i]; }
+};
+
+// Keeps a row packed across a reduction: without it the compiler carries the
+// unpacked (and centred) values over, at two to three times the registers.
+template <class T, int EPT>
+__device__ __forceinline__ void stay_packed(Pack<T, EPT>& v) {
+  for (auto& w : v.w) asm volatile("" : "+r"(w));
 }
 
-// The layout of a row: NT threads, each with K pieces of VEC elements; piece k
-// of thread t starts at column (k * NT + t) * VEC. VEC is 16 bytes of X, or 1
-// for rows that are not 16-byte aligned.
+// The layout of a row: NT threads, each with K pieces of VEC elements; piece k of
+// thread t starts at column (k * NT + t) * VEC. VEC is 16 bytes of X, or 1 for rows
+// that are not 16-byte aligned. A block holds GROUPS rows at a time.
 template <class X, int NT_, int EPT_, bool WIDE>
 struct Row {
   static constexpr int NT = NT_, EPT = EPT_;
   static constexpr int VEC = WIDE ? 16 / static_cast<int>(sizeof(X)) : 1;
   static constexpr int K = EPT / VEC;
-  // Threads of a block: eight rows (warps) per block for warp rows, else one row.
-  static constexpr int GROUPS = NT == 32 ? 8 : 1;
-  static constexpr int THREADS = NT * GROUPS;
+  static constexpr int THREADS = NT > 256 ? NT : 256, GROUPS = THREADS / NT;
+  // Blocks that an SM holds: 64 registers a thread in the forward, 80 in the gradient of
+  // eight 16-bit elements, else 128.
+  static constexpr int FWD_PER_SM = 1024 / THREADS;
+  static constexpr int BWD_PER_SM = EPT == 8 && sizeof(X) == 2 ? 3 : 512 / THREADS;
+  static constexpr int BWD2_PER_SM = 512 / THREADS;
 
+  static __device__ __forceinline__ int column(int k, int t) { return (k * NT + t) * VEC; }
+  static __device__ __forceinline__ bool inside(int i, int t, int D) { return column(i / VEC, t) < D; }
+
+  // Elements outside the row (or a null row) are `fill`.
   template <class T>
-  static __device__ __forceinline__ void load(const T* row, int t, int D, float (&v)[EPT], float fill = 0.f) {
+  static __device__ __forceinline__ void load(const T* row, int t, int D, Pack<T, EPT>& v, float fill = 0.f) {
+    constexpr int WORDS = VEC * static_cast<int>(sizeof(T)) / 4;  // of a piece; T may be wider than X
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = (k * NT + t) * VEC;
-      if (row != nullptr && c < D) {
-        load_n<T, VEC>(row + c, v + k * VEC);
+      const int c = column(k, t);
+      const bool in = row != nullptr && c < D;
+      if constexpr (VEC == 1) {
+        T e = from_f<T>(fill);
+        if (in) e = row[c];
+        if constexpr (sizeof(T) == 4)
+          v.set_bits(k, *reinterpret_cast<const uint32_t*>(&e));
+        else
+          v.set_bits(k, *reinterpret_cast<const uint16_t*>(&e));
+      } else if (in) {
+#pragma unroll
+        for (int q = 0; q < WORDS / 4; ++q) {
+          const uint4 u = reinterpret_cast<const uint4*>(row + c)[q];
+          uint32_t* w = v.w + k * WORDS + q * 4;
+          w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[k * VEC + j] = fill;
+        for (int j = 0; j < VEC; j += 2) v.set2(k * VEC + j, fill, fill);
       }
     }
   }
   template <class T>
-  static __device__ __forceinline__ void store(T* row, int t, int D, const float (&v)[EPT]) {
+  static __device__ __forceinline__ void store(T* row, int t, int D, const Pack<T, EPT>& v) {
+    constexpr int WORDS = VEC * static_cast<int>(sizeof(T)) / 4;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = (k * NT + t) * VEC;
-      if (c < D) store_n<T, VEC>(row + c, v + k * VEC);
+      const int c = column(k, t);
+      if (c >= D) continue;
+      if constexpr (VEC == 1) {
+        if constexpr (sizeof(T) == 4)
+          reinterpret_cast<uint32_t*>(row)[c] = v.bits(k);
+        else
+          reinterpret_cast<uint16_t*>(row)[c] = static_cast<uint16_t>(v.bits(k));
+      } else {
+#pragma unroll
+        for (int q = 0; q < WORDS / 4; ++q) {
+          const uint32_t* w = v.w + k * WORDS + q * 4;
+          reinterpret_cast<uint4*>(row + c)[q] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
     }
   }
-  static __device__ __forceinline__ bool inside(int i, int t, int D) { return ((i / VEC) * NT + t) * VEC < D; }
 };
 
-// Sums of N values over the NT threads of a row, returned to all of them. Block
-// rows go through shared memory; `red` holds 2 * N * NT/32 floats, and `phase`
-// alternates its halves so that one barrier per reduction is enough.
-template <int NT, int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float* red, int& phase) {
+// Sums of N values over the NT threads of a row, returned to all of them. Rows of
+// several warps go through shared memory and a barrier of their own; `phase`
+// alternates between two halves of the buffer so that one barrier is enough.
+constexpr int kMaxSums = 6;
+template <class R>
+struct Sums {
+  static constexpr int W = R::NT / 32;
+  float red[R::GROUPS][2][kMaxSums][W];
+};
+template <class R, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], Sums<R>& sums, int& phase) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   }
-  if constexpr (NT > 32) {
-    constexpr int W = NT / 32;
-    float* buf = red + phase * 8 * W;
+  if constexpr (R::NT > 32) {
+    constexpr int W = R::NT / 32;
+    const int grp = threadIdx.x / R::NT, warp = (threadIdx.x % R::NT) >> 5;
+    auto& buf = sums.red[grp][phase];
     phase ^= 1;
-    const int warp = threadIdx.x >> 5;
     if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) buf[i * W + warp] = v[i];
+      for (int i = 0; i < N; ++i) buf[i][warp] = v[i];
     }
-    __syncthreads();
+    if constexpr (R::GROUPS == 1)
+      __syncthreads();
+    else
+      asm volatile("bar.sync %0, %1;" ::"r"(grp + 1), "n"(R::NT) : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < W; ++w) s += buf[i * W + w];
+      for (int w = 0; w < W; ++w) s += buf[i][w];
       v[i] = s;
     }
   }
@@ -165,176 +217,219 @@ struct NormArgs {
 };
 
 template <class X, class P, class R>
-__global__ void __launch_bounds__(R::THREADS) norm_fwd_kernel(const NormArgs<X, P> a) {
+__global__ void __launch_bounds__(R::THREADS, R::FWD_PER_SM) norm_fwd_kernel(const NormArgs<X, P> a) {
   constexpr int EPT = R::EPT;
-  __shared__ float red[R::NT > 32 ? 16 * (R::NT / 32) : 1];
+  __shared__ Sums<R> sums;
   int phase = 0;
   const int t = threadIdx.x % R::NT;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * R::GROUPS + threadIdx.x / R::NT;
-  if (row >= a.rows) return;  // whole warps (warp rows) or no thread at all (block rows)
   const float inv = 1.f / static_cast<float>(a.D);
-  float x[EPT];
-  R::load(a.x + row * a.x_stride, t, a.D, x);
-  float s[1] = {0.f};
-#pragma unroll
-  for (int i = 0; i < EPT; ++i) s[0] += x[i];
-  row_sum<R::NT, 1>(s, red, phase);
-  const float mu = s[0] * inv;
-  float q[1] = {0.f};
-#pragma unroll
-  for (int i = 0; i < EPT; ++i) {
-    x[i] -= mu;
-    q[0] += R::inside(i, t, a.D) ? x[i] * x[i] : 0.f;
-  }
-  row_sum<R::NT, 1>(q, red, phase);
-  const float r = rsqrtf(q[0] * inv + a.eps);
-  float w[EPT], b[EPT];
+  const int64_t step = static_cast<int64_t>(gridDim.x) * R::GROUPS;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * R::GROUPS + threadIdx.x / R::NT;
+  if (row >= a.rows) return;  // whole groups, which have their own barriers
+  Pack<X, EPT> xn;  // the next row, loaded while this one is summed
+  R::load(a.x + row * a.x_stride, t, a.D, xn);
+  Pack<P, EPT> w, b;
   R::load(a.w, t, a.D, w, 1.f);
   R::load(a.b, t, a.D, b, 0.f);
+  for (; row < a.rows; row += step) {
+    Pack<X, EPT> x = xn;
+    if (row + step < a.rows) R::load(a.x + (row + step) * a.x_stride, t, a.D, xn);
+    float s[1] = {0.f};
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) x[i] = x[i] * r * w[i] + b[i];
-  R::store(a.y + row * a.D, t, a.D, x);
-  if (t == 0 && a.mean != nullptr) {
-    a.mean[row] = mu;
-    a.rstd[row] = r;
+    for (int i = 0; i < EPT; ++i) s[0] += x.at(i);
+    row_sum<R, 1>(s, sums, phase);
+    const float mu = s[0] * inv;
+    float q[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const float c = x.at(i) - mu;
+      q[0] += R::inside(i, t, a.D) ? c * c : 0.f;
+    }
+    row_sum<R, 1>(q, sums, phase);
+    const float r = rsqrtf(q[0] * inv + a.eps);
+#pragma unroll
+    for (int i = 0; i < EPT; i += 2)
+      x.set2(i, (x.at(i) - mu) * r * w.at(i) + b.at(i), (x.at(i + 1) - mu) * r * w.at(i + 1) + b.at(i + 1));
+    R::store(a.y + row * a.D, t, a.D, x);
+    if (t == 0 && a.mean != nullptr) {
+      a.mean[row] = mu;
+      a.rstd[row] = r;
+    }
   }
 }
 
 // Adds the row groups' column sums of a block and writes them to
 // part[block][which]; acc holds this thread's columns.
 template <class R>
-__device__ __forceinline__ void write_part(float* part, int which, int D, const float (&acc)[R::EPT], float* sums) {
+__device__ __forceinline__ void write_part(float* part, int which, int D, const float (&acc)[R::EPT], float* cols) {
   const int t = threadIdx.x % R::NT;
   float* dst = part + (static_cast<int64_t>(blockIdx.x) * 2 + which) * D;
   if constexpr (R::GROUPS == 1) {
-    R::store(dst, t, D, acc);
+#pragma unroll
+    for (int i = 0; i < R::EPT; ++i) {
+      const int c = R::column(i / R::VEC, t) + i % R::VEC;
+      if (c < D) dst[c] = acc[i];
+    }
   } else {
     const int grp = threadIdx.x / R::NT;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < R::EPT; ++i) {
-      const int c = ((i / R::VEC) * R::NT + t) * R::VEC + i % R::VEC;
-      if (c < D) sums[grp * D + c] = acc[i];
+      const int c = R::column(i / R::VEC, t) + i % R::VEC;
+      if (c < D) cols[grp * D + c] = acc[i];
     }
     __syncthreads();
     for (int c = threadIdx.x; c < D; c += R::THREADS) {
       float s = 0.f;
 #pragma unroll
-      for (int gi = 0; gi < R::GROUPS; ++gi) s += sums[gi * D + c];
+      for (int gi = 0; gi < R::GROUPS; ++gi) s += cols[gi * D + c];
       dst[c] = s;
     }
   }
 }
 
 template <class X, class P, class R>
-__global__ void __launch_bounds__(R::THREADS) norm_bwd_kernel(const NormArgs<X, P> a) {
+__global__ void __launch_bounds__(R::THREADS, R::BWD_PER_SM) norm_bwd_kernel(const NormArgs<X, P> a) {
   constexpr int EPT = R::EPT;
-  extern __shared__ float sums[];
-  __shared__ float red[R::NT > 32 ? 16 * (R::NT / 32) : 1];
+  extern __shared__ float cols[];
+  __shared__ Sums<R> sums;
   int phase = 0;
+  asm volatile("griddepcontrol.launch_dependents;");  // the parameter sums wait for this grid's end
   const int t = threadIdx.x % R::NT;
   const float inv = 1.f / static_cast<float>(a.D);
   float aw[EPT], ab[EPT];
 #pragma unroll
   for (int i = 0; i < EPT; ++i) aw[i] = ab[i] = 0.f;
+  Pack<P, EPT> w;
+  R::load(a.w, t, a.D, w, 1.f);
   const int64_t step = static_cast<int64_t>(gridDim.x) * R::GROUPS;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * R::GROUPS + threadIdx.x / R::NT; row < a.rows; row += step) {
-    const float mu = a.mean[row], r = a.rstd[row];
-    float x[EPT], dy[EPT], w[EPT];
-    R::load(a.x + row * a.x_stride, t, a.D, x);
-    R::load(a.dy + row * a.dy_stride, t, a.D, dy);
-    R::load(a.w, t, a.D, w, 1.f);
+  int64_t row = static_cast<int64_t>(blockIdx.x) * R::GROUPS + threadIdx.x / R::NT;
+  Pack<X, EPT> xn, dn;  // the next row, loaded while this one is summed
+  float mun = 0.f, rn = 0.f;
+  auto fetch = [&](int64_t at) {
+    if (at >= a.rows) return;
+    R::load(a.x + at * a.x_stride, t, a.D, xn);
+    R::load(a.dy + at * a.dy_stride, t, a.D, dn);
+    mun = a.mean[at];
+    rn = a.rstd[at];
+  };
+  fetch(row);
+  for (; row < a.rows; row += step) {
+    Pack<X, EPT> x = xn, dy = dn;
+    const float mu = mun, r = rn;
+    fetch(row + step);
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-      x[i] = (x[i] - mu) * r;
-      aw[i] += dy[i] * x[i];
-      ab[i] += dy[i];
-      w[i] *= dy[i];  // g; zero outside the row, as dy is
-      s[0] += w[i];
-      s[1] += w[i] * x[i];
+      // dy is zero outside the row, so nothing else has to be
+      const float xh = (x.at(i) - mu) * r, d = dy.at(i), g = d * w.at(i);
+      aw[i] += d * xh;
+      ab[i] += d;
+      s[0] += g;
+      s[1] += g * xh;
     }
-    row_sum<R::NT, 2>(s, red, phase);
+    row_sum<R, 2>(s, sums, phase);
+    stay_packed(x);
+    stay_packed(dy);
+    stay_packed(w);
     if (a.dx != nullptr) {
       const float mg = s[0] * inv, ma = s[1] * inv;
 #pragma unroll
-      for (int i = 0; i < EPT; ++i) x[i] = r * (w[i] - mg - x[i] * ma);
+      for (int i = 0; i < EPT; i += 2)
+        x.set2(i, r * (dy.at(i) * w.at(i) - mg - (x.at(i) - mu) * r * ma),
+               r * (dy.at(i + 1) * w.at(i + 1) - mg - (x.at(i + 1) - mu) * r * ma));
       R::store(a.dx + row * a.D, t, a.D, x);
     }
   }
-  if (a.want_dw) write_part<R>(a.part, 0, a.D, aw, sums);
-  if (a.want_db) write_part<R>(a.part, 1, a.D, ab, sums);
+  if (a.want_dw) write_part<R>(a.part, 0, a.D, aw, cols);
+  if (a.want_db) write_part<R>(a.part, 1, a.D, ab, cols);
 }
 
 template <class X, class P, class R>
-__global__ void __launch_bounds__(R::THREADS) norm_bwd2_kernel(const NormArgs<X, P> a) {
+__global__ void __launch_bounds__(R::THREADS, R::BWD2_PER_SM) norm_bwd2_kernel(const NormArgs<X, P> a) {
   constexpr int EPT = R::EPT;
-  extern __shared__ float sums[];
-  __shared__ float red[R::NT > 32 ? 16 * (R::NT / 32) : 1];
+  extern __shared__ float cols[];
+  __shared__ Sums<R> sums;
   int phase = 0;
+  asm volatile("griddepcontrol.launch_dependents;");
   const int t = threadIdx.x % R::NT;
   const float inv = 1.f / static_cast<float>(a.D);
   float agw[EPT];
 #pragma unroll
   for (int i = 0; i < EPT; ++i) agw[i] = 0.f;
+  Pack<P, EPT> w, uw, ub;
+  R::load(a.w, t, a.D, w, 1.f);
+  R::load(a.uw, t, a.D, uw);
+  R::load(a.ub, t, a.D, ub);
   const int64_t step = static_cast<int64_t>(gridDim.x) * R::GROUPS;
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * R::GROUPS + threadIdx.x / R::NT; row < a.rows; row += step) {
     const float mu = a.mean[row], r = a.rstd[row];
-    float x[EPT], dy[EPT], u[EPT];
-    R::load(a.x + row * a.x_stride, t, a.D, x, mu);  // xh is zero outside the row
+    Pack<X, EPT> x, dy, u;
+    R::load(a.x + row * a.x_stride, t, a.D, x);
     R::load(a.dy + row * a.dy_stride, t, a.D, dy);
     R::load(a.ux == nullptr ? nullptr : a.ux + row * a.ux_stride, t, a.D, u);
     float s[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // g, u, g xh, u xh, h, h xh
-    {
-      float w[EPT], uw[EPT];
-      R::load(a.w, t, a.D, w, 1.f);
-      R::load(a.uw, t, a.D, uw);
 #pragma unroll
-      for (int i = 0; i < EPT; ++i) {
-        x[i] = (x[i] - mu) * r;
-        const float g = dy[i] * w[i], h = dy[i] * uw[i];
-        s[0] += g;
-        s[1] += u[i];
-        s[2] += g * x[i];
-        s[3] += u[i] * x[i];
-        s[4] += h;
-        s[5] += h * x[i];
-      }
+    for (int i = 0; i < EPT; ++i) {
+      // dy and u are zero outside the row
+      const float xh = (x.at(i) - mu) * r, d = dy.at(i);
+      const float g = d * w.at(i), h = d * uw.at(i);
+      s[0] += g;
+      s[1] += u.at(i);
+      s[2] += g * xh;
+      s[3] += u.at(i) * xh;
+      s[4] += h;
+      s[5] += h * xh;
     }
-    row_sum<R::NT, 6>(s, red, phase);
+    row_sum<R, 6>(s, sums, phase);
+    stay_packed(x);
+    stay_packed(dy);
+    stay_packed(u);
+    stay_packed(w);
+    stay_packed(uw);
     const float mg = s[0] * inv, mu_u = s[1] * inv, ma = s[2] * inv, mc = s[3] * inv;
     float q[1] = {0.f};
-    float w[EPT];
-    R::load(a.w, t, a.D, w, 1.f);
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) q[0] += dy[i] * w[i] * (u[i] - mu_u - x[i] * mc);
-    row_sum<R::NT, 1>(q, red, phase);
+    for (int i = 0; i < EPT; ++i) {
+      const float xh = (x.at(i) - mu) * r;
+      q[0] += dy.at(i) * w.at(i) * (u.at(i) - mu_u - xh * mc);  // dy again
+    }
+    row_sum<R, 1>(q, sums, phase);
+    stay_packed(x);
+    stay_packed(dy);
+    stay_packed(u);
+    stay_packed(w);
     const float ms = q[0] * inv;
     // v = h - r (c g + a u): its mean and its mean against xh
     const float mv = s[4] * inv - r * (mc * mg + ma * mu_u);
     const float mvx = s[5] * inv - 2.f * r * ma * mc;
-    float uw[EPT], ub[EPT], gx[EPT], gdy[EPT];
-    R::load(a.uw, t, a.D, uw);
-    R::load(a.ub, t, a.D, ub);
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      const float pu = r * (u[i] - mu_u - x[i] * mc);
-      const float v = dy[i] * uw[i] - r * (mc * dy[i] * w[i] + ma * u[i]);
-      agw[i] += dy[i] * pu;
-      gdy[i] = w[i] * pu + x[i] * uw[i] + ub[i];
-      gx[i] = r * (v - mv - x[i] * mvx) - r * r * ms * x[i];
+    for (int i = 0; i < EPT; i += 2) {
+      float gd[2], gx[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float xh = (x.at(i + j) - mu) * r, d = dy.at(i + j);
+        const float pu = r * (u.at(i + j) - mu_u - xh * mc);
+        const float v = d * uw.at(i + j) - r * (mc * d * w.at(i + j) + ma * u.at(i + j));
+        agw[i + j] += d * pu;
+        gd[j] = w.at(i + j) * pu + xh * uw.at(i + j) + ub.at(i + j);
+        gx[j] = r * (v - mv - xh * mvx) - r * r * ms * xh;
+      }
+      dy.set2(i, gd[0], gd[1]);
+      x.set2(i, gx[0], gx[1]);
     }
-    R::store(a.gdy + row * a.D, t, a.D, gdy);
-    R::store(a.gx + row * a.D, t, a.D, gx);
+    R::store(a.gdy + row * a.D, t, a.D, dy);
+    R::store(a.gx + row * a.D, t, a.D, x);
   }
-  if (a.want_dw) write_part<R>(a.part, 0, a.D, agw, sums);
+  if (a.want_dw) write_part<R>(a.part, 0, a.D, agw, cols);
 }
 
-// out[c] = sum over blocks (in order within each of 16 interleaved shares, then
-// share by share) of part[block][which][c]. One block: 32 columns of one array.
+// out[c] = sum over blocks of part[block][which][c]: 32 interleaved shares, each in
+// block order, then the shares in order. One block: 32 columns of one array.
 template <class P>
-__global__ void __launch_bounds__(512) norm_param_reduce_kernel(const float* part, int blocks, int D, P* dw, P* db) {
-  __shared__ float s[16][33];
+__global__ void __launch_bounds__(1024) norm_param_reduce_kernel(const float* part, int blocks, int D, P* dw, P* db) {
+  __shared__ float s[32][33];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the blocks' sums are complete
   const int which = blockIdx.y;
   P* out = which == 0 ? dw : db;
   if (out == nullptr) return;
@@ -342,14 +437,15 @@ __global__ void __launch_bounds__(512) norm_param_reduce_kernel(const float* par
   const int c = blockIdx.x * 32 + tx;
   float acc = 0.f;
   if (c < D) {
-    for (int p = ty; p < blocks; p += 16) acc += part[(static_cast<int64_t>(p) * 2 + which) * D + c];
+#pragma unroll 4
+    for (int p = ty; p < blocks; p += 32) acc += part[(static_cast<int64_t>(p) * 2 + which) * D + c];
   }
   s[ty][tx] = acc;
   __syncthreads();
   if (ty == 0 && c < D) {
     float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v += s[i][tx];
+    for (int i = 0; i < 32; ++i) v += s[i][tx];
     out[c] = from_f<P>(v);
   }
 }
@@ -362,16 +458,19 @@ int sm_count() {
   return n < 1 ? 1 : n;
 }
 
-int row_threads(int D) { return D <= 1024 ? 32 : (D <= 4096 ? 128 : 512); }
+// Threads of a row: 32 to 256 with eight elements each, then 256 or 512 with 16, 512 with 32.
+int row_threads(int D) {
+  int nt = 32;
+  while (nt < 256 && nt * 8 < D) nt *= 2;
+  return D <= 4096 ? nt : 512;
+}
 
-// Blocks of the gradient kernels: enough row groups to fill the SMs, few enough
-// that the blocks' parameter sums stay small beside the rows.
-int grad_blocks(int64_t rows, int D, int sms) {
-  const int nt = row_threads(D);
-  const int64_t groups = nt == 32 ? 8 : 1;
-  const int64_t need = (rows + groups - 1) / groups;
-  const int64_t cap = static_cast<int64_t>(sms) * (nt == 512 ? 1 : (nt == 128 ? 4 : 2));
-  return static_cast<int>(need < cap ? (need < 1 ? 1 : need) : cap);
+// Blocks of the gradient kernels: all that fit on the SMs at once, or as many as there are rows for.
+int grad_blocks(const ttt_norm_problem& pb, bool second, int sms) {
+  const int nt = row_threads(pb.dim), threads = nt > 256 ? nt : 256;
+  const int64_t groups = threads / nt, need = (pb.rows + groups - 1) / groups;
+  const int per_sm = pb.dim <= 2048 && pb.dtype != TTT_F32 && !second ? 3 : 512 / threads;
+  return static_cast<int>(std::min<int64_t>(std::max<int64_t>(need, 1), static_cast<int64_t>(sms) * per_sm));
 }
 
 int check_norm(const ttt_norm_problem& pb) {
@@ -384,13 +483,13 @@ int check_norm(const ttt_norm_problem& pb) {
 enum Pass { kFwd, kBwd, kBwd2 };
 
 template <class X, class P, class R>
-cudaError_t launch_rows(const NormArgs<X, P>& a, Pass pass, int blocks, cudaStream_t s) {
+cudaError_t launch_rows(const NormArgs<X, P>& a, Pass pass, int blocks, int sms, cudaStream_t s) {
   if (pass == kFwd) {
-    const int64_t grid = (a.rows + R::GROUPS - 1) / R::GROUPS;
-    norm_fwd_kernel<X, P, R><<<static_cast<unsigned>(grid), R::THREADS, 0, s>>>(a);
+    const int64_t need = (a.rows + R::GROUPS - 1) / R::GROUPS, fit = static_cast<int64_t>(sms) * R::FWD_PER_SM;
+    norm_fwd_kernel<X, P, R><<<static_cast<unsigned>(std::min(need, fit)), R::THREADS, 0, s>>>(a);
     return cudaGetLastError();
   }
-  const size_t smem = R::GROUPS > 1 ? sizeof(float) * R::GROUPS * a.D : 0;
+  const size_t smem = R::GROUPS > 1 ? sizeof(float) * R::GROUPS * a.D : 0;  // at most 16 KB: D <= 8 * NT
   if (pass == kBwd)
     norm_bwd_kernel<X, P, R><<<blocks, R::THREADS, smem, s>>>(a);
   else
@@ -398,17 +497,15 @@ cudaError_t launch_rows(const NormArgs<X, P>& a, Pass pass, int blocks, cudaStre
   return cudaGetLastError();
 }
 
-// Elements per thread: the row rounded up to NT * {8, 16, 32}.
 template <class X, class P, bool WIDE>
-cudaError_t launch_width(const NormArgs<X, P>& a, Pass pass, int blocks, cudaStream_t s) {
-  const int D = a.D;
-  if (D <= 256) return launch_rows<X, P, Row<X, 32, 8, WIDE>>(a, pass, blocks, s);
-  if (D <= 512) return launch_rows<X, P, Row<X, 32, 16, WIDE>>(a, pass, blocks, s);
-  if (D <= 1024) return launch_rows<X, P, Row<X, 32, 32, WIDE>>(a, pass, blocks, s);
-  if (D <= 2048) return launch_rows<X, P, Row<X, 128, 16, WIDE>>(a, pass, blocks, s);
-  if (D <= 4096) return launch_rows<X, P, Row<X, 128, 32, WIDE>>(a, pass, blocks, s);
-  if (D <= 8192) return launch_rows<X, P, Row<X, 512, 16, WIDE>>(a, pass, blocks, s);
-  return launch_rows<X, P, Row<X, 512, 32, WIDE>>(a, pass, blocks, s);
+cudaError_t launch_width(const NormArgs<X, P>& a, Pass pass, int blocks, int sms, cudaStream_t s) {
+  if (a.D <= 256) return launch_rows<X, P, Row<X, 32, 8, WIDE>>(a, pass, blocks, sms, s);
+  if (a.D <= 512) return launch_rows<X, P, Row<X, 64, 8, WIDE>>(a, pass, blocks, sms, s);
+  if (a.D <= 1024) return launch_rows<X, P, Row<X, 128, 8, WIDE>>(a, pass, blocks, sms, s);
+  if (a.D <= 2048) return launch_rows<X, P, Row<X, 256, 8, WIDE>>(a, pass, blocks, sms, s);
+  if (a.D <= 4096) return launch_rows<X, P, Row<X, 256, 16, WIDE>>(a, pass, blocks, sms, s);
+  if (a.D <= 8192) return launch_rows<X, P, Row<X, 512, 16, WIDE>>(a, pass, blocks, sms, s);
+  return launch_rows<X, P, Row<X, 512, 32, WIDE>>(a, pass, blocks, sms, s);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -421,7 +518,8 @@ int run_norm(NormArgs<X, P> a, const ttt_norm_problem& pb, Pass pass, void* dw, 
   a.eps = pb.eps;
   a.want_dw = dw != nullptr;
   a.want_db = db != nullptr;
-  const int blocks = pass == kFwd ? 0 : grad_blocks(pb.rows, pb.dim, sm_count());
+  const int sms = sm_count();
+  const int blocks = pass == kFwd ? 0 : grad_blocks(pb, pass == kBwd2, sms);
   if (a.want_dw || a.want_db) {
     if (work == nullptr || !aligned16(work) || work_bytes < static_cast<int64_t>(blocks) * 2 * pb.dim * 4)
       return TTT_ERR_SCRATCH;
@@ -434,14 +532,24 @@ int run_norm(NormArgs<X, P> a, const ttt_norm_problem& pb, Pass pass, void* dw, 
     const void* rows_at[] = {a.x, a.dy, a.ux, a.w, a.b, a.uw, a.ub, a.y, a.dx, a.gx, a.gdy};
     for (const void* p : rows_at) wide = wide && aligned16(p);
     wide = wide && a.x_stride % V == 0 && a.dy_stride % V == 0 && a.ux_stride % V == 0;
-    const cudaError_t e = wide ? launch_width<X, P, true>(a, pass, blocks, s)
-                               : launch_width<X, P, false>(a, pass, blocks, s);
+    const cudaError_t e = wide ? launch_width<X, P, true>(a, pass, blocks, sms, s)
+                               : launch_width<X, P, false>(a, pass, blocks, sms, s);
     if (e != cudaSuccess) return TTT_ERR_LAUNCH;
   }
   if (a.want_dw || a.want_db) {
     const dim3 grid((pb.dim + 31) / 32, a.want_db ? 2 : 1);
-    norm_param_reduce_kernel<P><<<grid, 512, 0, s>>>(a.part, blocks, pb.dim, static_cast<P*>(dw), static_cast<P*>(db));
-    if (cudaGetLastError() != cudaSuccess) return TTT_ERR_LAUNCH;
+    cudaLaunchAttribute early;  // may start before the gradient kernel's end, for which it waits itself
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(1024);
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, norm_param_reduce_kernel<P>, static_cast<const float*>(a.part), blocks, pb.dim,
+                           static_cast<P*>(dw), static_cast<P*>(db)) != cudaSuccess)
+      return TTT_ERR_LAUNCH;
   }
   return TTT_OK;
 }
@@ -461,7 +569,7 @@ extern "C" {
 
 int64_t ttt_norm_work_bytes(const ttt_norm_problem* pb) {
   if (pb == nullptr || check_norm(*pb) != TTT_OK) return 0;
-  return static_cast<int64_t>(grad_blocks(pb->rows, pb->dim, sm_count())) * 2 * pb->dim * 4;
+  return static_cast<int64_t>(grad_blocks(*pb, false, sm_count())) * 2 * pb->dim * 4;
 }
 
 int ttt_norm_fwd(const ttt_norm_fwd_args* g, void* stream) {
