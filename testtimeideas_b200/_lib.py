@@ -197,7 +197,7 @@ def _register_fakes() -> None:
     @torch.library.register_fake("ttt::linear_ce")
     def _lce(h, w, targets, mask, reduction, ignore_index):
         loss = h.new_empty(targets.shape if reduction == 0 else (), dtype=torch.float32)
-        return loss, h.new_empty((_lce_state_bytes(targets.numel()),), dtype=torch.uint8)
+        return loss, h.new_empty((_lce_state_bytes(targets.numel(), h.shape[-1]),), dtype=torch.uint8)
 
     @torch.library.register_fake("ttt::linear_ce_bwd")
     def _lce_bwd(dloss, h, w, state, reduction, need_dh, need_dw):
@@ -549,10 +549,12 @@ def layer_norm_ad(x, w, b, eps: float):
 LCE_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
-def _lce_state_bytes(n: int) -> int:
-    """ttt_lce_state_bytes: the head, four arrays of n rows padded to 128 and one of n, each in 256-byte parts."""
+def _lce_state_bytes(n: int, dim: int) -> int:
+    """ttt_lce_state_bytes: the head, four arrays of n rows padded to 256, one of n, and the
+    gathered rows of h, each in 256-byte parts."""
     up = lambda b: (b + 255) // 256 * 256  # noqa: E731
-    return 256 + 4 * up((n + 127) // 128 * 128 * 4) + up(n * 4)
+    rows = up(n)
+    return 256 + 4 * up(rows * 4) + up(n * 4) + up(rows * ((dim + 7) // 8 * 8) * 2)
 
 
 def linear_ce_ad(h, w, targets, mask, reduction: str, ignore_index: int):

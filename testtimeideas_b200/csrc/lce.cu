@@ -2,12 +2,12 @@
 // of each pass and its row kernels. The tensor-core work is in lce_gemm.cu.
 //
 // The participating rows are listed first (slots), and h is gathered into a
-// compact copy, so masked rows cost no products and whatever they hold stays out
-// of every sum. Then
+// compact copy that the state keeps, so masked rows cost no products and whatever
+// they hold stays out of every sum. Then
 //   forward   statistics of z, combined per row into the base-2 log-sum-exp
-//   gradient  per piece of the vocabulary: G in 16 bits; G w added to fp32 partial
-//             rows; G^T h rounded into the piece's rows of dw; at the end the
-//             partial rows are added in order and scattered to dh
+//   gradient  per piece of the vocabulary: G in 16 bits; then in one launch G w,
+//             added to fp32 partial rows, and G^T h, rounded into the piece's rows
+//             of dw; at the end the partial rows are added in order and scattered
 //   second    statistics of (z, A) combined into rho; then as the gradient with
 //             (G, D) and two products per output
 // The stored derivatives carry a power of two that puts their largest possible
@@ -36,8 +36,8 @@ bool encode_2d(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64_
 
 namespace {
 
+using ttt::LceCoef;
 using ttt::LceHead;
-using ttt::LceScale;
 
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -58,22 +58,24 @@ struct Arena {  // hands out 256-byte aligned parts of a buffer (or only counts 
 
 struct State {
   LceHead* head;
-  int* idx;     // [n_pad] source row of a slot, -1 past the last
-  int* tgt;     // [n_pad] target of a slot, -1 past the last
-  float* mw;    // [n_pad] mask weight of a slot, 0 past the last
-  float* lse2;  // [n_pad] base-2 log-sum-exp of a slot, +inf past the last
-  int* slot;    // [n] slot of a source row, -1 if it takes no part
+  int* idx;      // [n_pad] source row of a slot, -1 past the last
+  int* tgt;      // [n_pad] target of a slot, -1 past the last
+  float* mw;     // [n_pad] mask weight of a slot, 0 past the last
+  float* lse2;   // [n_pad] base-2 log-sum-exp of a slot, +inf past the last
+  int* slot;     // [n] slot of a source row, -1 if it takes no part
+  uint16_t* hc;  // [n_pad][dim_pad] rows of h by slot, zeros past the last
 };
-int64_t state_layout(int64_t n, void* base, State* s) {
+int64_t state_layout(const ttt_lce_problem& pb, void* base, State* s) {
   Arena a(base);
-  const int64_t n_pad = up(n, ttt::kLceBM);
+  const int64_t n_pad = up(pb.n, ttt::kLceBM);
   State t;
   t.head = a.take<LceHead>(1);
   t.idx = a.take<int>(n_pad);
   t.tgt = a.take<int>(n_pad);
   t.mw = a.take<float>(n_pad);
   t.lse2 = a.take<float>(n_pad);
-  t.slot = a.take<int>(n);
+  t.slot = a.take<int>(pb.n);
+  t.hc = a.take<uint16_t>(n_pad * up(pb.dim, 8));
   if (s != nullptr) *s = t;
   return a.used;
 }
@@ -105,40 +107,45 @@ Plan make_plan(const ttt_lce_problem& pb, int pass, int sms) {
   const int64_t most = std::max<int64_t>(2048, budget / std::max<int64_t>(per_col, 1));
   const int64_t pieces = (q.vocab + most - 1) / most;
   q.piece = up((q.vocab + pieces - 1) / pieces, 256);
-  // Few token tiles: cut the contraction over the vocabulary so that the dh product fills the SMs.
-  const int64_t tiles = (q.n_pad / ttt::kLceBM) * ((q.dim + ttt::kLceBN - 1) / ttt::kLceBN);
-  const int64_t steps = std::max<int64_t>(1, std::min(q.piece, q.vocab) / ttt::kLceBK);
-  q.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / std::max<int64_t>(tiles, 1), steps / 8)));
+  // The hidden gradient's contraction over the piece is cut where a whole one would
+  // be longer than a pair's share of both products (few tokens); no share is shorter
+  // than eight steps.
+  const int64_t pairs = std::max(1, sms / 2), cols = std::min(q.piece, q.vocab);
+  const int64_t mt = q.n_pad / ttt::kLceBM, dt = up(q.dim, ttt::kLceBN) / ttt::kLceBN;
+  const int64_t kt = up(cols, ttt::kLceBK) / ttt::kLceBK, vt = up(cols, ttt::kLceBM) / ttt::kLceBM;
+  const int64_t share = std::max<int64_t>(1, (mt * dt * kt + vt * dt * (q.n_pad / ttt::kLceBK)) / pairs);
+  q.splits = static_cast<int>(std::max<int64_t>(1, std::min((kt + share - 1) / share, kt / 8)));
   return q;
 }
 
 struct Work {
-  uint16_t *hc, *uc;  // gathered h and uh, [n_pad][dim_pad]
-  float2* part;       // statistics of half tiles, [2 * tiles][n_pad]
-  float* ztgt;        // [n_pad]
-  float* rows;        // [n_pad] row losses (forward), gradients by c (second)
-  LceScale* scale;
-  float* coef;        // [n_pad]
-  float* rho;         // [n_pad]
-  uint16_t *g, *d;    // stored derivatives, [n_pad][piece]
-  float* acc;         // [splits][n_pad][dim_pad]
+  float2* part;        // statistics of half tiles, [2 * tiles][n_pad]
+  float* ztgt;         // [n_pad]
+  float* rows;         // [n_pad] row losses (forward), derivatives by c (second)
+  float* sums;         // [n_pad / 32] their sums by block
+  unsigned* counters;  // [0] ticket of the products, [1] max_bits, [2] ticket of the row sums
+  uint16_t* uc;        // gathered uh, [n_pad][dim_pad]
+  float* coef;         // [n_pad]
+  float* rho;          // [n_pad]
+  uint16_t *g, *d;     // stored derivatives, [n_pad][piece]
+  float* acc;          // [splits][n_pad][dim_pad]
 };
 int64_t work_layout(const Plan& q, int pass, void* base, Work* w) {
   Arena a(base);
   Work t{};
   const int64_t rows = q.n_pad, mat = rows * q.dim_pad;
-  t.hc = a.take<uint16_t>(mat);
-  if (pass == 2) t.uc = a.take<uint16_t>(mat);
+  t.counters = a.take<unsigned>(3);
   if (pass != 1) {
     const int bn = pass == 0 ? ttt::kLceBN : ttt::kLceBNDual;
     t.part = a.take<float2>(2 * ((q.vocab + bn - 1) / bn) * rows);
     t.ztgt = a.take<float>(rows);
     t.rows = a.take<float>(rows);
+    t.sums = a.take<float>(rows / 32);
   }
   if (pass != 0) {
-    t.scale = a.take<LceScale>(1);
     t.coef = a.take<float>(rows);
     if (pass == 2) t.rho = a.take<float>(rows);
+    if (pass == 2) t.uc = a.take<uint16_t>(mat);
     t.g = a.take<uint16_t>(rows * q.piece);
     if (pass == 2) t.d = a.take<uint16_t>(rows * q.piece);
     t.acc = a.take<float>(static_cast<int64_t>(q.splits) * mat);
@@ -160,20 +167,31 @@ __device__ __forceinline__ float block_sum(float v, float* buf) {
   return s;
 }
 
+__device__ __forceinline__ float block_max(float v, float* buf) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = 0.f;
+  for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) s = fmaxf(s, buf[i]);
+  return s;
+}
+
 struct RowArgs {
   int64_t n, vocab, ignore_index;
   int n_pad, dim, dim_pad, mask_kind, reduction;
   const int64_t* targets;
   const void* mask;
-  const uint16_t* src[2];  // h, uh
-  int64_t src_stride[2];
-  uint16_t* dst[2];  // hc, uc
-  int wide;          // rows can be copied in 16-byte pieces
+  const uint16_t* src;  // h (forward) or uh
+  int64_t src_stride;
+  uint16_t* dst;  // its compact copy
+  int wide;       // rows can be copied in 16-byte pieces
   State st;
   float* loss;
   const float* dloss;
   float* coef;
-  LceScale* scale;
+  unsigned* counters;
   int* err;
   int* err_host;
 };
@@ -190,40 +208,46 @@ __device__ __forceinline__ int row_kind(const RowArgs& a, int64_t i, float m) {
   return t >= 0 && t < a.vocab ? 1 : -1;
 }
 
-// Copies source row `row` (or zeros, row < 0) into slot `s` of array `which`; one warp.
-__device__ __forceinline__ void copy_row(const RowArgs& a, int which, int64_t row, int64_t s, int lane) {
-  uint16_t* dst = a.dst[which] + s * a.dim_pad;
-  if (a.src[which] == nullptr) return;
-  const uint16_t* src = row < 0 ? nullptr : a.src[which] + row * a.src_stride[which];
+// Copies source row `row` (or zeros, row < 0) into slot `s`; one warp.
+__device__ __forceinline__ void copy_row(const RowArgs& a, int64_t row, int64_t s, int lane) {
+  if (a.src == nullptr) return;
+  uint16_t* dst = a.dst + s * a.dim_pad;
+  const uint16_t* src = row < 0 ? nullptr : a.src + row * a.src_stride;
   if (a.wide) {
+#pragma unroll 4
     for (int c = lane * 8; c < a.dim; c += 256)
       *reinterpret_cast<uint4*>(dst + c) =
           src == nullptr ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(src + c);
   } else {
+#pragma unroll 4
     for (int c = lane; c < a.dim; c += 32) dst[c] = src == nullptr ? 0 : src[c];
   }
 }
 
-// Lists the participating rows and gathers h. Block b owns rows [64 b, 64 b + 64);
+// Lists the participating rows and gathers h. Block b owns rows [32 b, 32 b + 32);
 // it counts the participating rows before them itself (n / 2 reads of 8 to 12 bytes
 // on average, from L2), so that one launch does without a scan across blocks. The
 // last block also knows the totals and clears the slots up to the next whole tile.
-constexpr int kListRows = 64;
+constexpr int kListRows = 32;
 __global__ void __launch_bounds__(256) lce_list_kernel(const RowArgs a) {
   __shared__ float buf[8];
   __shared__ int cnt[8];
   __shared__ int slots[kListRows];
   __shared__ int total;
+  asm volatile("griddepcontrol.launch_dependents;");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kListRows;
   const bool last = blockIdx.x == gridDim.x - 1;
-  // participating rows (and, in the last block, the mask's sum) before row0
+  // participating rows before row0, and the mask's sum and largest magnitude over them
   int before = 0;
-  float msum = 0.f;
+  float msum = 0.f, mmax = 0.f;
+#pragma unroll 4
   for (int64_t i = threadIdx.x; i < row0; i += 256) {
     const float m = mask_weight(a, i);
-    before += row_kind(a, i, m) > 0;
+    const bool in = row_kind(a, i, m) > 0;
+    before += in;
     msum += m;
+    mmax = in ? fmaxf(mmax, fabsf(m)) : mmax;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
@@ -232,106 +256,112 @@ __global__ void __launch_bounds__(256) lce_list_kernel(const RowArgs a) {
   if (warp == 0) {
     int base = 0;
     for (int i = 0; i < 8; ++i) base += cnt[i];
-    for (int part = 0; part < kListRows / 32; ++part) {
-      const int64_t i = row0 + part * 32 + lane;
-      float m = 0.f;
-      int kind = 0;
-      if (i < a.n) {
-        m = mask_weight(a, i);
-        kind = row_kind(a, i, m);
-        if (kind < 0) ttt::report_error(a.err, a.err_host, TTT_ERR_WORD_TARGET | (static_cast<int>(i) & 0xffffff));
-        msum += m;
-      }
-      const unsigned bits = __ballot_sync(0xffffffffu, kind > 0);
-      const int s = kind > 0 ? base + __popc(bits & ((1u << lane) - 1)) : -1;
-      base += __popc(bits);
-      slots[part * 32 + lane] = s;
-      if (i < a.n) {
-        a.st.slot[i] = s;
-        if (s >= 0) {
-          a.st.idx[s] = static_cast<int>(i);
-          a.st.tgt[s] = static_cast<int>(a.targets[i]);
-          a.st.mw[s] = m;
-        } else if (a.reduction == TTT_LCE_NONE) {
-          a.loss[i] = 0.f;
-        }
+    const int64_t i = row0 + lane;
+    float m = 0.f;
+    int kind = 0;
+    if (i < a.n) {
+      m = mask_weight(a, i);
+      kind = row_kind(a, i, m);
+      if (kind < 0) ttt::report_error(a.err, a.err_host, TTT_ERR_WORD_TARGET | (static_cast<int>(i) & 0xffffff));
+      msum += m;
+      mmax = kind > 0 ? fmaxf(mmax, fabsf(m)) : mmax;
+    }
+    const unsigned bits = __ballot_sync(0xffffffffu, kind > 0);
+    const int s = kind > 0 ? base + __popc(bits & ((1u << lane) - 1)) : -1;
+    base += __popc(bits);
+    slots[lane] = s;
+    if (i < a.n) {
+      a.st.slot[i] = s;
+      if (s >= 0) {
+        a.st.idx[s] = static_cast<int>(i);
+        a.st.tgt[s] = static_cast<int>(a.targets[i]);
+        a.st.mw[s] = m;
+      } else if (a.reduction == TTT_LCE_NONE) {
+        a.loss[i] = 0.f;
       }
     }
     if (lane == 0) total = base;
   }
   __syncthreads();
   for (int j = warp; j < kListRows; j += 8)
-    if (slots[j] >= 0) copy_row(a, 0, row0 + j, slots[j], lane);
+    if (slots[j] >= 0) copy_row(a, row0 + j, slots[j], lane);
   if (!last) return;
   const int n_active = total;
   const int end = min((n_active + ttt::kLceBM - 1) / ttt::kLceBM * ttt::kLceBM, a.n_pad);
   for (int s = n_active + warp; s < end; s += 8) {
-    copy_row(a, 0, -1, s, lane);
+    copy_row(a, -1, s, lane);
     if (lane == 0) a.st.idx[s] = -1, a.st.tgt[s] = -1, a.st.mw[s] = 0.f, a.st.lse2[s] = INFINITY;
   }
   msum = block_sum(msum, buf);
+  mmax = block_max(mmax, buf);
   if (threadIdx.x == 0) {
     a.st.head->n_active = n_active;
     float denom = 1.f;
     if (a.reduction == TTT_LCE_MEAN)
       denom = a.mask_kind == TTT_LCE_MASK_NONE ? static_cast<float>(a.n) : fmaxf(msum, 1.f);
     a.st.head->denom = denom;
+    a.st.head->mw_max = mmax;
+    a.st.head->ticket = 0;
   }
 }
 
-// Power of two that brings `big` (the largest magnitude to store) near 2^13; 1 for 0, inf and NaN.
-__device__ __forceinline__ void set_scale(LceScale* s, float big) {
-  float f = 1.f;
-  if (big > 0.f && big < INFINITY) {
-    int e;
-    frexpf(big, &e);  // big < 2^e
-    e = max(-100, min(100, 13 - e));
-    f = ldexpf(1.f, e);
-  }
-  s->scale = f;
-  s->inv = 1.f / f;
-}
-
-__device__ __forceinline__ float row_coef(const RowArgs& a, int s) {
-  const int i = a.st.idx[s];
-  if (a.reduction == TTT_LCE_NONE) return a.dloss[i] * a.st.mw[s];
-  return a.dloss[0] * (a.st.mw[s] / a.st.head->denom);
-}
-
-// Gathers h (and uh) into slots and forms the row coefficients c; block 0 also
-// finds their largest magnitude and sets the scale of the stored derivatives
-// (the second gradient raises it in lce_rho_kernel).
-__global__ void __launch_bounds__(256) lce_gather_kernel(const RowArgs a) {
+// Lists the row coefficients c and gathers uh into slots; block 0 also finds the
+// largest |c| (the second gradient raises it in lce_rho_kernel).
+__global__ void __launch_bounds__(256) lce_coef_kernel(const RowArgs a) {
   __shared__ float buf[8];
+  asm volatile("griddepcontrol.launch_dependents;");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_active = a.st.head->n_active;
   const int end = min((n_active + ttt::kLceBM - 1) / ttt::kLceBM * ttt::kLceBM, a.n_pad);
+  auto coef = [&](int s) {
+    if (a.reduction == TTT_LCE_NONE) return a.dloss[a.st.idx[s]] * a.st.mw[s];
+    return *a.dloss * (a.st.mw[s] / a.st.head->denom);
+  };
   for (int s = blockIdx.x * 8 + warp; s < end; s += gridDim.x * 8) {
-    const int64_t row = s < n_active ? a.st.idx[s] : -1;
-    copy_row(a, 0, row, s, lane);
-    copy_row(a, 1, row, s, lane);
-    if (lane == 0) a.coef[s] = s < n_active ? row_coef(a, s) : 0.f;
+    copy_row(a, s < n_active ? a.st.idx[s] : -1, s, lane);
+    if (lane == 0) a.coef[s] = s < n_active ? coef(s) : 0.f;
   }
   if (blockIdx.x != 0) return;
   float big = 0.f;
-  for (int s = threadIdx.x; s < n_active; s += 256) big = fmaxf(big, fabsf(row_coef(a, s)));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-  if (lane == 0) buf[warp] = big;
-  __syncthreads();
+#pragma unroll 4
+  for (int s = threadIdx.x; s < n_active; s += 256) big = fmaxf(big, fabsf(coef(s)));
+  big = block_max(big, buf);
   if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) big = fmaxf(big, buf[i]);
-    a.scale->max_bits = __float_as_uint(big);
-    set_scale(a.scale, big);
+    a.counters[1] = __float_as_uint(big);
+    a.counters[2] = 0;
   }
 }
 
-// Merges the half tiles' (max, sum) of a row: 32 rows and 8 shares of the tiles per
-// block, shares in order. Writes lse2, and the row's weighted loss to rows[slot]
-// (and loss[row] with TTT_LCE_NONE).
-__global__ void __launch_bounds__(256) lce_lse_kernel(const State st, const float2* part, const float* ztgt, int parts,
-                                                      int n_pad, int reduction, float* rows, float* loss) {
-  __shared__ float2 sh[8][33];
+// Adds rows[] of this block's 32 slots (warp 0, v of each lane) and, in the last block
+// to finish, the blocks' sums in block order: out = total / denom. A fixed order.
+__device__ __forceinline__ void total_rows(float v, float* sums, unsigned* ticket, float denom, float* out) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  unsigned done = 0;
+  if (threadIdx.x == 0) {
+    sums[blockIdx.x] = v;
+    __threadfence();
+    done = atomicAdd(ticket, 1u);
+  }
+  done = __shfl_sync(0xffffffffu, done, 0);
+  if (done != gridDim.x - 1) return;
+  __threadfence();
+  float t = 0.f;
+#pragma unroll 4
+  for (unsigned i = threadIdx.x; i < gridDim.x; i += 32) t += __ldcg(sums + i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if (threadIdx.x == 0) *out = t / denom;
+}
+
+// Merges the half tiles' (max, sum) of a row: 32 rows and 16 shares of the tiles per
+// block, shares in order. Writes lse2 and the row's weighted loss.
+constexpr int kShares = 16;
+__global__ void __launch_bounds__(32 * kShares) lce_lse_kernel(const State st, const float2* part, const float* ztgt,
+                                                               int parts, int n_pad, int reduction, float* sums,
+                                                               float* loss) {
+  __shared__ float2 sh[kShares][33];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
   const int s = blockIdx.x * 32 + lane, n_active = st.head->n_active;
   float m = -INFINITY, l = 0.f;
@@ -341,66 +371,65 @@ __global__ void __launch_bounds__(256) lce_lse_kernel(const State st, const floa
     l = l * exp2f(m - sub) + o.y * exp2f(o.x - sub);
     m = top;
   };
-  if (s < n_active)
-    for (int i = share; i < parts; i += 8) merge(part[static_cast<int64_t>(i) * n_pad + s]);
+  if (s < n_active) {
+#pragma unroll 4
+    for (int i = share; i < parts; i += kShares) merge(part[static_cast<int64_t>(i) * n_pad + s]);
+  }
   sh[share][lane] = make_float2(m, l);
   __syncthreads();
-  if (share != 0 || s >= n_active) return;
-  for (int i = 1; i < 8; ++i) merge(sh[i][lane]);
-  const float lse2 = m + log2f(l);
-  st.lse2[s] = lse2;
-  const float v = st.mw[s] * (kLn2 * lse2 - ztgt[s]);
-  rows[s] = v;
-  if (reduction == TTT_LCE_NONE) loss[st.idx[s]] = v;
-}
-
-// out = sum over the slots of rows[] / N, in a fixed order (one block).
-__global__ void __launch_bounds__(1024) lce_total_kernel(const LceHead* head, const float* rows, float* out) {
-  __shared__ float buf[32];
+  if (share != 0) return;
   float v = 0.f;
-  for (int s = threadIdx.x; s < head->n_active; s += 1024) v += rows[s];
-  v = block_sum(v, buf);
-  if (threadIdx.x == 0) *out = v / head->denom;
+  if (s < n_active) {
+    for (int i = 1; i < kShares; ++i) merge(sh[i][lane]);
+    const float lse2 = m + log2f(l);
+    st.lse2[s] = lse2;
+    v = st.mw[s] * (kLn2 * lse2 - ztgt[s]);
+    if (reduction == TTT_LCE_NONE) loss[st.idx[s]] = v;
+  }
+  if (reduction != TTT_LCE_NONE) total_rows(v, sums, &st.head->ticket, st.head->denom, loss);
 }
 
-// Adds the half tiles' sums P A of a row into rho, raises the scale's bound to the
-// largest |c| (max |P A| + |rho|), which bounds |D|, and forms the derivative by c.
-__global__ void __launch_bounds__(256) lce_rho_kernel(const State st, const float2* part, const float* ztgt,
-                                                      const float* coef, int parts, int n_pad, int reduction,
-                                                      float* rho, LceScale* scale, float* rows, float* gdloss) {
-  __shared__ float2 sh[8][33];
+// Adds the half tiles' sums P A of a row into rho, raises the bound of what is stored
+// to the largest |c| (max |P A| + |rho|), which bounds |D|, and forms the derivative by c.
+__global__ void __launch_bounds__(32 * kShares) lce_rho_kernel(const State st, const float2* part, const float* ztgt,
+                                                               const float* coef, int parts, int n_pad, int reduction,
+                                                               float* rho, unsigned* counters, float* sums,
+                                                               float* gdloss) {
+  __shared__ float2 sh[kShares][33];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
   const int s = blockIdx.x * 32 + lane, n_active = st.head->n_active;
   float sum = 0.f, big = 0.f;
-  if (s < n_active)
-    for (int i = share; i < parts; i += 8) {
+  if (s < n_active) {
+#pragma unroll 4
+    for (int i = share; i < parts; i += kShares) {
       const float2 o = part[static_cast<int64_t>(i) * n_pad + s];
       sum += o.x;
       big = fmaxf(big, o.y);
     }
+  }
   sh[share][lane] = make_float2(sum, big);
   __syncthreads();
   if (share != 0) return;
+  float dc = 0.f;
   if (s < n_active) {
-    for (int i = 1; i < 8; ++i) {
+    for (int i = 1; i < kShares; ++i) {
       sum += sh[i][lane].x;
       big = fmaxf(big, sh[i][lane].y);
     }
     rho[s] = sum;
-    const float dc = st.mw[s] * (sum - ztgt[s]);
-    rows[s] = dc;
+    dc = st.mw[s] * (sum - ztgt[s]);
     if (gdloss != nullptr && reduction == TTT_LCE_NONE) gdloss[st.idx[s]] = dc;
     big = fabsf(coef[s]) * (big + fabsf(sum));
-  } else if (s < (n_active + ttt::kLceBM - 1) / ttt::kLceBM * ttt::kLceBM) {
+  } else if (s < n_pad) {
     rho[s] = 0.f;
   }
   if (s >= n_active || !(big < INFINITY)) big = 0.f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-  if (lane == 0) atomicMax(&scale->max_bits, __float_as_uint(big));  // non-negative: ordered like its bits
+  if (lane == 0) atomicMax(counters + 1, __float_as_uint(big));  // non-negative: ordered like its bits
+  if (gdloss != nullptr && reduction != TTT_LCE_NONE) total_rows(dc, sums, counters + 2, st.head->denom, gdloss);
 }
-
-__global__ void lce_scale_kernel(LceScale* scale) { set_scale(scale, __uint_as_float(scale->max_bits)); }
 
 __global__ void lce_zero_rows_kernel(const int* slot, int64_t n, float* out) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -409,18 +438,21 @@ __global__ void lce_zero_rows_kernel(const int* slot, int64_t n, float* out) {
 
 // dh[i] = sum over the splits (in order) of acc[split][slot_i] / scale, 0 for rows left out. One warp per row.
 template <bool BF16>
-__global__ void __launch_bounds__(256) lce_scatter_kernel(const int* slot, const LceScale* scale, const float* acc,
+__global__ void __launch_bounds__(256) lce_scatter_kernel(const int* slot, const LceCoef coef, const float* acc,
                                                           int splits, int64_t n, int n_pad, int dim, int dim_pad,
                                                           uint16_t* dh) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (i >= n) return;
   const int lane = threadIdx.x & 31;
   const int s = slot[i];
-  const float inv = scale->inv;
+  const float inv = 1.f / coef.scale();
   uint16_t* dst = dh + i * dim;
+#pragma unroll 2
   for (int c = lane * 4; c < dim; c += 128) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (s >= 0) {
+#pragma unroll 4
       for (int k = 0; k < splits; ++k) {
         const float4 o =
             *reinterpret_cast<const float4*>(acc + (static_cast<int64_t>(k) * n_pad + s) * dim_pad + c);
@@ -475,50 +507,71 @@ struct Weight {
   const uint16_t* row(int64_t r) const { return p + r * stride; }
 };
 
+// A launch whose start may overlap the previous kernel's end; the kernel waits for it itself.
+template <class... K, class... A>
+int launch_early(void (*kern)(K...), int64_t grid, int threads, cudaStream_t s, A... args) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.stream = s;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return launched(cudaLaunchKernelEx(&cfg, kern, static_cast<K>(args)...));
+}
+
 struct Pass {
   const ttt_lce_problem& pb;
   Plan q;
   State st;
   Work w;
+  LceCoef coef;
   int sms;
   bool bf16;
   int* err;
   int* err_host;
   cudaStream_t s;
 
-  Pass(const ttt_lce_problem& p, int pass, const void* state, void* work, int32_t* e, void* stream)
+  Pass(const ttt_lce_problem& p, int pass, const void* state, void* work, const float* dloss, int32_t* e,
+       void* stream)
       : pb(p), sms(device_sms()), bf16(p.dtype == TTT_BF16), err(e),
         err_host(e != nullptr ? ttt::registered_error_mirror() : nullptr), s(static_cast<cudaStream_t>(stream)) {
     q = make_plan(p, pass, sms);
-    state_layout(p.n, const_cast<void*>(state), &st);
+    state_layout(p, const_cast<void*>(state), &st);
     work_layout(q, pass, work, &w);
+    const bool listed = pass == 2 || (pass == 1 && p.reduction == TTT_LCE_NONE);
+    coef = {st.head, dloss, st.mw, listed ? w.coef : nullptr, w.counters + 1};
   }
-  RowArgs row_args() const {
+  // Row kernels; src is gathered into dst when given.
+  RowArgs row_args(const void* src, int64_t stride, uint16_t* dst) const {
     RowArgs a;
     std::memset(&a, 0, sizeof(a));
     a.n = pb.n, a.vocab = pb.vocab, a.ignore_index = pb.ignore_index;
     a.n_pad = static_cast<int>(q.n_pad), a.dim = q.dim, a.dim_pad = q.dim_pad;
     a.mask_kind = pb.mask_kind, a.reduction = pb.reduction;
+    a.src = static_cast<const uint16_t*>(src), a.src_stride = stride, a.dst = dst;
+    a.wide = q.dim % 8 == 0 && aligned(src, 16) && stride % 8 == 0;
     a.st = st;
+    a.dloss = coef.dloss, a.coef = w.coef, a.counters = w.counters;
     a.err = err, a.err_host = err_host;
     return a;
   }
-  void set_source(RowArgs& a, int which, const void* src, int64_t stride, uint16_t* dst) const {
-    a.src[which] = static_cast<const uint16_t*>(src);
-    a.src_stride[which] = stride;
-    a.dst[which] = dst;
-    const bool ok = q.dim % 8 == 0 && aligned(src, 16) && stride % 8 == 0;
-    a.wide = which == 0 ? ok : a.wide && (src == nullptr || ok);
+  int list_coef(const void* uh, int64_t stride) const {
+    const int64_t blocks = uh != nullptr ? std::min<int64_t>(q.n_pad / 8, sms * 8) : 1 + q.n_pad / 2048;
+    lce_coef_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(row_args(uh, stride, w.uc));
+    return launched();
   }
-  ttt::LceGemm gemm() const {
+  ttt::LceGemm gemm(int64_t col0, int64_t cols) const {
     ttt::LceGemm g;
     std::memset(&g, 0, sizeof(g));
-    g.head = st.head, g.scale = w.scale;
-    g.tgt = st.tgt, g.lse2 = st.lse2, g.coef = w.coef, g.rho = w.rho;
-    g.part = w.part, g.ztgt = w.ztgt, g.acc = w.acc;
+    g.head = st.head, g.coef = coef;
+    g.tgt = st.tgt, g.lse2 = st.lse2, g.rho = w.rho;
+    g.part = w.part, g.ztgt = w.ztgt, g.ticket = w.counters;
     g.n_pad = static_cast<int>(q.n_pad), g.dim = q.dim, g.dim_pad = q.dim_pad;
-    g.cols = static_cast<int>(q.vocab);
-    g.seg_mask = 1, g.splits = 1;
+    g.col0 = static_cast<int>(col0), g.cols = static_cast<int>(cols);
+    g.splits = 1;
     g.err = err, g.err_host = err_host;
     return g;
   }
@@ -526,73 +579,64 @@ struct Pass {
   bool map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t stride, int bc, int br) const {
     return ttt::encode_2d(m, bf16, base, cols, rows, stride, bc, br);
   }
-  bool map_rows(CUtensorMap* m, const uint16_t* x, int bc, int br) const {  // hc, uc
-    return map(m, x, q.dim, q.n_pad, q.dim_pad, bc, br);
+  // Operands of the logit kinds: rows of hc or uc (128 a CTA), rows of a piece of w or uw (bn / 2 a CTA).
+  bool map_rows(CUtensorMap* m, const uint16_t* x) const {
+    return map(m, x, q.dim, q.n_pad, q.dim_pad, ttt::kLceBK, ttt::kLceBM / 2);
+  }
+  bool map_weight(CUtensorMap* m, const Weight& w, const ttt::LceGemm& g, int bn) const {
+    return map(m, w.row(g.col0), q.dim, g.cols, w.stride, ttt::kLceBK, bn / 2);
   }
 };
 
-// The gradients of a piece-wise pass: outh [n, dim] and outw [vocab, dim] (either
-// may be null) from stored derivatives: in the gradient G alone; in the second
-// gradient G and D, with the weight-like matrices and gathered rows they meet:
-//   outh = sum_i deriv_i wmat_i, outw = sum_i deriv_i^T rows_i   (i = 0, 1)
+// The gradients of a piece-wise pass: outh [n, dim] and outw [vocab, dim] (either may
+// be null). Per product i with stored derivative S_i, weight-like W_i and rows R_i:
+//   outh = sum_i S_i W_i, outw = sum_i S_i^T R_i
+// gradient: (G, w, h); second gradient: (D, w, h) and (G, uw, uh).
 int run_pieces(const Pass& p, const Weight& w, const Weight* uw, bool second, bool has_uh, uint16_t* outh,
                uint16_t* outw) {
   const Plan& q = p.q;
   if (outh == nullptr && outw == nullptr) return TTT_OK;
+  const int bn = second ? ttt::kLceBNDual : ttt::kLceBN;
+  constexpr int bk = ttt::kLceBK;
   for (int64_t col0 = 0; col0 < q.vocab; col0 += q.piece) {
     const int64_t cols = std::min(q.piece, q.vocab - col0);
     // z (and A) -> G (and D)
-    ttt::LceGemm g = p.gemm();
-    g.col0 = static_cast<int>(col0), g.cols = static_cast<int>(cols);
-    const int bn = second ? ttt::kLceBNDual : ttt::kLceBN;
-    bool ok = p.map_rows(&g.a[0], p.w.hc, 64, 128) && p.map(&g.b[0], w.row(col0), q.dim, cols, w.stride, 64, bn) &&
-              p.map(&g.out[0], p.w.g, cols, q.n_pad, q.piece, 64, 128);
+    ttt::LceGemm g = p.gemm(col0, cols);
+    bool ok = p.map_rows(&g.a[0], p.st.hc) && p.map_weight(&g.b[0], w, g, bn) &&
+              p.map(&g.out[0], p.w.g, cols, q.n_pad, q.piece, 64, 32);
     if (second) {
-      g.seg_mask = (has_uh ? 1 : 0) | (uw != nullptr ? 2 : 0);
-      ok = ok && p.map_rows(&g.a[1], p.w.uc, 64, 128) &&
-           p.map(&g.b[1], (uw != nullptr ? *uw : w).row(col0), q.dim, cols, (uw != nullptr ? *uw : w).stride, 64, bn) &&
-           p.map(&g.out[1], p.w.d, cols, q.n_pad, q.piece, 64, 128);
+      g.seg_w = (has_uh ? 1 : 0) | (uw != nullptr ? 2 : 0);
+      ok = ok && p.map_rows(&g.a[1], p.w.uc) && p.map_weight(&g.b[1], uw != nullptr ? *uw : w, g, bn) &&
+           p.map(&g.out[1], p.w.d, cols, q.n_pad, q.piece, 64, 32);
     }
     if (!ok) return TTT_ERR_TENSOR_MAP;
     TTT_TRY(p.run(g, second ? ttt::kLceDualGrad : ttt::kLceGrad));
-    if (outh != nullptr) {
-      // first gradient: G w; second: D w + G uw
-      ttt::LceGemm h = p.gemm();
-      h.col0 = g.col0, h.cols = g.cols;
-      h.splits = q.splits;
-      h.accumulate = col0 > 0;
-      ok = p.map(&h.a[0], second ? p.w.d : p.w.g, cols, q.n_pad, q.piece, 64, 128) &&
-           p.map(&h.b[0], w.row(col0), q.dim, cols, w.stride, 64, 64);
-      if (second && uw != nullptr) {
-        h.seg_mask = 3;
-        ok = ok && p.map(&h.a[1], p.w.g, cols, q.n_pad, q.piece, 64, 128) &&
-             p.map(&h.b[1], uw->row(col0), q.dim, cols, uw->stride, 64, 64);
-      }
+    // both products in one launch
+    ttt::LceGemm t = p.gemm(col0, cols);
+    t.acc = outh != nullptr ? p.w.acc : nullptr;
+    t.dw = outw != nullptr ? outw + col0 * q.dim : nullptr;
+    t.seg_w = outh != nullptr ? (second && uw != nullptr ? 3 : 1) : 0;
+    t.seg_h = outw != nullptr ? (second && has_uh ? 3 : 1) : 0;
+    t.splits = q.splits;
+    t.accumulate = col0 > 0;
+    for (int i = 0; i < (second ? 2 : 1); ++i) {
+      const uint16_t* stored = second && i == 0 ? p.w.d : p.w.g;
+      const Weight& wi = i == 0 || uw == nullptr ? w : *uw;
+      const uint16_t* ri = i == 0 || !has_uh ? p.st.hc : p.w.uc;
+      ok = p.map(&t.gk[i], stored, cols, q.n_pad, q.piece, bk, ttt::kLceBM / 2) &&
+           p.map(&t.gm[i], stored, cols, q.n_pad, q.piece, 64, bk) &&
+           p.map(&t.bw[i], wi.row(col0), q.dim, cols, wi.stride, 64, bk) &&
+           p.map(&t.bh[i], ri, q.dim, q.n_pad, q.dim_pad, 64, bk);
       if (!ok) return TTT_ERR_TENSOR_MAP;
-      TTT_TRY(p.run(h, ttt::kLceDH));
     }
-    if (outw != nullptr) {
-      // first gradient: G^T h; second: D^T h + G^T uh
-      ttt::LceGemm v = p.gemm();
-      v.col0 = g.col0, v.cols = g.cols;
-      v.dw = outw + col0 * q.dim;
-      ok = p.map(&v.a[0], second ? p.w.d : p.w.g, cols, q.n_pad, q.piece, 64, 64) &&
-           p.map_rows(&v.b[0], p.w.hc, 64, 64);
-      if (second && has_uh) {
-        v.seg_mask = 3;
-        ok = ok && p.map(&v.a[1], p.w.g, cols, q.n_pad, q.piece, 64, 64) && p.map_rows(&v.b[1], p.w.uc, 64, 64);
-      }
-      if (!ok) return TTT_ERR_TENSOR_MAP;
-      TTT_TRY(p.run(v, ttt::kLceDW));
-    }
+    if (t.dw != nullptr && q.dim % 8 == 0 && !p.map(&t.dw_out, t.dw, q.dim, cols, q.dim, 64, 32))
+      return TTT_ERR_TENSOR_MAP;
+    TTT_TRY(p.run(t, ttt::kLceProd));
   }
-  if (outh != nullptr) {
-    const unsigned grid = static_cast<unsigned>((q.n + 7) / 8);
-    auto kern = p.bf16 ? lce_scatter_kernel<true> : lce_scatter_kernel<false>;
-    kern<<<grid, 256, 0, p.s>>>(p.st.slot, p.w.scale, p.w.acc, q.splits, q.n, static_cast<int>(q.n_pad), q.dim,
-                                q.dim_pad, outh);
-    TTT_TRY(launched());
-  }
+  if (outh != nullptr)
+    TTT_TRY(launch_early(p.bf16 ? lce_scatter_kernel<true> : lce_scatter_kernel<false>, (q.n + 7) / 8, 256, p.s,
+                         p.st.slot, p.coef, p.w.acc, q.splits, q.n, static_cast<int>(q.n_pad), q.dim, q.dim_pad,
+                         outh));
   return TTT_OK;
 }
 
@@ -604,7 +648,7 @@ extern "C" {
 
 int64_t ttt_lce_state_bytes(const ttt_lce_problem* pb) {
   if (pb == nullptr || check_lce(*pb) != TTT_OK) return 0;
-  return state_layout(pb->n, nullptr, nullptr);
+  return state_layout(*pb, nullptr, nullptr);
 }
 
 int64_t ttt_lce_work_bytes(const ttt_lce_problem* pb, int pass) {
@@ -623,27 +667,18 @@ int ttt_lce_fwd(const ttt_lce_fwd_args* a, void* stream) {
   if ((a->mask == nullptr) != (pb.mask_kind == TTT_LCE_MASK_NONE)) return TTT_ERR_NULL;
   if (a->work == nullptr || a->work_bytes < ttt_lce_work_bytes(&pb, 0)) return TTT_ERR_SCRATCH;
   if (!aligned(a->work, 256) || !aligned(a->state, 256)) return TTT_ERR_ALIGN;
-  Pass p(pb, 0, a->state, a->work, a->err, stream);
-  RowArgs r = p.row_args();
+  Pass p(pb, 0, a->state, a->work, nullptr, a->err, stream);
+  RowArgs r = p.row_args(a->h, a->h_stride, p.st.hc);
   r.targets = a->targets, r.mask = a->mask, r.loss = a->loss;
-  p.set_source(r, 0, a->h, a->h_stride, p.w.hc);
   lce_list_kernel<<<static_cast<unsigned>((pb.n + kListRows - 1) / kListRows), 256, 0, p.s>>>(r);
   TTT_TRY(launched());
-  ttt::LceGemm g = p.gemm();
+  ttt::LceGemm g = p.gemm(0, pb.vocab);
   const Weight w(a->w, a->w_stride, pb);
-  if (!p.map_rows(&g.a[0], p.w.hc, 64, 128) ||
-      !p.map(&g.b[0], w.p, p.q.dim, p.q.vocab, w.stride, 64, ttt::kLceBN))
-    return TTT_ERR_TENSOR_MAP;
+  if (!p.map_rows(&g.a[0], p.st.hc) || !p.map_weight(&g.b[0], w, g, ttt::kLceBN)) return TTT_ERR_TENSOR_MAP;
   TTT_TRY(p.run(g, ttt::kLceStats));
   const int parts = 2 * static_cast<int>((pb.vocab + ttt::kLceBN - 1) / ttt::kLceBN);
-  lce_lse_kernel<<<static_cast<unsigned>((pb.n + 31) / 32), 256, 0, p.s>>>(p.st, p.w.part, p.w.ztgt, parts, g.n_pad,
-                                                                           pb.reduction, p.w.rows, a->loss);
-  TTT_TRY(launched());
-  if (pb.reduction != TTT_LCE_NONE) {
-    lce_total_kernel<<<1, 1024, 0, p.s>>>(p.st.head, p.w.rows, a->loss);
-    TTT_TRY(launched());
-  }
-  return TTT_OK;
+  return launch_early(lce_lse_kernel, (pb.n + 31) / 32, 32 * kShares, p.s, p.st, p.w.part, p.w.ztgt, parts, g.n_pad,
+                      pb.reduction, p.w.sums, a->loss);
 }
 
 int ttt_lce_bwd(const ttt_lce_bwd_args* a, void* stream) {
@@ -658,12 +693,8 @@ int ttt_lce_bwd(const ttt_lce_bwd_args* a, void* stream) {
   if (a->h == nullptr) return TTT_ERR_NULL;
   if (a->work == nullptr || a->work_bytes < ttt_lce_work_bytes(&pb, 1)) return TTT_ERR_SCRATCH;
   if (!aligned(a->work, 256) || !aligned(a->state, 256)) return TTT_ERR_ALIGN;
-  Pass p(pb, 1, a->state, a->work, a->err, stream);
-  RowArgs r = p.row_args();
-  r.dloss = a->dloss, r.coef = p.w.coef, r.scale = p.w.scale;
-  p.set_source(r, 0, a->h, a->h_stride, p.w.hc);
-  lce_gather_kernel<<<static_cast<unsigned>(std::min<int64_t>(p.q.n_pad / 8, p.sms * 8)), 256, 0, p.s>>>(r);
-  TTT_TRY(launched());
+  Pass p(pb, 1, a->state, a->work, a->dloss, a->err, stream);
+  if (p.coef.coef != nullptr) TTT_TRY(p.list_coef(nullptr, 0));
   return run_pieces(p, Weight(a->w, a->w_stride, pb), nullptr, false, false, static_cast<uint16_t*>(a->dh),
                     static_cast<uint16_t*>(a->dw));
 }
@@ -687,34 +718,21 @@ int ttt_lce_bwd2(const ttt_lce_bwd2_args* a, void* stream) {
   if (a->h == nullptr) return TTT_ERR_NULL;
   if (a->work == nullptr || a->work_bytes < ttt_lce_work_bytes(&pb, 2)) return TTT_ERR_SCRATCH;
   if (!aligned(a->work, 256) || !aligned(a->state, 256)) return TTT_ERR_ALIGN;
-  Pass p(pb, 2, a->state, a->work, a->err, stream);
-  RowArgs r = p.row_args();
-  r.dloss = a->dloss, r.coef = p.w.coef, r.scale = p.w.scale;
-  p.set_source(r, 0, a->h, a->h_stride, p.w.hc);
-  p.set_source(r, 1, a->uh, a->uh_stride, p.w.uc);
-  lce_gather_kernel<<<static_cast<unsigned>(std::min<int64_t>(p.q.n_pad / 8, p.sms * 8)), 256, 0, s>>>(r);
-  TTT_TRY(launched());
+  Pass p(pb, 2, a->state, a->work, a->dloss, a->err, stream);
+  TTT_TRY(p.list_coef(a->uh, a->uh_stride));
   const Weight w(a->w, a->w_stride, pb);
   const Weight uw = a->uw != nullptr ? Weight(a->uw, a->uw_stride, pb) : w;
-  ttt::LceGemm g = p.gemm();
-  g.seg_mask = (a->uh != nullptr ? 1 : 0) | (a->uw != nullptr ? 2 : 0);
-  if (!p.map_rows(&g.a[0], p.w.hc, 64, 128) || !p.map_rows(&g.a[1], p.w.uc, 64, 128) ||
-      !p.map(&g.b[0], w.p, p.q.dim, p.q.vocab, w.stride, 64, ttt::kLceBNDual) ||
-      !p.map(&g.b[1], uw.p, p.q.dim, p.q.vocab, uw.stride, 64, ttt::kLceBNDual))
+  ttt::LceGemm g = p.gemm(0, pb.vocab);
+  g.seg_w = (a->uh != nullptr ? 1 : 0) | (a->uw != nullptr ? 2 : 0);
+  if (!p.map_rows(&g.a[0], p.st.hc) || !p.map_rows(&g.a[1], p.w.uc) ||
+      !p.map_weight(&g.b[0], w, g, ttt::kLceBNDual) || !p.map_weight(&g.b[1], uw, g, ttt::kLceBNDual))
     return TTT_ERR_TENSOR_MAP;
   TTT_TRY(p.run(g, ttt::kLceDualStats));
   const int parts = 2 * static_cast<int>((pb.vocab + ttt::kLceBNDual - 1) / ttt::kLceBNDual);
-  lce_rho_kernel<<<static_cast<unsigned>(p.q.n_pad / 32), 256, 0, s>>>(p.st, p.w.part, p.w.ztgt, p.w.coef, parts,
-                                                                       g.n_pad, pb.reduction, p.w.rho, p.w.scale,
-                                                                       p.w.rows, a->gdloss);
-  TTT_TRY(launched());
-  lce_scale_kernel<<<1, 1, 0, s>>>(p.w.scale);
-  TTT_TRY(launched());
-  if (a->gdloss != nullptr) {
-    if (pb.reduction == TTT_LCE_NONE)
-      lce_zero_rows_kernel<<<static_cast<unsigned>((pb.n + 255) / 256), 256, 0, s>>>(p.st.slot, pb.n, a->gdloss);
-    else
-      lce_total_kernel<<<1, 1024, 0, s>>>(p.st.head, p.w.rows, a->gdloss);
+  TTT_TRY(launch_early(lce_rho_kernel, p.q.n_pad / 32, 32 * kShares, s, p.st, p.w.part, p.w.ztgt, p.w.coef, parts,
+                       g.n_pad, pb.reduction, p.w.rho, p.w.counters, p.w.sums, a->gdloss));
+  if (a->gdloss != nullptr && pb.reduction == TTT_LCE_NONE) {
+    lce_zero_rows_kernel<<<static_cast<unsigned>((pb.n + 255) / 256), 256, 0, s>>>(p.st.slot, pb.n, a->gdloss);
     TTT_TRY(launched());
   }
   return run_pieces(p, w, a->uw != nullptr ? &uw : nullptr, true, a->uh != nullptr, static_cast<uint16_t*>(a->gh),

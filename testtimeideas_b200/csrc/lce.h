@@ -11,56 +11,77 @@ namespace ttt {
 
 // Head of the state buffer, written by the forward.
 struct LceHead {
-  int n_active;  // participating rows, listed first
-  float denom;   // N of the mean, 1 otherwise
-};
-// Head of the work space of a gradient.
-struct LceScale {
-  float scale;        // power of two that the stored derivatives carry
-  float inv;          // 1 / scale
-  unsigned max_bits;  // second gradient: bits of the largest |stored value| / scale
+  int n_active;     // participating rows, listed first
+  float denom;      // N of the mean, 1 otherwise
+  float mw_max;     // largest |mask weight| of the participating rows
+  unsigned ticket;  // blocks of the forward's last kernel that are done
 };
 
-// Tile sides. Rows of a tile are tokens (or, for the weight gradient, vocabulary
-// entries); the fp32 accumulators of a tile fill half of tensor memory, so that
-// one tile is formed while the previous one is read out.
-constexpr int kLceBM = 128;
-constexpr int kLceBN = 256;     // single-product tiles
-constexpr int kLceBNDual = 128; // two accumulators side by side
+// Where the row coefficients c of a gradient come from: listed (per-row upstream
+// gradients, and the second gradient), or formed from the one upstream value.
+struct LceCoef {
+  const LceHead* head;
+  const float* dloss;        // one value (unused when coef is set)
+  const float* mw;           // mask weights by slot
+  const float* coef;         // c by slot, or null
+  const unsigned* max_bits;  // with coef: bits of the largest magnitude to store
+
+  __device__ __forceinline__ float row(int slot) const {
+    return coef != nullptr ? coef[slot] : *dloss * (mw[slot] / head->denom);
+  }
+  // Power of two that brings the largest magnitude to store near 2^13 (1 for 0, inf and NaN).
+  __device__ __forceinline__ float scale() const {
+    const float big = coef != nullptr ? __uint_as_float(*max_bits) : fabsf(*dloss) * (head->mw_max / head->denom);
+    if (!(big > 0.f && big < INFINITY)) return 1.f;
+    int e;
+    frexpf(big, &e);  // big < 2^e
+    return ldexpf(1.f, max(-100, min(100, 13 - e)));
+  }
+};
+
+// A tile is formed by a pair of CTAs: 256 rows, 128 in each CTA. Rows are tokens
+// or, for the weight gradient, vocabulary entries. The fp32 accumulators of a tile
+// fill half of each CTA's tensor memory, so that one tile is formed while the
+// previous one is read out.
+constexpr int kLceBM = 256;
+constexpr int kLceBN = 256;      // single-product tiles
+constexpr int kLceBNDual = 128;  // two accumulators side by side
 constexpr int kLceBK = 64;
 
 enum LceKind : int {
-  kLceStats = 0,      // z -> per-row (max, sum) of the tile, z at the target
+  kLceStats = 0,      // z -> per-row (max, sum) of the half tile, z at the target
   kLceGrad = 1,       // z -> G
-  kLceDualStats = 2,  // z, A -> per-row sum P A of the tile, its largest |P A|, A at the target
+  kLceDualStats = 2,  // z, A -> per-row sum P A of the half tile, its largest |P A|, A at the target
   kLceDualGrad = 3,   // z, A -> G, D
-  kLceDH = 4,         // G w (+ D w + G uw): fp32 partial rows
-  kLceDW = 5,         // G^T h (+ D^T h + G^T uh): 16-bit rows of the weight gradient
+  kLceProd = 4,       // G w (+ D w + G uw) as fp32 partial rows, and G^T h (+ D^T h + G^T uh) as 16-bit rows
 };
 
 struct LceGemm {
-  // Operand maps. Logit kinds: a = {h, uh}, b = {w, uw}, K-major. kLceDH: per
-  // segment a = stored derivative (K-major), b = w or uw (MN-major). kLceDW: per
-  // segment a = stored derivative (MN-major), b = h or uh (MN-major).
+  // Logit kinds: a = {h, uh}, b = {w, uw}, K-major operands.
   CUtensorMap a[2], b[2];
   CUtensorMap out[2];  // logit gradient kinds: stores of G and D
+  // kLceProd, per product: the stored derivative as K-major (gk) and MN-major (gm)
+  // operand, and what it meets, MN-major: w or uw (bw), h or uh (bh).
+  CUtensorMap gk[2], gm[2], bw[2], bh[2];
+  CUtensorMap dw_out;  // kLceProd: stores of the weight gradient's rows (when dim % 8 == 0)
   const LceHead* head;
-  const LceScale* scale;
+  LceCoef coef;
   // rows of the state / work arrays, indexed by row slot
   const int* tgt;
   const float* lse2;
-  const float* coef;
   const float* rho;
-  float2* part;  // statistics kinds: [2 * n_tiles][n_pad]
-  float* ztgt;   // statistics kinds: value at the target
-  float* acc;    // kLceDH: [splits][n_pad][dim_pad]
-  uint16_t* dw;  // kLceDW: row 0 of the piece, [cols][dim]
-  int n_pad;     // row slots (multiple of 128)
+  float2* part;      // statistics kinds: [2 * n_tiles][n_pad]
+  float* ztgt;       // statistics kinds: value at the target
+  float* acc;        // kLceProd: [splits][n_pad][dim_pad], or null (no hidden gradient)
+  uint16_t* dw;      // kLceProd: row 0 of the piece, [cols][dim], or null (no weight gradient)
+  unsigned* ticket;  // next tile of the following kLceProd launch (zeroed by the gradient kinds)
+  int n_pad;         // row slots (multiple of 256)
   int dim, dim_pad;
-  int col0, cols;  // the vocabulary piece
-  int seg_mask;    // segments (products) in use: bit 0, bit 1
-  int splits;      // kLceDH: shares of the piece's columns
-  int accumulate;  // kLceDH: add to acc instead of overwriting it
+  int col0, cols;    // the vocabulary piece
+  int seg_w, seg_h;  // kLceProd: products in use (bits) of the hidden and of the weight gradient;
+                     // dual kinds: seg_w bit 0 uh given, bit 1 uw given
+  int splits;        // kLceProd: shares of the piece's columns in the hidden gradient
+  int accumulate;    // kLceProd: add to acc instead of overwriting it
   int* err;
   int* err_host;
 };

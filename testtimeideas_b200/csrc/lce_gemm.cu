@@ -1,16 +1,23 @@
 // Tensor-core kernels of the linear cross entropy (see lce.h for the kinds and
 // include/ttt_ops.h for the formulas).
 //
-// One persistent kernel template: each CTA walks a list of output tiles;
+// One persistent kernel template for pairs of CTAs (clusters of two): a pair forms
+// 256-row tiles with tcgen05.mma over both SMs (cta_group::2), so that each CTA
+// stages its own 128 rows of A and only half of B. That halves the shared-memory
+// and L2 traffic of B, which is what bounds the same tiles on single CTAs.
 //   warps 0..7  epilogue: warp w owns TMEM lanes 32*(w%4)..+31 (one tile row per
 //               thread) and one half of the tile's columns (w/4)
-//   warp 8      TMA producer of the operand ring
-//   warp 9      MMA issuer, into one of two accumulator buffers in TMEM, so that
-//               a tile's products run while the previous tile is read out
-// The logits never leave the chip: the statistics kinds reduce them to two
-// floats per row and half tile, the gradient kinds turn them into the 16-bit
-// derivative of the logits of one piece of the vocabulary, which the product
-// kinds contract with w and h.
+//   warp 8      TMA producer of this CTA's operands; all bytes of a stage arrive on
+//               the leader's (even CTA's) barrier
+//   warp 9      leader only: MMA issuer, into one of two accumulator buffers in
+//               TMEM, so that a tile's products run while the previous one is read
+//   warp 10     kLceProd, leader only: hands out tiles from a global counter. Its
+//               two kinds of tiles differ in length by up to a factor of ten; taken
+//               in order of length by whichever pair is free, all pairs end within
+//               one short tile. Which pair forms a tile does not change its value.
+// The logits never leave the chip: the statistics kinds reduce them to two floats
+// per row and half tile, the gradient kinds turn them into the 16-bit derivative of
+// the logits of one piece of the vocabulary, which kLceProd contracts with w and h.
 #include "attn_pipe.cuh"
 #include "lce.h"
 
@@ -19,6 +26,68 @@ namespace ttt {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+// ---------------------------------------------------------------- pair-of-CTAs helpers
+TTT_DEV uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Address of this CTA's shared variable `p` in CTA `rank` of the pair.
+TTT_DEV uint32_t peer_addr(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+TTT_DEV void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+TTT_DEV int ld_peer(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+TTT_DEV void st_peer(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+TTT_DEV void arrive_peer(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// Acquire at pair scope, for data written by the other CTA before its arrival.
+TTT_DEV void acquire_pair() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+
+// 2-D tiled load into this CTA's shared memory, its bytes counted on a barrier of the pair.
+TTT_DEV void load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+TTT_DEV void umma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrive on `bar` of both CTAs when every product issued so far has completed.
+TTT_DEV void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+TTT_DEV void tmem_alloc_pair(uint32_t* dst, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+TTT_DEV void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
 
 TTT_DEV void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
@@ -37,177 +106,232 @@ TTT_DEV float tmem_ld1(uint32_t taddr) {
   return __uint_as_float(r);
 }
 
-// Named barrier over the 128 threads of one column half.
-TTT_DEV void half_bar(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }
-// The same with a vote: true if every thread's ok is (so that all leave together).
-TTT_DEV bool half_all(int half, bool ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\t"
-      "barrier.cta.red.and.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
-      : "=r"(r)
-      : "r"(1 + half), "r"(ok ? 1u : 0u)
-      : "memory");
-  return r != 0;
-}
-
 template <int KIND>
 struct LceCfg {
-  static constexpr bool LOGIT = KIND <= kLceDualGrad;
+  static constexpr bool LOGIT = KIND != kLceProd;
   static constexpr bool DUAL = KIND == kLceDualStats || KIND == kLceDualGrad;
   static constexpr bool GRAD = KIND == kLceGrad || KIND == kLceDualGrad;
   static constexpr int BM = kLceBM, BN = DUAL ? kLceBNDual : kLceBN, BK = kLceBK;
-  static constexpr int TILE_A = BM * BK * 2, TILE_B = BN * BK * 2;
+  static constexpr int ROWS_A = BM / 2, ROWS_B = BN / 2;  // of a CTA
+  static constexpr int TILE_A = ROWS_A * BK * 2, TILE_B = ROWS_B * BK * 2;
   static constexpr int STAGE = (DUAL ? 2 : 1) * (TILE_A + TILE_B);
-  static constexpr int NSTAGE = DUAL ? 3 : 4;
-  static constexpr int PANEL = BM * 128;  // staging of one [128 x 64] 16-bit store box
+  static constexpr int NSTAGE = 196608 / STAGE;  // 192 KB: 6 single or 4 dual stages
+  static constexpr int PANEL = 32 * 128;         // staging of one warp's [32 x 64] 16-bit store box
   static constexpr int OFF_STORE = NSTAGE * STAGE;
-  static constexpr int OFF_BAR = OFF_STORE + 2 * PANEL;
-  static constexpr int NBAR = 2 * NSTAGE + 5;
-  static constexpr int SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
-  static constexpr int NTHREADS = 320, WARP_LOAD = 8, WARP_MMA = 9;
+  static constexpr int OFF_BAR = OFF_STORE + 8 * PANEL;
+  static constexpr int NBAR = 2 * NSTAGE + 9;
+  static constexpr int SMEM = OFF_BAR + NBAR * 8 + 32 + 1024;
+  static constexpr int NTHREADS = 352, WARP_LOAD = 8, WARP_MMA = 9, WARP_SCHED = 10;
   static constexpr int HALF = BN / 2;  // columns (of each accumulator) per epilogue half
   static_assert(SMEM <= 232448, "tile set exceeds shared memory");
 };
 
-// Tile t of the list, and its contraction range [k0, k1) in 64-wide steps.
+// A tile of the list and its contraction range [k0, k1) in 64-wide steps.
 struct LceTile {
   int m, n, split, k0, k1;
+  bool dw;  // kLceProd: a tile of the weight gradient
 };
 
+struct LceSizes {
+  int mt, dt, kt, nk, n_dh, n_dw, n_tiles;
+  bool dw_first;
+};
 template <int KIND>
-TTT_DEV int lce_tiles(const LceGemm& p, int n_active) {
+TTT_DEV LceSizes lce_sizes(const LceGemm& p, int n_active) {
   using C = LceCfg<KIND>;
-  const int mt = (n_active + C::BM - 1) / C::BM, dt = (p.dim + C::BN - 1) / C::BN;
-  if constexpr (C::LOGIT) return mt * ((p.cols + C::BN - 1) / C::BN);
-  if constexpr (KIND == kLceDH) return mt * dt * p.splits;
-  return ((p.cols + C::BM - 1) / C::BM) * dt;
+  LceSizes s;
+  s.mt = (n_active + C::BM - 1) / C::BM;
+  s.dt = (p.dim + C::BN - 1) / C::BN;
+  s.kt = (p.cols + C::BK - 1) / C::BK;   // steps over the piece's columns
+  s.nk = (n_active + C::BK - 1) / C::BK; // steps over the rows
+  if constexpr (C::LOGIT) {
+    s.n_tiles = s.mt * ((p.cols + C::BN - 1) / C::BN);
+  } else {
+    s.n_dh = p.acc != nullptr ? s.mt * s.dt * p.splits : 0;
+    s.n_dw = p.dw != nullptr ? ((p.cols + C::BM - 1) / C::BM) * s.dt : 0;
+    s.n_tiles = s.n_dh + s.n_dw;
+    s.dw_first = s.nk * __popc(p.seg_h) > s.kt / p.splits * __popc(p.seg_w);  // longer tiles first
+  }
+  return s;
 }
 template <int KIND>
-TTT_DEV LceTile lce_tile(const LceGemm& p, int n_active, int t) {
+TTT_DEV LceTile lce_tile(const LceGemm& p, const LceSizes& s, int t) {
   using C = LceCfg<KIND>;
-  const int mt = (n_active + C::BM - 1) / C::BM, dt = (p.dim + C::BN - 1) / C::BN;
   if constexpr (C::LOGIT) {
-    // token tiles fastest: the CTAs running together share a few vocabulary tiles
-    return {t % mt, t / mt, 0, 0, (p.dim + C::BK - 1) / C::BK};
-  } else if constexpr (KIND == kLceDH) {
-    const int s = t / (dt * mt), kt = (p.cols + C::BK - 1) / C::BK;
-    return {(t / dt) % mt, t % dt, s, split_begin(kt, s, p.splits), split_begin(kt, s + 1, p.splits)};
+    // token tiles fastest: the pairs running together share a few vocabulary tiles
+    return {t % s.mt, t / s.mt, 0, 0, (p.dim + C::BK - 1) / C::BK, false};
   } else {
-    return {t / dt, t % dt, 0, 0, (n_active + C::BK - 1) / C::BK};
+    const bool dw = s.dw_first ? t < s.n_dw : t >= s.n_dh;
+    const int i = dw ? (s.dw_first ? t : t - s.n_dh) : (s.dw_first ? t - s.n_dw : t);
+    if (dw) return {i / s.dt, i % s.dt, 0, 0, s.nk, true};
+    const int sp = i / (s.dt * s.mt);
+    return {(i / s.dt) % s.mt, i % s.dt, sp, split_begin(s.kt, sp, p.splits), split_begin(s.kt, sp + 1, p.splits),
+            false};
   }
 }
 
-// Packs 64 columns of a row into the half's staging panel and stores the
-// panel's box at (x, y); all 128 threads of the half call this.
+// Walks the tiles of this pair: a fixed stride, or (kLceProd) what the scheduler
+// warp hands out through a two-entry ring in both CTAs' shared memory. Used by one
+// warp (the epilogue) or one thread (producer, issuer).
+template <int KIND>
+struct LceWalk {
+  int i = 0, pairs, pair, n_tiles;
+  volatile int* ring;
+  uint64_t* full;
+  uint32_t empty_leader;  // address of the leader's sched_empty[0]
+  // The next tile, or -1 at the end (or when aborting). WARP: called by a whole warp.
+  template <bool WARP>
+  TTT_DEV int next(const Guard& g) {
+    if constexpr (KIND != kLceProd) {
+      const int t = pair + i * pairs;
+      ++i;
+      return t < n_tiles ? t : -1;
+    } else {
+      const int slot = i & 1;
+      bool ok = mbar_wait(full + slot, (i >> 1) & 1, g, 0x55);
+      if constexpr (WARP) ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return -1;
+      acquire_pair();
+      const int t = ring[slot];
+      if constexpr (WARP) __syncwarp();  // every lane has read the entry
+      if (!WARP || (threadIdx.x & 31) == 0) arrive_peer(empty_leader + slot * 8);
+      ++i;
+      return t < n_tiles ? t : -1;
+    }
+  }
+};
+
+// Packs 64 columns of this warp's 32 rows into its staging panel and stores the box at (x, y).
 template <bool BF16>
-TTT_DEV void store_panel(uint8_t* panel, const CUtensorMap* map, int half, int r, int x, int y, const float (&v)[64]) {
+TTT_DEV void store_panel(uint8_t* panel, const CUtensorMap* map, int lane, int x, int y, const float (&v)[64]) {
   uint32_t w[32];
 #pragma unroll
   for (int j = 0; j < 32; ++j) w[j] = pack2<BF16>(v[2 * j], v[2 * j + 1]);
-  if (r == 0) bulk_wait_read();  // the previous store has left the panel
-  half_bar(half);
+  if (lane == 0) bulk_wait_read();  // the previous store has left the panel
+  __syncwarp();
 #pragma unroll
   for (int ch = 0; ch < 8; ++ch)
-    *reinterpret_cast<uint4*>(panel + r * 128 + ((ch ^ (r & 7)) << 4)) =
+    *reinterpret_cast<uint4*>(panel + lane * 128 + ((ch ^ (lane & 7)) << 4)) =
         make_uint4(w[4 * ch], w[4 * ch + 1], w[4 * ch + 2], w[4 * ch + 3]);
   fence_async_smem();
-  half_bar(half);
-  if (r == 0) {
+  __syncwarp();
+  if (lane == 0) {
     tma_store_2d(map, panel, x, y);
     bulk_commit();
   }
 }
 
 template <int KIND, bool BF16>
-__global__ void __launch_bounds__(LceCfg<KIND>::NTHREADS, 1) lce_gemm_kernel(const __grid_constant__ LceGemm p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREADS, 1)
+    lce_gemm_kernel(const __grid_constant__ LceGemm p) {
   using C = LceCfg<KIND>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  uint64_t* full = bars;                       // [NSTAGE] TMA -> MMA
-  uint64_t* empty = bars + C::NSTAGE;          // [NSTAGE] MMA -> TMA
-  uint64_t* acc_full = bars + 2 * C::NSTAGE;   // [2] MMA -> epilogue
-  uint64_t* acc_free = acc_full + 2;           // [2] epilogue (256 arrivals) -> MMA
-  uint64_t* drain = acc_full + 4;              // MMA issuer's last commit
+  uint64_t* full = bars;                      // [NSTAGE] leader's: both CTAs' loads -> MMA
+  uint64_t* empty = bars + C::NSTAGE;         // [NSTAGE] each CTA's: MMA -> its producer
+  uint64_t* acc_full = bars + 2 * C::NSTAGE;  // [2] each CTA's: MMA -> its epilogue
+  uint64_t* acc_free = acc_full + 2;          // [2] leader's: 16 epilogue warps -> MMA
+  uint64_t* drain = acc_full + 4;             // each CTA's: the issuer's last commit
+  uint64_t* sched_full = acc_full + 5;        // [2] each CTA's: scheduler -> its warps
+  uint64_t* sched_empty = acc_full + 7;       // [2] leader's: 19 readers -> scheduler
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::NBAR);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* ring = reinterpret_cast<volatile int*>(tmem_slot + 2);  // [2]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cta_rank();
+  asm volatile("griddepcontrol.launch_dependents;");
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::NBAR; ++i) mbar_init(bars + i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(acc_free + i, 256);
-    *abort_flag = (p.err != nullptr && *reinterpret_cast<volatile int*>(p.err) != 0) ? 1 : 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_free + i, 16);
+      mbar_init(sched_empty + i, 19);
+    }
     fence_mbar_init();
   }
-  __syncthreads();
-  if (*abort_flag) return;
-  if (warp == 0) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
-  }
+  __syncwarp();
+  if (warp == 0) tmem_alloc_pair(tmem_slot, 512);
+  // everything below reads what earlier kernels of the stream wrote
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (threadIdx.x == 0) *abort_flag = (p.err != nullptr && *reinterpret_cast<volatile int*>(p.err) != 0) ? 1 : 0;
   tc_fence_before();
   __syncthreads();
+  pair_sync();
   tc_fence_after();
+  // both CTAs work or neither does
+  const bool go = *abort_flag == 0 && ld_peer(peer_addr(const_cast<const int*>(abort_flag), rank ^ 1)) == 0;
+  pair_sync();
   const uint32_t tmem = *tmem_slot;
   Guard g{abort_flag, p.err, p.err_host};
   const int n_active = p.head->n_active;
-  const int n_tiles = lce_tiles<KIND>(p, n_active);
-  const bool seg0 = (p.seg_mask & 1) != 0, seg1 = (p.seg_mask & 2) != 0;
+  const LceSizes sz = lce_sizes<KIND>(p, n_active);
+  LceWalk<KIND> walk;
+  walk.pairs = static_cast<int>(gridDim.x) >> 1;
+  walk.pair = static_cast<int>(blockIdx.x) >> 1;
+  walk.n_tiles = sz.n_tiles;
+  walk.ring = ring;
+  walk.full = sched_full;
+  walk.empty_leader = peer_addr(sched_empty, 0);
+  const bool seg0 = (p.seg_w & 1) != 0, seg1 = (p.seg_w & 2) != 0;  // dual kinds
+  if (C::GRAD && go && blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;  // for the products that follow
 
-  if (warp == C::WARP_LOAD) {
+  if (go && warp == C::WARP_LOAD) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
-      const uint32_t dual_bytes = 16384u * (2 + (seg0 ? 1 : 0) + (seg1 ? 1 : 0));
+      const uint32_t dual_bytes = 2u * (C::TILE_A * (seg0 ? 2 : 1) + C::TILE_B * (seg1 ? 2 : 1));
+      const int row_a = static_cast<int>(rank) * C::ROWS_A, row_b = static_cast<int>(rank) * C::ROWS_B;
       int it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < n_tiles; t += gridDim.x) {
-        const LceTile tl = lce_tile<KIND>(p, n_active, t);
-        for (int seg = 0; ok && seg < (C::LOGIT ? 1 : 2); ++seg) {
-          if (!C::LOGIT && !(seg == 0 ? seg0 : seg1)) continue;
+      for (int t; ok && (t = walk.template next<false>(g)) >= 0;) {
+        const LceTile tl = lce_tile<KIND>(p, sz, t);
+        const int segs = C::LOGIT ? 1 : (tl.dw ? p.seg_h : p.seg_w);
+        for (int seg = 0; ok && seg < 2; ++seg) {
+          if (!(segs >> seg & 1)) continue;
           for (int k = tl.k0; k < tl.k1; ++k, ++it) {
             const int s = it % C::NSTAGE;
             if (it >= C::NSTAGE && !(ok = mbar_wait(empty + s, ((it / C::NSTAGE) - 1) & 1, g, 0x51))) break;
             uint8_t* st = smem + s * C::STAGE;
-            if constexpr (C::DUAL) {
-              mbar_arrive_tx(full + s, dual_bytes);
-              tma_load_2d(st, &p.a[0], full + s, k * C::BK, tl.m * C::BM);
-              if (seg0) tma_load_2d(st + C::TILE_A, &p.a[1], full + s, k * C::BK, tl.m * C::BM);
-              tma_load_2d(st + 2 * C::TILE_A, &p.b[0], full + s, k * C::BK, tl.n * C::BN);
-              if (seg1)
-                tma_load_2d(st + 2 * C::TILE_A + C::TILE_B, &p.b[1], full + s, k * C::BK, tl.n * C::BN);
+            uint8_t* stb = st + (C::DUAL ? 2 : 1) * C::TILE_A;
+            if (rank == 0) mbar_arrive_tx(full + s, C::DUAL ? dual_bytes : 2u * C::STAGE);
+            const uint32_t bar = peer_addr(full + s, 0);
+            const int kc = k * C::BK;
+            if constexpr (C::LOGIT) {
+              load_pair(st, &p.a[0], bar, kc, tl.m * C::BM + row_a);
+              load_pair(stb, &p.b[0], bar, kc, tl.n * C::BN + row_b);
+              if constexpr (C::DUAL) {
+                if (seg0) load_pair(st + C::TILE_A, &p.a[1], bar, kc, tl.m * C::BM + row_a);
+                if (seg1) load_pair(stb + C::TILE_B, &p.b[1], bar, kc, tl.n * C::BN + row_b);
+              }
             } else {
-              mbar_arrive_tx(full + s, C::STAGE);
-              if constexpr (KIND == kLceDW) {
+              if (tl.dw) {
                 for (int q = 0; q < 2; ++q)
-                  tma_load_2d(st + q * 8192, &p.a[seg], full + s, tl.m * C::BM + q * 64, k * C::BK);
+                  load_pair(st + q * 8192, &p.gm[seg], bar, tl.m * C::BM + row_a + q * 64, kc);
               } else {
-                tma_load_2d(st, &p.a[seg], full + s, k * C::BK, tl.m * C::BM);
+                load_pair(st, &p.gk[seg], bar, kc, tl.m * C::BM + row_a);
               }
-              if constexpr (C::LOGIT) {
-                tma_load_2d(st + C::TILE_A, &p.b[0], full + s, k * C::BK, tl.n * C::BN);
-              } else {
-                for (int q = 0; q < 4; ++q)
-                  tma_load_2d(st + C::TILE_A + q * 8192, &p.b[seg], full + s, tl.n * C::BN + q * 64, k * C::BK);
-              }
+              const CUtensorMap* b = tl.dw ? &p.bh[seg] : &p.bw[seg];
+              for (int q = 0; q < 2; ++q) load_pair(stb + q * 8192, b, bar, tl.n * C::BN + row_b + q * 64, kc);
             }
           }
         }
       }
-      for (int j = max(0, it - C::NSTAGE); j < it; ++j) mbar_drain(full + j % C::NSTAGE, (j / C::NSTAGE) & 1);
+      if (rank == 0)
+        for (int j = max(0, it - C::NSTAGE); j < it; ++j) mbar_drain(full + j % C::NSTAGE, (j / C::NSTAGE) & 1);
     }
-  } else if (warp == C::WARP_MMA) {
+  } else if (go && warp == C::WARP_MMA && rank == 0) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {
-      constexpr bool A_MN = KIND == kLceDW, B_MN = !C::LOGIT;
-      constexpr uint32_t idesc = idesc_f16(C::BM, C::BN, BF16, A_MN, B_MN);
-      auto da = [](uint32_t tile, int kk) { return A_MN ? desc_mnmajor(tile, C::BK, kk) : desc_kmajor(tile, C::BM, kk); };
-      auto db = [](uint32_t tile, int kk) { return B_MN ? desc_mnmajor(tile, C::BK, kk) : desc_kmajor(tile, C::BN, kk); };
+      constexpr bool B_MN = !C::LOGIT;
+      constexpr uint32_t id_k = idesc_f16(C::BM, C::BN, BF16, false, B_MN), id_mn = idesc_f16(C::BM, C::BN, BF16, true, B_MN);
+      auto db = [](uint32_t tile, int kk) {
+        return B_MN ? desc_mnmajor(tile, C::BK, kk) : desc_kmajor(tile, C::ROWS_B, kk);
+      };
       int it = 0, nth = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < n_tiles; t += gridDim.x) {
-        const LceTile tl = lce_tile<KIND>(p, n_active, t);
-        const int steps = (tl.k1 - tl.k0) * (C::LOGIT ? 1 : (seg0 ? 1 : 0) + (seg1 ? 1 : 0));
+      for (int t; ok && (t = walk.template next<false>(g)) >= 0;) {
+        const LceTile tl = lce_tile<KIND>(p, sz, t);
+        const int steps = (tl.k1 - tl.k0) * (C::LOGIT ? 1 : __popc(tl.dw ? p.seg_h : p.seg_w));
         if (steps == 0) continue;  // the epilogue writes zeros by itself
         const int buf = nth & 1;
         if (nth >= 2 && !(ok = mbar_wait(acc_free + buf, ((nth >> 1) - 1) & 1, g, 0x52))) break;
@@ -220,54 +344,78 @@ __global__ void __launch_bounds__(LceCfg<KIND>::NTHREADS, 1) lce_gemm_kernel(con
           if constexpr (C::DUAL) {
             const uint32_t a0 = st, a1 = st + C::TILE_A, b0 = st + 2 * C::TILE_A, b1 = b0 + C::TILE_B;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) umma_ss(d, da(a0, kk), db(b0, kk), idesc, (k | kk) ? 1u : 0u);
+            for (int kk = 0; kk < 4; ++kk)
+              umma_pair(d, desc_kmajor(a0, C::ROWS_A, kk), db(b0, kk), id_k, (k | kk) ? 1u : 0u);
             if (seg0) {
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk) umma_ss(d + C::BN, da(a1, kk), db(b0, kk), idesc, (k | kk) ? 1u : 0u);
+              for (int kk = 0; kk < 4; ++kk)
+                umma_pair(d + C::BN, desc_kmajor(a1, C::ROWS_A, kk), db(b0, kk), id_k, (k | kk) ? 1u : 0u);
             }
             if (seg1) {
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk)
-                umma_ss(d + C::BN, da(a0, kk), db(b1, kk), idesc, (seg0 || (k | kk)) ? 1u : 0u);
+                umma_pair(d + C::BN, desc_kmajor(a0, C::ROWS_A, kk), db(b1, kk), id_k, (seg0 || (k | kk)) ? 1u : 0u);
             }
+          } else if (!C::LOGIT && tl.dw) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_pair(d, desc_mnmajor(st, C::BK, kk), db(st + C::TILE_A, kk), id_mn, (k | kk) ? 1u : 0u);
           } else {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma_ss(d, da(st, kk), db(st + C::TILE_A, kk), idesc, (k | kk) ? 1u : 0u);
+              umma_pair(d, desc_kmajor(st, C::ROWS_A, kk), db(st + C::TILE_A, kk), id_k, (k | kk) ? 1u : 0u);
           }
-          umma_commit(empty + s);
+          commit_pair(empty + s);
         }
         if (!ok) break;
-        umma_commit(acc_full + buf);
+        commit_pair(acc_full + buf);
         ++nth;
       }
-      umma_commit(drain);
+      commit_pair(drain);
       mbar_drain(drain, 0);
     }
-  } else {
+  } else if (KIND == kLceProd && go && warp == C::WARP_SCHED && rank == 0) {
+    // ------------------------------------------------------------ tile scheduler
+    if (lane == 0) {
+      const uint32_t ring_peer = peer_addr(const_cast<const int*>(ring), 1), full_peer = peer_addr(sched_full, 1);
+      for (int i = 0;; ++i) {
+        const int slot = i & 1;
+        if (i >= 2 && !mbar_wait(sched_empty + slot, ((i >> 1) - 1) & 1, g, 0x56)) break;
+        const int t = static_cast<int>(min(atomicAdd(p.ticket, 1u), 0x7fffffffu));
+        ring[slot] = t;
+        st_peer(ring_peer + slot * 4, t);
+        mbar_arrive(sched_full + slot);
+        arrive_peer(full_peer + slot * 8);
+        if (t >= sz.n_tiles) break;
+      }
+    }
+  } else if (go && warp < 8) {
     // ------------------------------------------------------------ epilogue
     const int quarter = warp & 3, half = warp >> 2;
-    const int r = quarter * 32 + lane;
+    const int r = static_cast<int>(rank) * C::ROWS_A + quarter * 32 + lane;  // row of the tile
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    uint8_t* panel = smem + C::OFF_STORE + half * C::PANEL;
-    const float inv = (KIND == kLceDW) ? p.scale->inv : 1.f;
-    const float mul = C::GRAD ? p.scale->scale : 1.f;
+    uint8_t* panel = smem + C::OFF_STORE + warp * C::PANEL;
+    const uint32_t free_leader = peer_addr(acc_free, 0);
+    const float mul = C::GRAD ? p.coef.scale() : (KIND == kLceProd ? 1.f / p.coef.scale() : 1.f);
     int nth = 0;
-    for (int t = blockIdx.x; t < n_tiles; t += gridDim.x) {
-      const LceTile tl = lce_tile<KIND>(p, n_active, t);
-      const bool have = tl.k1 > tl.k0 && (C::LOGIT || p.seg_mask != 0);
+    for (int t; (t = walk.template next<true>(g)) >= 0;) {
+      const LceTile tl = lce_tile<KIND>(p, sz, t);
+      const bool have = tl.k1 > tl.k0 && (C::LOGIT || (tl.dw ? p.seg_h : p.seg_w) != 0);
       const int buf = nth & 1;
-      bool ok = true;
       if (have) {
-        ok = mbar_wait(acc_full + buf, (nth >> 1) & 1, g, 0x54);
+        if (!__all_sync(0xffffffffu, mbar_wait(acc_full + buf, (nth >> 1) & 1, g, 0x54))) break;
         ++nth;
       }
-      if constexpr (C::GRAD) ok = half_all(half, ok);
-      if (!ok) break;
       tc_fence_after();
+      // the accumulators are in registers: the issuer may use the buffer again
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_peer(free_leader + buf * 8);
+      };
       const uint32_t acc = tmem + lane_off + buf * 256 + half * C::HALF;
       const int slot = tl.m * C::BM + r;
-      const int c0 = tl.n * C::BN + half * C::HALF;  // first column within the piece (logit kinds)
+      const int c0 = tl.n * C::BN + half * C::HALF;  // first column of this half
 
       if constexpr (KIND == kLceStats) {
         const int target = p.tgt[slot] - p.col0;
@@ -302,8 +450,7 @@ __global__ void __launch_bounds__(LceCfg<KIND>::NTHREADS, 1) lce_gemm_kernel(con
           const float z = tmem_ld1(acc + col);
           if (lane == src) p.ztgt[slot] = z;
         }
-        tc_fence_before();
-        mbar_arrive(acc_free + buf);
+        release();
         p.part[static_cast<int64_t>(tl.n * 2 + half) * p.n_pad + slot] = make_float2(mx * kLog2e, sum);
       } else if constexpr (KIND == kLceDualStats) {
         const int target = p.tgt[slot] - p.col0;
@@ -330,13 +477,13 @@ __global__ void __launch_bounds__(LceCfg<KIND>::NTHREADS, 1) lce_gemm_kernel(con
           const float a = tmem_ld1(acc + C::BN + col);
           if (lane == src) p.ztgt[slot] = a;
         }
-        tc_fence_before();
-        mbar_arrive(acc_free + buf);
+        release();
         p.part[static_cast<int64_t>(tl.n * 2 + half) * p.n_pad + slot] = make_float2(sum, big);
       } else if constexpr (C::GRAD) {
         const int target = p.tgt[slot] - p.col0;
-        const float lse2 = p.lse2[slot], coef = p.coef[slot] * mul;
+        const float lse2 = p.lse2[slot], coef = slot < n_active ? p.coef.row(slot) * mul : 0.f;
         const float rho = C::DUAL ? p.rho[slot] : 0.f;
+        const int row0 = tl.m * C::BM + static_cast<int>(rank) * C::ROWS_A + quarter * 32;
 #pragma unroll 1
         for (int q = 0; q < C::HALF / 64; ++q) {
           float v[64];
@@ -351,14 +498,12 @@ __global__ void __launch_bounds__(LceCfg<KIND>::NTHREADS, 1) lce_gemm_kernel(con
             tmem_ld_nw<64>(acc + C::BN, d);
             tmem_wait_ld();
             reg_fence(d);
-            tc_fence_before();
-            mbar_arrive(acc_free + buf);
+            release();
 #pragma unroll
             for (int j = 0; j < 64; ++j) d[j] = coef * v[j] * (d[j] - rho);
-            store_panel<BF16>(panel, &p.out[1], half, r, cq, tl.m * C::BM, d);
+            store_panel<BF16>(panel, &p.out[1], lane, cq, row0, d);
           } else if (q == C::HALF / 64 - 1) {
-            tc_fence_before();
-            mbar_arrive(acc_free + buf);
+            release();
           }
           const bool here = target >= cq && target < cq + 64;
           if (__any_sync(0xffffffffu, here)) {
@@ -368,14 +513,15 @@ __global__ void __launch_bounds__(LceCfg<KIND>::NTHREADS, 1) lce_gemm_kernel(con
           }
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] *= coef;
-          store_panel<BF16>(panel, &p.out[0], half, r, cq, tl.m * C::BM, v);
+          store_panel<BF16>(panel, &p.out[0], lane, cq, row0, v);
         }
-      } else if constexpr (KIND == kLceDH) {
+      } else if (!tl.dw) {
         float* dst = p.acc + (static_cast<int64_t>(tl.split) * p.n_pad + slot) * p.dim_pad;
 #pragma unroll 1
         for (int q = 0; q < C::HALF / 32; ++q) {
           float v[32];
           tmem_ld32(acc + q * 32, v);
+          if (q == C::HALF / 32 - 1) release();
           const int cq = c0 + q * 32;
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
@@ -390,54 +536,55 @@ __global__ void __launch_bounds__(LceCfg<KIND>::NTHREADS, 1) lce_gemm_kernel(con
             }
           }
         }
-        tc_fence_before();
-        mbar_arrive(acc_free + buf);
       } else {
+        const bool boxes = (p.dim & 7) == 0;  // else the rows are not aligned for tensor-map stores
         const int row = tl.m * C::BM + r;
-        uint16_t* dst = p.dw + static_cast<int64_t>(row) * p.dim;
-        const bool wide = (p.dim & 7) == 0;
+        const int row0 = tl.m * C::BM + static_cast<int>(rank) * C::ROWS_A + quarter * 32;
 #pragma unroll 1
-        for (int q = 0; q < C::HALF / 32; ++q) {
-          float v[32];
+        for (int q = 0; q < C::HALF / 64; ++q) {
+          float v[64];
           if (have) {
-            tmem_ld32(acc + q * 32, v);
+            tmem_ld_nw<64>(acc + q * 64, v);
+            tmem_wait_ld();
+            reg_fence(v);
+            if (q == C::HALF / 64 - 1) release();
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0.f;
+            for (int j = 0; j < 64; ++j) v[j] = 0.f;
           }
-          const int cq = c0 + q * 32;
-          if (row < p.cols) {
+          const int cq = c0 + q * 64;
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              uint4 w;
-              w.x = pack2<BF16>(v[j] * inv, v[j + 1] * inv);
-              w.y = pack2<BF16>(v[j + 2] * inv, v[j + 3] * inv);
-              w.z = pack2<BF16>(v[j + 4] * inv, v[j + 5] * inv);
-              w.w = pack2<BF16>(v[j + 6] * inv, v[j + 7] * inv);
-              if (wide) {
-                if (cq + j < p.dim) *reinterpret_cast<uint4*>(dst + cq + j) = w;
-              } else {
-                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+          for (int j = 0; j < 64; ++j) v[j] *= mul;
+          if (cq >= p.dim || row0 >= p.cols) continue;
+          if (boxes) {
+            store_panel<BF16>(panel, &p.dw_out, lane, cq, row0, v);
+          } else if (row < p.cols) {
+            uint16_t* dst = p.dw + static_cast<int64_t>(row) * p.dim + cq;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  if (cq + j + e < p.dim) dst[cq + j + e] = static_cast<uint16_t>(u[e >> 1] >> ((e & 1) * 16));
-              }
+            for (int j = 0; j < 64; j += 2) {
+              const uint32_t w = pack2<BF16>(v[j], v[j + 1]);
+              if (cq + j < p.dim) dst[j] = static_cast<uint16_t>(w);
+              if (cq + j + 1 < p.dim) dst[j + 1] = static_cast<uint16_t>(w >> 16);
             }
           }
         }
-        if (have) {
-          tc_fence_before();
-          mbar_arrive(acc_free + buf);
-        }
       }
     }
-    if (C::GRAD && r == 0) bulk_wait_all();  // this thread's stores have completed
+    if (lane == 0) bulk_wait_all();  // this thread's stores have completed
   }
 
+  // No CTA leaves while the other may still signal its barriers. After an abort, a
+  // millisecond lets this CTA's own loads land before its shared memory is given up.
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag != 0 && go) {
+    const unsigned long long t0 = global_ns();
+    while (global_ns() - t0 < 1000000ull) {
+    }
+  }
+  pair_sync();
   tc_fence_after();
-  if (warp == 0) tmem_dealloc(tmem, 512);
+  if (warp == 0) tmem_dealloc_pair(tmem, 512);
 }
 
 template <int KIND, bool BF16>
@@ -446,8 +593,17 @@ cudaError_t launch_kind(const LceGemm& p, int sms, cudaStream_t stream) {
   auto kern = lce_gemm_kernel<KIND, BF16>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return e;
-  kern<<<sms, C::NTHREADS, C::SMEM, stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchAttribute early;  // the prologue may overlap the previous kernel's end (griddepcontrol.wait)
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(sms < 2 ? 2 : sms & ~1));
+  cfg.blockDim = dim3(C::NTHREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
 }  // namespace
@@ -461,8 +617,7 @@ cudaError_t launch_lce_gemm(const LceGemm& p, int kind, bool bf16, int sms, cuda
     TTT_LCE(kLceGrad)
     TTT_LCE(kLceDualStats)
     TTT_LCE(kLceDualGrad)
-    TTT_LCE(kLceDH)
-    TTT_LCE(kLceDW)
+    TTT_LCE(kLceProd)
   }
 #undef TTT_LCE
   return cudaErrorInvalidValue;
