@@ -128,6 +128,8 @@ typedef struct {
   const void* mask;       /* [n] of mask_kind, or NULL */
   float* loss;            /* [n] or [1] */
   void* state;
+  int32_t need_state; /* 0: no gradient will be asked for; state is then only scratch (a few rows take a
+                         shorter path), 1 otherwise */
   int32_t* err;
   void* work;
   int64_t work_bytes;

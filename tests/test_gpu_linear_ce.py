@@ -258,6 +258,37 @@ def test_small_probabilities_in_fp16():
     assert _norm(dw[1:], rw[1:]) <= 4 * U[torch.float16]
 
 
+@pytest.mark.parametrize("n,d,v", [(1, 8, 1), (1, 768, 32000), (2, 512, 63), (3, 8192, 65), (4, 1000, 4097),
+                                   (4, 100, 300), (5, 256, 1000), (1, 8200, 500)])
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_scores_without_gradients(n, d, v, dtype):
+    """Few rows without gradients (their own kernel up to four) agree with the definition and with
+    the path that keeps state, for each reduction, with a row left out and NaN in it."""
+    inp = _inputs(n, d, v, dtype, seed=n + d + v)
+    h = inp["h"].clone()
+    for mask in (None, "bool", "weights", "none"):
+        m = _mask(n, mask, seed=n)
+        if m is not None and mask != "none":
+            m[0] = 1
+            if n > 2:
+                m[1] = 0
+                h[1] = float("nan")
+        for reduction in ("none", "mean", "sum"):
+            loss = tb.linear_cross_entropy(h, inp["w"], inp["t"], m, reduction=reduction)
+            ref = _definition(inp["h"].double(), inp["w"].double(), inp["t"], m, reduction)
+            assert loss.shape == ref.shape
+            # up to 8192 products of |z| < 16 in fp32: 2^-24 sqrt(8192) 16 on average, as in LOSS_TOL
+            assert float((loss.double() - ref).abs().max()) <= 5 * LOSS_TOL * max(1.0, float(ref.abs().max()))
+            kept = tb.linear_cross_entropy(h.clone().requires_grad_(True), inp["w"], inp["t"], m, reduction=reduction)
+            assert float((loss - kept.detach()).abs().max()) <= 5 * LOSS_TOL * max(1.0, float(ref.abs().max()))
+        h = inp["h"].clone()
+    t = inp["t"].clone()
+    t[n - 1] = v
+    tb.linear_cross_entropy(inp["h"], inp["w"], t)
+    with pytest.raises(_lib.KernelError, match="target outside"):
+        _lib.check_device_errors()
+
+
 def test_large_logits():
     """Logits of several hundred: the running maximum keeps the exponentials finite; u per unit of logit
     error does not enter, as z is exact products summed in fp32 (256 * 2^-24 * 400 < 0.01 absolute)."""

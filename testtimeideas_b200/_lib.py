@@ -195,7 +195,7 @@ def _register_fakes() -> None:
         return x.new_empty(x.shape), x.new_empty(x.shape), gw
 
     @torch.library.register_fake("ttt::linear_ce")
-    def _lce(h, w, targets, mask, reduction, ignore_index):
+    def _lce(h, w, targets, mask, reduction, ignore_index, need_state):
         loss = h.new_empty(targets.shape if reduction == 0 else (), dtype=torch.float32)
         return loss, h.new_empty((_lce_state_bytes(targets.numel(), h.shape[-1]),), dtype=torch.uint8)
 

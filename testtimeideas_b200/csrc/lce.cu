@@ -39,7 +39,7 @@ namespace {
 using ttt::LceCoef;
 using ttt::LceHead;
 
-constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
 
 // ---------------------------------------------------------------- state and work layouts
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
@@ -118,6 +118,9 @@ Plan make_plan(const ttt_lce_problem& pb, int pass, int sms) {
   return q;
 }
 
+// Parts of the statistics: half tiles, or up to two blocks per SM of lce_score_kernel.
+int64_t score_parts(int64_t vocab) { return std::max<int64_t>(2 * ((vocab + ttt::kLceBN - 1) / ttt::kLceBN), 512); }
+
 struct Work {
   float2* part;        // statistics of half tiles, [2 * tiles][n_pad]
   float* ztgt;         // [n_pad]
@@ -136,8 +139,8 @@ int64_t work_layout(const Plan& q, int pass, void* base, Work* w) {
   const int64_t rows = q.n_pad, mat = rows * q.dim_pad;
   t.counters = a.take<unsigned>(3);
   if (pass != 1) {
-    const int bn = pass == 0 ? ttt::kLceBN : ttt::kLceBNDual;
-    t.part = a.take<float2>(2 * ((q.vocab + bn - 1) / bn) * rows);
+    const int64_t parts = pass == 0 ? score_parts(q.vocab) : 2 * ((q.vocab + ttt::kLceBNDual - 1) / ttt::kLceBNDual);
+    t.part = a.take<float2>(parts * rows);
     t.ztgt = a.take<float>(rows);
     t.rows = a.take<float>(rows);
     t.sums = a.take<float>(rows / 32);
@@ -380,7 +383,11 @@ __global__ void __launch_bounds__(32 * kShares) lce_lse_kernel(const State st, c
   if (share != 0) return;
   float v = 0.f;
   if (s < n_active) {
-    for (int i = 1; i < kShares; ++i) merge(sh[i][lane]);
+    for (int i = 1; i < kShares; ++i) m = fmaxf(m, sh[i][lane].x);
+    const float sub = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < kShares; ++i) l += sh[i][lane].y * exp2f(sh[i][lane].x - sub);
     const float lse2 = m + log2f(l);
     st.lse2[s] = lse2;
     v = st.mw[s] * (kLn2 * lse2 - ztgt[s]);
@@ -429,6 +436,138 @@ __global__ void __launch_bounds__(32 * kShares) lce_rho_kernel(const State st, c
   for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
   if (lane == 0) atomicMax(counters + 1, __float_as_uint(big));  // non-negative: ordered like its bits
   if (gdloss != nullptr && reduction != TTT_LCE_NONE) total_rows(dc, sums, counters + 2, st.head->denom, gdloss);
+}
+
+// Losses of a few rows without gradients (the score of a token): a product with so
+// few rows is bound by reading w once, so CUDA cores form it. Every warp takes four
+// vocabulary rows at a time (their loads in flight together), adds up its lanes'
+// products with the rows of h held in shared memory, and keeps a running (max, sum)
+// per row; blocks write theirs as one part each, which lce_lse_kernel merges. Block
+// 0 lists the rows. Against the tensor-core path (list, 256-row tiles, merge) at 1 x
+// 768 x 32000 bf16 this saves a launch and 10 us of 26.
+constexpr int kScoreRows = 4, kScoreWarps = 16, kScoreMaxDim = 8192;
+template <bool BF16, int NR>
+__global__ void __launch_bounds__(32 * kScoreWarps) lce_score_kernel(const RowArgs a, const uint16_t* w, int64_t w_stride,
+                                                                     float2* part, float* ztgt) {
+  extern __shared__ __align__(16) uint16_t hs[];  // [NR][dim]
+  __shared__ float2 sh[kScoreWarps][NR];
+  __shared__ int rows[NR], tgts[NR], count;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    float m = 0.f;
+    int kind = 0;
+    if (lane < a.n) {
+      m = mask_weight(a, lane);
+      kind = row_kind(a, lane, m);
+      if (kind < 0 && blockIdx.x == 0) ttt::report_error(a.err, a.err_host, TTT_ERR_WORD_TARGET | lane);
+    }
+    const unsigned bits = __ballot_sync(0xffffffffu, kind > 0);
+    const int s = __popc(bits & ((1u << lane) - 1));
+    if (kind > 0) {
+      rows[s] = lane;
+      tgts[s] = static_cast<int>(a.targets[lane]);
+    }
+    if (lane == 0) count = __popc(bits);
+    if (blockIdx.x == 0) {
+      if (kind > 0) {
+        a.st.idx[s] = lane;
+        a.st.mw[s] = m;
+      } else if (lane < a.n && a.reduction == TTT_LCE_NONE) {
+        a.loss[lane] = 0.f;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+      if (lane == 0) {
+        a.st.head->n_active = __popc(bits);
+        a.st.head->ticket = 0;
+        a.st.head->denom = a.reduction != TTT_LCE_MEAN              ? 1.f
+                           : a.mask_kind == TTT_LCE_MASK_NONE ? static_cast<float>(a.n)
+                                                              : fmaxf(m, 1.f);
+      }
+    }
+  }
+  __syncthreads();
+  const int nr = count;
+  for (int r = 0; r < NR; ++r)
+    for (int c = threadIdx.x; c < a.dim; c += blockDim.x)
+      hs[r * a.dim + c] = r < nr ? a.src[rows[r] * a.src_stride + c] : 0;
+  __syncthreads();
+  float mx[NR], sum[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) mx[r] = -INFINITY, sum[r] = 0.f;
+  const int vocab = static_cast<int>(a.vocab);
+  constexpr int U = 4;
+  for (int v0 = (blockIdx.x * kScoreWarps + warp) * U; v0 < vocab; v0 += gridDim.x * kScoreWarps * U) {
+    float z[NR][U];
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+#pragma unroll
+      for (int u = 0; u < U; ++u) z[r][u] = 0.f;
+#pragma unroll 2
+    for (int c = lane * 8; c < a.dim; c += 256) {
+      uint4 q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        q[u] = __ldcs(reinterpret_cast<const uint4*>(w + min(v0 + u, vocab - 1) * w_stride + c));
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const uint4 hq = *reinterpret_cast<const uint4*>(hs + r * a.dim + c);
+        const uint32_t hw[4] = {hq.x, hq.y, hq.z, hq.w};
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t ww[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            z[r][u] = fmaf(ttt::to_f32<BF16>(static_cast<uint16_t>(ww[e])),
+                           ttt::to_f32<BF16>(static_cast<uint16_t>(hw[e])), z[r][u]);
+            z[r][u] = fmaf(ttt::to_f32<BF16>(static_cast<uint16_t>(ww[e] >> 16)),
+                           ttt::to_f32<BF16>(static_cast<uint16_t>(hw[e] >> 16)), z[r][u]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int u = 0; u < U; ++u) z[r][u] += __shfl_xor_sync(0xffffffffu, z[r][u], o);
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      if (lane == 0 && r < nr && tgts[r] >= v0 && tgts[r] < v0 + U) {
+        float zt = z[r][0];
+#pragma unroll
+        for (int u = 1; u < U; ++u) zt = tgts[r] == v0 + u ? z[r][u] : zt;
+        ztgt[r] = zt;
+      }
+      float top = mx[r];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        z[r][u] = v0 + u < vocab ? z[r][u] * kLog2e : -INFINITY;
+        top = fmaxf(top, z[r][u]);
+      }
+      const float sub = top == -INFINITY ? 0.f : top;
+      sum[r] *= exp2f(mx[r] - sub);
+#pragma unroll
+      for (int u = 0; u < U; ++u) sum[r] += exp2f(z[r][u] - sub);
+      mx[r] = top;
+    }
+  }
+  if (lane == 0) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) sh[warp][r] = make_float2(mx[r], sum[r]);
+  }
+  __syncthreads();
+  if (threadIdx.x < nr) {
+    const int r = threadIdx.x;
+    float m = -INFINITY, l = 0.f;
+    for (int i = 0; i < kScoreWarps; ++i) m = fmaxf(m, sh[i][r].x);
+    const float sub = m == -INFINITY ? 0.f : m;
+    for (int i = 0; i < kScoreWarps; ++i) l += sh[i][r].y * exp2f(sh[i][r].x - sub);
+    part[static_cast<int64_t>(blockIdx.x) * a.n_pad + r] = make_float2(m, l);
+  }
 }
 
 __global__ void lce_zero_rows_kernel(const int* slot, int64_t n, float* out) {
@@ -661,6 +800,7 @@ int ttt_lce_fwd(const ttt_lce_fwd_args* a, void* stream) {
   const ttt_lce_problem& pb = a->pb;
   TTT_TRY(check_lce(pb));
   TTT_TRY(check_weight(a->w, a->w_stride, pb));
+  if (a->need_state != 0 && a->need_state != 1) return TTT_ERR_UNSUPPORTED;
   if (pb.n == 0)
     return pb.reduction == TTT_LCE_NONE ? TTT_OK : zero(a->loss, 4, static_cast<cudaStream_t>(stream));
   if (a->h == nullptr || a->targets == nullptr) return TTT_ERR_NULL;
@@ -670,10 +810,22 @@ int ttt_lce_fwd(const ttt_lce_fwd_args* a, void* stream) {
   Pass p(pb, 0, a->state, a->work, nullptr, a->err, stream);
   RowArgs r = p.row_args(a->h, a->h_stride, p.st.hc);
   r.targets = a->targets, r.mask = a->mask, r.loss = a->loss;
+  const Weight w(a->w, a->w_stride, pb);
+  if (a->need_state == 0 && pb.n <= kScoreRows && pb.dim % 8 == 0 && pb.dim <= kScoreMaxDim) {
+    const int blocks = static_cast<int>(std::min<int64_t>((pb.vocab + 4 * kScoreWarps - 1) / (4 * kScoreWarps),
+                                                          std::min<int64_t>(p.sms, score_parts(pb.vocab))));
+    auto kern = p.bf16 ? (pb.n == 1 ? lce_score_kernel<true, 1> : lce_score_kernel<true, kScoreRows>)
+                       : (pb.n == 1 ? lce_score_kernel<false, 1> : lce_score_kernel<false, kScoreRows>);
+    const int smem = (pb.n == 1 ? 1 : kScoreRows) * pb.dim * 2;
+    if (smem > 48 * 1024) TTT_TRY(launched(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)));
+    kern<<<blocks, 32 * kScoreWarps, smem, p.s>>>(r, w.p, w.stride, p.w.part, p.w.ztgt);
+    TTT_TRY(launched());
+    return launch_early(lce_lse_kernel, 1, 32 * kShares, p.s, p.st, p.w.part, p.w.ztgt, blocks, static_cast<int>(p.q.n_pad),
+                        pb.reduction, p.w.sums, a->loss);
+  }
   lce_list_kernel<<<static_cast<unsigned>((pb.n + kListRows - 1) / kListRows), 256, 0, p.s>>>(r);
   TTT_TRY(launched());
   ttt::LceGemm g = p.gemm(0, pb.vocab);
-  const Weight w(a->w, a->w_stride, pb);
   if (!p.map_rows(&g.a[0], p.st.hc) || !p.map_weight(&g.b[0], w, g, ttt::kLceBN)) return TTT_ERR_TENSOR_MAP;
   TTT_TRY(p.run(g, ttt::kLceStats));
   const int parts = 2 * static_cast<int>((pb.vocab + ttt::kLceBN - 1) / ttt::kLceBN);

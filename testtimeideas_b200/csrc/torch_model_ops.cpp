@@ -237,7 +237,8 @@ at::Tensor lce_work(const ttt_lce_problem& pb, int pass, const at::Tensor& like)
 }
 
 std::tuple<at::Tensor, at::Tensor> op_linear_ce(const at::Tensor& h_, const at::Tensor& w_, const at::Tensor& targets_,
-                                                const OptTensor& mask_, int64_t reduction, int64_t ignore_index) {
+                                                const OptTensor& mask_, int64_t reduction, int64_t ignore_index,
+                                                bool need_state) {
   ttt_lce_problem pb = lce_problem(h_, w_, reduction, ignore_index);
   TORCH_CHECK(targets_.device() == h_.device() && at::isIntegralType(targets_.scalar_type(), false),
               "linear cross entropy: targets must be integers on hidden's device");
@@ -272,6 +273,7 @@ std::tuple<at::Tensor, at::Tensor> op_linear_ce(const at::Tensor& h_, const at::
   // an empty loss has no storage; the entry point wants an address
   a.loss = loss.numel() > 0 ? loss.data_ptr<float>() : reinterpret_cast<float*>(word.data_ptr());
   a.state = state.numel() > 0 ? state.data_ptr() : nullptr;
+  a.need_state = need_state ? 1 : 0;
   a.err = word.data_ptr<int32_t>();
   a.work = ptr(work);
   a.work_bytes = work.defined() ? work.numel() : 0;
@@ -476,6 +478,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     if (at::GradMode::is_enabled()) {
       out = LayerNormBwdFn::apply(up[0], v[0], opt(v[1]), v[2], v[3], need, p_type);
     } else {
+      at::AutoDispatchBelowADInplaceOrView below;
       auto [dx, dw, db] = raw_layer_norm_bwd().call(up[0], v[0], opt(v[1]), v[2], v[3], (need & 1) != 0,
                                                     (need & 2) != 0, (need & 4) != 0,
                                                     static_cast<at::ScalarType>(p_type));
@@ -497,6 +500,7 @@ bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
 at::Tensor op_layer_norm_ad(const at::Tensor& x, const OptTensor& w_, const OptTensor& b_, double eps) {
   const at::Tensor w = defined_or(w_), b = defined_or(b_);
   if (wants_grad({&x, &w, &b})) return LayerNormFn::apply(x, w_, b_, eps);
+  at::AutoDispatchBelowADInplaceOrView below;
   return std::get<0>(raw_layer_norm().call(x, w_, b_, eps, false));
 }
 
@@ -534,7 +538,7 @@ struct LinearCEFn : torch::autograd::Function<LinearCEFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& targets,
                             const OptTensor& mask, int64_t reduction, int64_t ignore_index) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [loss, state] = raw_linear_ce().call(h, w, targets, mask, reduction, ignore_index);
+    auto [loss, state] = raw_linear_ce().call(h, w, targets, mask, reduction, ignore_index, true);
     ctx->save_for_backward({h, w, state});
     ctx->set_materialize_grads(false);
     ctx->saved_data["reduction"] = reduction;
@@ -550,6 +554,7 @@ struct LinearCEFn : torch::autograd::Function<LinearCEFn> {
     if (at::GradMode::is_enabled()) {
       out = LinearCEBwdFn::apply(up[0], v[0], v[1], v[2], reduction, need);
     } else {
+      at::AutoDispatchBelowADInplaceOrView below;
       auto [dh, dw] = raw_linear_ce_bwd().call(up[0], v[0], v[1], v[2], reduction, (need & 1) != 0, (need & 2) != 0);
       out = {dh, dw};
     }
@@ -562,7 +567,8 @@ struct LinearCEFn : torch::autograd::Function<LinearCEFn> {
 at::Tensor op_linear_ce_ad(const at::Tensor& h, const at::Tensor& w, const at::Tensor& targets, const OptTensor& mask,
                            int64_t reduction, int64_t ignore_index) {
   if (wants_grad({&h, &w})) return LinearCEFn::apply(h, w, targets, mask, reduction, ignore_index);
-  return std::get<0>(raw_linear_ce().call(h, w, targets, mask, reduction, ignore_index));
+  at::AutoDispatchBelowADInplaceOrView below;
+  return std::get<0>(raw_linear_ce().call(h, w, targets, mask, reduction, ignore_index, false));
 }
 
 }  // namespace
@@ -576,9 +582,10 @@ TORCH_LIBRARY_FRAGMENT(ttt, m) {
         "bool need_db, ScalarType p_type) -> (Tensor dx, Tensor dw, Tensor db)");
   m.def("layer_norm_bwd2(Tensor dy, Tensor x, Tensor? w, Tensor mean, Tensor rstd, Tensor? ux, Tensor? uw, "
         "Tensor? ub) -> (Tensor gdy, Tensor gx, Tensor gw)");
-  // reduction: 0 none, 1 mean, 2 sum; state (bytes) is what the gradients need of the forward.
-  m.def("linear_ce(Tensor h, Tensor w, Tensor targets, Tensor? mask, int reduction, int ignore_index) -> "
-        "(Tensor loss, Tensor state)");
+  // reduction: 0 none, 1 mean, 2 sum; state (bytes) is what the gradients need of the forward
+  // (filled only with need_state).
+  m.def("linear_ce(Tensor h, Tensor w, Tensor targets, Tensor? mask, int reduction, int ignore_index, bool "
+        "need_state) -> (Tensor loss, Tensor state)");
   m.def("linear_ce_bwd(Tensor dloss, Tensor h, Tensor w, Tensor state, int reduction, bool need_dh, bool need_dw) -> "
         "(Tensor dh, Tensor dw)");
   m.def("linear_ce_bwd2(Tensor dloss, Tensor h, Tensor w, Tensor state, int reduction, Tensor? uh, Tensor? uw, "
