@@ -87,6 +87,12 @@ CONFIGS = {
                workload="BASELINE config 5: TTT-E2E meta step, 12 layers d_model=768 12 heads d_ff=3072 vocab 32000, "
                         "bf16, b=1 T=8192, inner_steps=1 inner_lr=0.01 on the first 6144 tokens, outer loss on the "
                         "last 2048, all parameters updated, attention on the kernels"),
+    # the same step with the norms and the token loss on the kernels too (no logits in memory)
+    "c5k": dict(b=1, h=12, t=8192, d=64, dtype="bf16", causal=True, scale_in=1.0, step="meta",
+                model=dict(n_layers=12, d_model=768, n_heads=12, d_ff=3072, vocab_size=32000, max_seq_len=8192,
+                           window_size=None, kernel_norm_loss=True),
+                workload="BASELINE config 5 with kernel_norm_loss: attention, layer norms and linear cross entropy on "
+                         "the kernels, otherwise as c5"),
     # the forward-only streaming path of the reference's latency demo (scripts/demo_infer.py:11-27,
     # :70-100): its model, seq 8192 in chunks of 512 new tokens, each call over the last 512 tokens
     "c5s": dict(b=1, h=8, t=8192, d=64, dtype="bf16", causal=True, scale_in=1.0, step="stream",

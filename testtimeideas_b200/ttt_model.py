@@ -10,7 +10,9 @@ outer loss is the masked loss of the updated model. Backpropagating the outer
 loss differentiates through the inner step, i.e. through the first-order
 attention backward: that is the grad-grad attention step, including the
 gradient with respect to the upstream gradient (∂dO), which the kernels'
-double backward provides.
+double backward provides. With ``kernel_norm_loss`` the norms and the token loss
+of that step, its gradient and the gradient's gradient run on the kernels of
+``norm_loss`` as well.
 """
 
 from __future__ import annotations
@@ -23,6 +25,7 @@ import torch.nn.functional as F
 from torch import nn
 from torch.func import functional_call
 
+from .norm_loss import LayerNorm, linear_cross_entropy
 from .ttt_e2e import WindowedSelfAttention
 
 
@@ -39,10 +42,17 @@ class ModelConfig:
     use_gradgrad_attention: bool = True
     suffix_layers: int = -1  # layers updated by the inner loop (-1: all); the rest form the prefix
     dual_mlp: bool = True    # suffix blocks add a slow MLP to the fast one
+    # norms and token loss on the kernels of norm_loss (same parameters and values; the
+    # loss then goes from ln_f's output straight to the head weight, without logits)
+    kernel_norm_loss: bool = False
 
 
 def _mlp(cfg: ModelConfig) -> nn.Sequential:
     return nn.Sequential(nn.Linear(cfg.d_model, cfg.d_ff), nn.GELU(), nn.Linear(cfg.d_ff, cfg.d_model))
+
+
+def _norm(cfg: ModelConfig) -> nn.LayerNorm:
+    return LayerNorm(cfg.d_model) if cfg.kernel_norm_loss else nn.LayerNorm(cfg.d_model)
 
 
 class PrefixBlock(nn.Module):
@@ -50,9 +60,9 @@ class PrefixBlock(nn.Module):
 
     def __init__(self, cfg: ModelConfig):
         super().__init__()
-        self.ln1 = nn.LayerNorm(cfg.d_model)
+        self.ln1 = _norm(cfg)
         self.attn = WindowedSelfAttention(cfg.d_model, cfg.n_heads, cfg.window_size, cfg.use_gradgrad_attention)
-        self.ln2 = nn.LayerNorm(cfg.d_model)
+        self.ln2 = _norm(cfg)
         self.mlp = _mlp(cfg)
         self.dropout = nn.Dropout(cfg.dropout)
 
@@ -66,9 +76,9 @@ class SuffixBlock(nn.Module):
 
     def __init__(self, cfg: ModelConfig):
         super().__init__()
-        self.ln1 = nn.LayerNorm(cfg.d_model)
+        self.ln1 = _norm(cfg)
         self.attn = WindowedSelfAttention(cfg.d_model, cfg.n_heads, cfg.window_size, cfg.use_gradgrad_attention)
-        self.ln2 = nn.LayerNorm(cfg.d_model)
+        self.ln2 = _norm(cfg)
         self.mlp_fast = _mlp(cfg)
         self.mlp_slow = _mlp(cfg) if cfg.dual_mlp else None
         self.dropout = nn.Dropout(cfg.dropout)
@@ -93,7 +103,7 @@ class TTTModel(nn.Module):
         self.prefix_layers = cfg.n_layers - n_suffix
         self.prefix_blocks = nn.ModuleList(PrefixBlock(cfg) for _ in range(self.prefix_layers))
         self.suffix_blocks = nn.ModuleList(SuffixBlock(cfg) for _ in range(n_suffix))
-        self.ln_f = nn.LayerNorm(cfg.d_model)
+        self.ln_f = _norm(cfg)
         self.head = nn.Linear(cfg.d_model, cfg.vocab_size, bias=False)
 
     def prefix_forward(self, input_ids):
@@ -103,22 +113,24 @@ class TTTModel(nn.Module):
             x = blk(x)
         return x
 
-    def suffix_forward(self, hidden):
+    def suffix_forward(self, hidden, with_head: bool = True):
         x = hidden
         for blk in self.suffix_blocks:
             x = blk(x)
-        return self.head(self.ln_f(x))
+        x = self.ln_f(x)
+        return self.head(x) if with_head else x
 
-    def forward(self, input_ids=None, *, mode: str = "full", prefix_hidden=None):
+    def forward(self, input_ids=None, *, mode: str = "full", prefix_hidden=None, with_head: bool = True):
         """Token ids to logits. mode="prefix" stops after the prefix blocks and returns
         their hidden states; mode="suffix" starts from such states (prefix_hidden);
-        any other mode runs the whole model, as the reference's does."""
+        any other mode runs the whole model, as the reference's does. with_head=False
+        returns the head's input in place of the logits."""
         start_from_hidden = mode == "suffix"
         given, what = (prefix_hidden, "prefix_hidden") if start_from_hidden else (input_ids, "input_ids")
         if given is None:
             raise ValueError(f"TTTModel.forward(mode={mode!r}) needs {what}")
         hidden = prefix_hidden if start_from_hidden else self.prefix_forward(input_ids)
-        return hidden if mode == "prefix" else self.suffix_forward(hidden)
+        return hidden if mode == "prefix" else self.suffix_forward(hidden, with_head)
 
 
 def compute_loss(logits, targets, mask=None):
@@ -154,6 +166,35 @@ def _suffix_logits(model: TTTModel, params: Dict[str, torch.Tensor], hidden: tor
     return functional_call(model, params, (None,), {"mode": "suffix", "prefix_hidden": hidden})
 
 
+def _suffix_loss(model: TTTModel, params: Dict[str, torch.Tensor], hidden: torch.Tensor, targets, mask) -> torch.Tensor:
+    """compute_loss of the suffix's logits; with cfg.kernel_norm_loss the same value
+    without the logits in memory."""
+    if not model.cfg.kernel_norm_loss:
+        return compute_loss(_suffix_logits(model, params, hidden), targets, mask)
+    x = functional_call(model, params, (None,), {"mode": "suffix", "prefix_hidden": hidden, "with_head": False})
+    return linear_cross_entropy(x, params["head.weight"], targets, mask)
+
+
+@torch.no_grad()
+def token_losses(model: TTTModel, params: Dict[str, torch.Tensor], input_ids, targets, mask=None,
+                 chunk_size: Optional[int] = None) -> torch.Tensor:
+    """Each position's cross entropy (0 where the mask is 0) under parameters ``params``,
+    for instance those of ttt_apply: the scores of a text after test-time adaptation."""
+    prefix = functional_call(model, params, (input_ids,), {"mode": "prefix"})
+    out = []
+    for hid, tgt, msk in zip(_chunks(prefix, chunk_size), _chunks(targets, chunk_size),
+                             _chunks(torch.ones_like(targets, dtype=torch.float32) if mask is None else mask,
+                                     chunk_size)):
+        x = functional_call(model, params, (None,), {"mode": "suffix", "prefix_hidden": hid, "with_head": False})
+        if model.cfg.kernel_norm_loss:
+            out.append(linear_cross_entropy(x, params["head.weight"], tgt, msk, reduction="none"))
+        else:
+            logits = F.linear(x, params["head.weight"])
+            ce = F.cross_entropy(logits.reshape(-1, logits.size(-1)), tgt.reshape(-1), reduction="none")
+            out.append(ce.view(tgt.shape) * msk)
+    return torch.cat(out, dim=1)
+
+
 def _inner_scan(model: TTTModel, params: Dict[str, torch.Tensor], fast: List[str], prefix: torch.Tensor, targets,
                 inner_mask, inner_lr: float, inner_steps: int, chunk_size: Optional[int],
                 create_graph: bool) -> Tuple[Dict[str, torch.Tensor], torch.Tensor]:
@@ -164,7 +205,7 @@ def _inner_scan(model: TTTModel, params: Dict[str, torch.Tensor], fast: List[str
     inner_losses = []
     for hid, tgt, msk in zip(_chunks(prefix, chunk_size), _chunks(targets, chunk_size), _chunks(inner_mask, chunk_size)):
         for _ in range(inner_steps):
-            loss = compute_loss(_suffix_logits(model, params, hid), tgt, msk)
+            loss = _suffix_loss(model, params, hid, tgt, msk)
             grads = torch.autograd.grad(loss, [params[n] for n in fast], create_graph=create_graph,
                                         retain_graph=create_graph)
             params = dict(params)
@@ -188,7 +229,7 @@ def meta_step(model: TTTModel, input_ids, targets, inner_mask, outer_mask, inner
         w = msk.sum()
         if w.item() <= 0:
             continue
-        total = total + compute_loss(_suffix_logits(model, params, hid), tgt, msk) * w
+        total = total + _suffix_loss(model, params, hid, tgt, msk) * w
         weight = weight + w
     return inner_loss, total / weight.clamp_min(1.0)
 
