@@ -93,6 +93,51 @@ struct Plan {
   int64_t piece;  // vocabulary columns per piece
   int splits;     // shares of a piece's columns in the dh product
 };
+// Time (in 64-wide steps of a pair of CTAs) until `pairs` pairs that take the next tile
+// when free have formed n_long tiles of `len` steps and then n_short of `slen`.
+int64_t makespan(int64_t pairs, int64_t n_long, int64_t len, int64_t n_short, int64_t slen) {
+  const int64_t k = n_long / pairs, r = n_long % pairs;  // r pairs hold one long tile more
+  const int64_t full = (k + (r > 0 ? 1 : 0)) * len;
+  auto room = [&](int64_t x) {  // short tiles that fit before time x
+    const int64_t a = x > full ? (x - full) / slen : 0, b = x > k * len ? (x - k * len) / slen : 0;
+    return r > 0 ? r * a + (pairs - r) * b : pairs * b;
+  };
+  int64_t lo = full, hi = full + (n_short / pairs + 1) * slen;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) / 2;
+    if (room(mid) >= n_short)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return lo;
+}
+
+// The shares into which the hidden gradient's contraction over a piece is cut: more of
+// them let the pairs end together and fill the GPU with few tokens, but each costs a
+// pass over fp32 partial rows. The count with the least time is taken, with a step at
+// 0.3 us (512 cycles), a tile's start and end at eight steps, and the partial rows
+// written and read at 6.5 TB/s. At 8192 x 768 x 32000 the second gradient's pieces (96
+// tiles of 512 steps against 189 of 264) take 1552 steps uncut and 1408 in three shares.
+int plan_splits(const Plan& q, int segs, int64_t pairs) {
+  const int64_t cols = std::min(q.piece, q.vocab);
+  const int64_t dt = up(q.dim, ttt::kLceBN) / ttt::kLceBN, kt = up(cols, 64) / 64;
+  const int64_t n_dh = q.n_pad / ttt::kLceBM * dt, n_dw = up(cols, ttt::kLceBM) / ttt::kLceBM * dt;
+  const int64_t dw_len = q.n_pad / 64 * segs + 8;
+  int best = 1;
+  double best_time = 0;
+  for (const int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
+    if (s > 1 && kt / s < 8) break;
+    const int64_t dh_len = (kt + s - 1) / s * segs + 8;
+    const int64_t steps = dh_len > dw_len ? makespan(pairs, n_dh * s, dh_len, n_dw, dw_len)
+                                          : makespan(pairs, n_dw, dw_len, n_dh * s, dh_len);
+    const double bytes = 8.0 * s * static_cast<double>(q.n_pad) * q.dim_pad;
+    const double time = static_cast<double>(steps) + bytes / (6.5e6 * 0.3);
+    if (s == 1 || time < best_time) best = s, best_time = time;
+  }
+  return best;
+}
+
 Plan make_plan(const ttt_lce_problem& pb, int pass, int sms) {
   Plan q;
   q.n = pb.n;
@@ -107,14 +152,7 @@ Plan make_plan(const ttt_lce_problem& pb, int pass, int sms) {
   const int64_t most = std::max<int64_t>(2048, budget / std::max<int64_t>(per_col, 1));
   const int64_t pieces = (q.vocab + most - 1) / most;
   q.piece = up((q.vocab + pieces - 1) / pieces, 256);
-  // The hidden gradient's contraction over the piece is cut where a whole one would
-  // be longer than a pair's share of both products (few tokens); no share is shorter
-  // than eight steps.
-  const int64_t pairs = std::max(1, sms / 2), cols = std::min(q.piece, q.vocab);
-  const int64_t mt = q.n_pad / ttt::kLceBM, dt = up(q.dim, ttt::kLceBN) / ttt::kLceBN;
-  const int64_t kt = up(cols, ttt::kLceBK) / ttt::kLceBK, vt = up(cols, ttt::kLceBM) / ttt::kLceBM;
-  const int64_t share = std::max<int64_t>(1, (mt * dt * kt + vt * dt * (q.n_pad / ttt::kLceBK)) / pairs);
-  q.splits = static_cast<int>(std::max<int64_t>(1, std::min((kt + share - 1) / share, kt / 8)));
+  q.splits = plan_splits(q, pass == 2 ? 2 : 1, std::max(1, sms / 2));
   return q;
 }
 
@@ -720,10 +758,10 @@ struct Pass {
   }
   // Operands of the logit kinds: rows of hc or uc (128 a CTA), rows of a piece of w or uw (bn / 2 a CTA).
   bool map_rows(CUtensorMap* m, const uint16_t* x) const {
-    return map(m, x, q.dim, q.n_pad, q.dim_pad, ttt::kLceBK, ttt::kLceBM / 2);
+    return map(m, x, q.dim, q.n_pad, q.dim_pad, ttt::kLcePanel, ttt::kLceBM / 2);
   }
   bool map_weight(CUtensorMap* m, const Weight& w, const ttt::LceGemm& g, int bn) const {
-    return map(m, w.row(g.col0), q.dim, g.cols, w.stride, ttt::kLceBK, bn / 2);
+    return map(m, w.row(g.col0), q.dim, g.cols, w.stride, ttt::kLcePanel, bn / 2);
   }
 };
 
@@ -736,7 +774,7 @@ int run_pieces(const Pass& p, const Weight& w, const Weight* uw, bool second, bo
   const Plan& q = p.q;
   if (outh == nullptr && outw == nullptr) return TTT_OK;
   const int bn = second ? ttt::kLceBNDual : ttt::kLceBN;
-  constexpr int bk = ttt::kLceBK;
+  constexpr int panel = ttt::kLcePanel, bk = ttt::kLceBK;
   for (int64_t col0 = 0; col0 < q.vocab; col0 += q.piece) {
     const int64_t cols = std::min(q.piece, q.vocab - col0);
     // z (and A) -> G (and D)
@@ -762,10 +800,10 @@ int run_pieces(const Pass& p, const Weight& w, const Weight* uw, bool second, bo
       const uint16_t* stored = second && i == 0 ? p.w.d : p.w.g;
       const Weight& wi = i == 0 || uw == nullptr ? w : *uw;
       const uint16_t* ri = i == 0 || !has_uh ? p.st.hc : p.w.uc;
-      ok = p.map(&t.gk[i], stored, cols, q.n_pad, q.piece, bk, ttt::kLceBM / 2) &&
-           p.map(&t.gm[i], stored, cols, q.n_pad, q.piece, 64, bk) &&
-           p.map(&t.bw[i], wi.row(col0), q.dim, cols, wi.stride, 64, bk) &&
-           p.map(&t.bh[i], ri, q.dim, q.n_pad, q.dim_pad, 64, bk);
+      ok = p.map(&t.gk[i], stored, cols, q.n_pad, q.piece, panel, ttt::kLceBM / 2) &&
+           p.map(&t.gm[i], stored, cols, q.n_pad, q.piece, panel, bk) &&
+           p.map(&t.bw[i], wi.row(col0), q.dim, cols, wi.stride, panel, bk) &&
+           p.map(&t.bh[i], ri, q.dim, q.n_pad, q.dim_pad, panel, bk);
       if (!ok) return TTT_ERR_TENSOR_MAP;
     }
     if (t.dw != nullptr && q.dim % 8 == 0 && !p.map(&t.dw_out, t.dw, q.dim, cols, q.dim, 64, 32))

@@ -46,7 +46,8 @@ struct LceCoef {
 constexpr int kLceBM = 256;
 constexpr int kLceBN = 256;      // single-product tiles
 constexpr int kLceBNDual = 128;  // two accumulators side by side
-constexpr int kLceBK = 64;
+constexpr int kLcePanel = 64;    // columns of an operand box (128 bytes, the swizzle's width)
+constexpr int kLceBK = 128;      // contraction of a stage (64 in the dual kinds)
 
 enum LceKind : int {
   kLceStats = 0,      // z -> per-row (max, sum) of the half tile, z at the target

@@ -11,10 +11,11 @@
 //               the leader's (even CTA's) barrier
 //   warp 9      leader only: MMA issuer, into one of two accumulator buffers in
 //               TMEM, so that a tile's products run while the previous one is read
-//   warp 10     kLceProd, leader only: hands out tiles from a global counter. Its
-//               two kinds of tiles differ in length by up to a factor of ten; taken
-//               in order of length by whichever pair is free, all pairs end within
-//               one short tile. Which pair forms a tile does not change its value.
+// kLceProd's two kinds of tiles differ in length by up to a factor of ten. There the
+// leader's producer takes the next tile from a global counter when it has issued the
+// last load of the current one, and passes it on to the pair's other warps: taken in
+// order of length by whichever pair is free, all pairs end within one short tile.
+// Which pair forms a tile does not change its value.
 // The logits never leave the chip: the statistics kinds reduce them to two floats
 // per row and half tile, the gradient kinds turn them into the 16-bit derivative of
 // the logits of one piece of the vocabulary, which kLceProd contracts with w and h.
@@ -72,6 +73,18 @@ TTT_DEV void umma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// Non-blocking look at a barrier phase.
+TTT_DEV uint32_t mbar_probe(const uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done;
+}
+
 // Arrive on `bar` of both CTAs when every product issued so far has completed.
 TTT_DEV void commit_pair(uint64_t* bar) {
   asm volatile(
@@ -111,17 +124,18 @@ struct LceCfg {
   static constexpr bool LOGIT = KIND != kLceProd;
   static constexpr bool DUAL = KIND == kLceDualStats || KIND == kLceDualGrad;
   static constexpr bool GRAD = KIND == kLceGrad || KIND == kLceDualGrad;
-  static constexpr int BM = kLceBM, BN = DUAL ? kLceBNDual : kLceBN, BK = kLceBK;
+  static constexpr int BM = kLceBM, BN = DUAL ? kLceBNDual : kLceBN;
+  static constexpr int BK = DUAL ? kLcePanel : kLceBK, PANELS = BK / kLcePanel;  // of a stage's contraction
   static constexpr int ROWS_A = BM / 2, ROWS_B = BN / 2;  // of a CTA
   static constexpr int TILE_A = ROWS_A * BK * 2, TILE_B = ROWS_B * BK * 2;
   static constexpr int STAGE = (DUAL ? 2 : 1) * (TILE_A + TILE_B);
-  static constexpr int NSTAGE = 196608 / STAGE;  // 192 KB: 6 single or 4 dual stages
+  static constexpr int NSTAGE = 196608 / STAGE;  // 192 KB: 3 single or 4 dual stages
   static constexpr int PANEL = 32 * 128;         // staging of one warp's [32 x 64] 16-bit store box
   static constexpr int OFF_STORE = NSTAGE * STAGE;
   static constexpr int OFF_BAR = OFF_STORE + 8 * PANEL;
   static constexpr int NBAR = 2 * NSTAGE + 9;
   static constexpr int SMEM = OFF_BAR + NBAR * 8 + 32 + 1024;
-  static constexpr int NTHREADS = 352, WARP_LOAD = 8, WARP_MMA = 9, WARP_SCHED = 10;
+  static constexpr int NTHREADS = 320, WARP_LOAD = 8, WARP_MMA = 9;
   static constexpr int HALF = BN / 2;  // columns (of each accumulator) per epilogue half
   static_assert(SMEM <= 232448, "tile set exceeds shared memory");
 };
@@ -170,17 +184,19 @@ TTT_DEV LceTile lce_tile(const LceGemm& p, const LceSizes& s, int t) {
   }
 }
 
-// Walks the tiles of this pair: a fixed stride, or (kLceProd) what the scheduler
-// warp hands out through a two-entry ring in both CTAs' shared memory. Used by one
-// warp (the epilogue) or one thread (producer, issuer).
+// Walks the tiles of this pair: a fixed stride, or (kLceProd) what the leader's
+// producer takes from the counter and writes into a two-entry ring in both CTAs'
+// shared memory. Used by one warp (the epilogue) or one thread (producer, issuer).
+enum LceRole { kTaker, kThread, kWarp };
 template <int KIND>
 struct LceWalk {
   int i = 0, pairs, pair, n_tiles;
+  uint32_t rank;
+  unsigned* ticket;
   volatile int* ring;
-  uint64_t* full;
-  uint32_t empty_leader;  // address of the leader's sched_empty[0]
-  // The next tile, or -1 at the end (or when aborting). WARP: called by a whole warp.
-  template <bool WARP>
+  uint64_t *full, *empty;
+  // The next tile, or -1 at the end (or when aborting).
+  template <LceRole ROLE>
   TTT_DEV int next(const Guard& g) {
     if constexpr (KIND != kLceProd) {
       const int t = pair + i * pairs;
@@ -188,13 +204,23 @@ struct LceWalk {
       return t < n_tiles ? t : -1;
     } else {
       const int slot = i & 1;
-      bool ok = mbar_wait(full + slot, (i >> 1) & 1, g, 0x55);
-      if constexpr (WARP) ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return -1;
-      acquire_pair();
-      const int t = ring[slot];
-      if constexpr (WARP) __syncwarp();  // every lane has read the entry
-      if (!WARP || (threadIdx.x & 31) == 0) arrive_peer(empty_leader + slot * 8);
+      int t;
+      if (ROLE == kTaker && rank == 0) {
+        if (i >= 2 && !mbar_wait(empty + slot, ((i >> 1) - 1) & 1, g, 0x56)) return -1;
+        t = static_cast<int>(min(atomicAdd(ticket, 1u), 0x7fffffffu));
+        ring[slot] = t;
+        st_peer(peer_addr(const_cast<const int*>(ring) + slot, 1), t);
+        mbar_arrive(full + slot);
+        arrive_peer(peer_addr(full + slot, 1));
+      } else {
+        bool ok = mbar_wait(full + slot, (i >> 1) & 1, g, 0x55);
+        if constexpr (ROLE == kWarp) ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return -1;
+        acquire_pair();
+        t = ring[slot];
+        if constexpr (ROLE == kWarp) __syncwarp();  // every lane has read the entry
+        if (ROLE != kWarp || (threadIdx.x & 31) == 0) arrive_peer(peer_addr(empty + slot, 0));
+      }
       ++i;
       return t < n_tiles ? t : -1;
     }
@@ -233,8 +259,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
   uint64_t* acc_full = bars + 2 * C::NSTAGE;  // [2] each CTA's: MMA -> its epilogue
   uint64_t* acc_free = acc_full + 2;          // [2] leader's: 16 epilogue warps -> MMA
   uint64_t* drain = acc_full + 4;             // each CTA's: the issuer's last commit
-  uint64_t* sched_full = acc_full + 5;        // [2] each CTA's: scheduler -> its warps
-  uint64_t* sched_empty = acc_full + 7;       // [2] leader's: 19 readers -> scheduler
+  uint64_t* sched_full = acc_full + 5;        // [2] each CTA's: a ring entry is there
+  uint64_t* sched_empty = acc_full + 7;       // [2] leader's: its 18 readers have it
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::NBAR);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* ring = reinterpret_cast<volatile int*>(tmem_slot + 2);  // [2]
@@ -246,7 +272,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
     for (int i = 0; i < C::NBAR; ++i) mbar_init(bars + i, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_free + i, 16);
-      mbar_init(sched_empty + i, 19);
+      mbar_init(sched_empty + i, 18);
     }
     fence_mbar_init();
   }
@@ -270,9 +296,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
   walk.pairs = static_cast<int>(gridDim.x) >> 1;
   walk.pair = static_cast<int>(blockIdx.x) >> 1;
   walk.n_tiles = sz.n_tiles;
+  walk.rank = rank;
+  walk.ticket = p.ticket;
   walk.ring = ring;
   walk.full = sched_full;
-  walk.empty_leader = peer_addr(sched_empty, 0);
+  walk.empty = sched_empty;
   const bool seg0 = (p.seg_w & 1) != 0, seg1 = (p.seg_w & 2) != 0;  // dual kinds
   if (C::GRAD && go && blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;  // for the products that follow
 
@@ -283,7 +311,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
       const int row_a = static_cast<int>(rank) * C::ROWS_A, row_b = static_cast<int>(rank) * C::ROWS_B;
       int it = 0;
       bool ok = true;
-      for (int t; ok && (t = walk.template next<false>(g)) >= 0;) {
+      for (int t; ok && (t = walk.template next<kTaker>(g)) >= 0;) {
         const LceTile tl = lce_tile<KIND>(p, sz, t);
         const int segs = C::LOGIT ? 1 : (tl.dw ? p.seg_h : p.seg_w);
         for (int seg = 0; ok && seg < 2; ++seg) {
@@ -297,21 +325,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
             const uint32_t bar = peer_addr(full + s, 0);
             const int kc = k * C::BK;
             if constexpr (C::LOGIT) {
-              load_pair(st, &p.a[0], bar, kc, tl.m * C::BM + row_a);
-              load_pair(stb, &p.b[0], bar, kc, tl.n * C::BN + row_b);
+              for (int q = 0; q < C::PANELS; ++q) {
+                load_pair(st + q * C::ROWS_A * 128, &p.a[0], bar, kc + q * 64, tl.m * C::BM + row_a);
+                load_pair(stb + q * C::ROWS_B * 128, &p.b[0], bar, kc + q * 64, tl.n * C::BN + row_b);
+              }
               if constexpr (C::DUAL) {
                 if (seg0) load_pair(st + C::TILE_A, &p.a[1], bar, kc, tl.m * C::BM + row_a);
                 if (seg1) load_pair(stb + C::TILE_B, &p.b[1], bar, kc, tl.n * C::BN + row_b);
               }
             } else {
-              if (tl.dw) {
-                for (int q = 0; q < 2; ++q)
-                  load_pair(st + q * 8192, &p.gm[seg], bar, tl.m * C::BM + row_a + q * 64, kc);
-              } else {
-                load_pair(st, &p.gk[seg], bar, kc, tl.m * C::BM + row_a);
-              }
+              // MN-major panels: BK rows of 64 columns; K-major ones: 128 rows of 64 columns
               const CUtensorMap* b = tl.dw ? &p.bh[seg] : &p.bw[seg];
-              for (int q = 0; q < 2; ++q) load_pair(stb + q * 8192, b, bar, tl.n * C::BN + row_b + q * 64, kc);
+              for (int q = 0; q < 2; ++q) {
+                if (tl.dw)
+                  load_pair(st + q * C::BK * 128, &p.gm[seg], bar, tl.m * C::BM + row_a + q * 64, kc);
+                else
+                  load_pair(st + q * C::ROWS_A * 128, &p.gk[seg], bar, kc + q * 64, tl.m * C::BM + row_a);
+                load_pair(stb + q * C::BK * 128, b, bar, tl.n * C::BN + row_b + q * 64, kc);
+              }
             }
           }
         }
@@ -327,9 +358,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
       auto db = [](uint32_t tile, int kk) {
         return B_MN ? desc_mnmajor(tile, C::BK, kk) : desc_kmajor(tile, C::ROWS_B, kk);
       };
+      constexpr int KS = C::BK / 16;
       int it = 0, nth = 0;
-      bool ok = true;
-      for (int t; ok && (t = walk.template next<false>(g)) >= 0;) {
+      bool ready = false, ok = true;  // ready: the next stage has been seen full
+      for (int t; ok && (t = walk.template next<kThread>(g)) >= 0;) {
         const LceTile tl = lce_tile<KIND>(p, sz, t);
         const int steps = (tl.k1 - tl.k0) * (C::LOGIT ? 1 : __popc(tl.dw ? p.seg_h : p.seg_w));
         if (steps == 0) continue;  // the epilogue writes zeros by itself
@@ -338,34 +370,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
         const uint32_t d = tmem + buf * 256;
         for (int k = 0; k < steps; ++k, ++it) {
           const int s = it % C::NSTAGE;
-          if (!(ok = mbar_wait(full + s, (it / C::NSTAGE) & 1, g, 0x53))) break;
+          if (!ready && !(ok = mbar_wait(full + s, (it / C::NSTAGE) & 1, g, 0x53))) break;
           tc_fence_after();
           const uint32_t st = smem_u32(smem + s * C::STAGE);
+          const uint64_t* next_full = full + (it + 1) % C::NSTAGE;
+          const uint32_t next_par = ((it + 1) / C::NSTAGE) & 1;
           if constexpr (C::DUAL) {
             const uint32_t a0 = st, a1 = st + C::TILE_A, b0 = st + 2 * C::TILE_A, b1 = b0 + C::TILE_B;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
+            for (int kk = 0; kk < KS; ++kk)
               umma_pair(d, desc_kmajor(a0, C::ROWS_A, kk), db(b0, kk), id_k, (k | kk) ? 1u : 0u);
             if (seg0) {
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
+              for (int kk = 0; kk < KS; ++kk)
                 umma_pair(d + C::BN, desc_kmajor(a1, C::ROWS_A, kk), db(b0, kk), id_k, (k | kk) ? 1u : 0u);
             }
             if (seg1) {
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
+              for (int kk = 0; kk < KS; ++kk)
                 umma_pair(d + C::BN, desc_kmajor(a0, C::ROWS_A, kk), db(b1, kk), id_k, (seg0 || (k | kk)) ? 1u : 0u);
             }
           } else if (!C::LOGIT && tl.dw) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
+            for (int kk = 0; kk < KS; ++kk)
               umma_pair(d, desc_mnmajor(st, C::BK, kk), db(st + C::TILE_A, kk), id_mn, (k | kk) ? 1u : 0u);
           } else {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
+            for (int kk = 0; kk < KS; ++kk)
               umma_pair(d, desc_kmajor(st, C::ROWS_A, kk), db(st + C::TILE_A, kk), id_k, (k | kk) ? 1u : 0u);
           }
           commit_pair(empty + s);
+          ready = mbar_probe(next_full, next_par) != 0;
         }
         if (!ok) break;
         commit_pair(acc_full + buf);
@@ -373,21 +408,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
       }
       commit_pair(drain);
       mbar_drain(drain, 0);
-    }
-  } else if (KIND == kLceProd && go && warp == C::WARP_SCHED && rank == 0) {
-    // ------------------------------------------------------------ tile scheduler
-    if (lane == 0) {
-      const uint32_t ring_peer = peer_addr(const_cast<const int*>(ring), 1), full_peer = peer_addr(sched_full, 1);
-      for (int i = 0;; ++i) {
-        const int slot = i & 1;
-        if (i >= 2 && !mbar_wait(sched_empty + slot, ((i >> 1) - 1) & 1, g, 0x56)) break;
-        const int t = static_cast<int>(min(atomicAdd(p.ticket, 1u), 0x7fffffffu));
-        ring[slot] = t;
-        st_peer(ring_peer + slot * 4, t);
-        mbar_arrive(sched_full + slot);
-        arrive_peer(full_peer + slot * 8);
-        if (t >= sz.n_tiles) break;
-      }
     }
   } else if (go && warp < 8) {
     // ------------------------------------------------------------ epilogue
@@ -398,7 +418,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
     const uint32_t free_leader = peer_addr(acc_free, 0);
     const float mul = C::GRAD ? p.coef.scale() : (KIND == kLceProd ? 1.f / p.coef.scale() : 1.f);
     int nth = 0;
-    for (int t; (t = walk.template next<true>(g)) >= 0;) {
+    for (int t; (t = walk.template next<kWarp>(g)) >= 0;) {
       const LceTile tl = lce_tile<KIND>(p, sz, t);
       const bool have = tl.k1 > tl.k0 && (C::LOGIT || (tl.dw ? p.seg_h : p.seg_w) != 0);
       const int buf = nth & 1;
