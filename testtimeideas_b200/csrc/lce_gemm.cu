@@ -85,6 +85,13 @@ TTT_DEV uint32_t mbar_probe(const uint64_t* bar, uint32_t parity) {
   return done;
 }
 
+// One thread of the (converged) warp; the same one every time.
+TTT_DEV bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+  return r != 0;
+}
+
 // Arrive on `bar` of both CTAs when every product issued so far has completed.
 TTT_DEV void commit_pair(uint64_t* bar) {
   asm volatile(
@@ -265,7 +272,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* ring = reinterpret_cast<volatile int*>(tmem_slot + 2);  // [2]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
   asm volatile("griddepcontrol.launch_dependents;");
   if (threadIdx.x == 0) {
@@ -352,7 +359,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
     }
   } else if (go && warp == C::WARP_MMA && rank == 0) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    // The whole warp walks along, so that the compiler keeps descriptors and addresses in
+    // uniform registers; one thread issues. (A single thread on its own took ~96 cycles a
+    // product, more than a 128-wide one lasts.)
+    {
+      const bool leader = elect_one();
       constexpr bool B_MN = !C::LOGIT;
       constexpr uint32_t id_k = idesc_f16(C::BM, C::BN, BF16, false, B_MN), id_mn = idesc_f16(C::BM, C::BN, BF16, true, B_MN);
       auto db = [](uint32_t tile, int kk) {
@@ -361,20 +372,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
       constexpr int KS = C::BK / 16;
       int it = 0, nth = 0;
       bool ready = false, ok = true;  // ready: the next stage has been seen full
-      for (int t; ok && (t = walk.template next<kThread>(g)) >= 0;) {
+      for (int t; ok && (t = walk.template next<kWarp>(g)) >= 0;) {
         const LceTile tl = lce_tile<KIND>(p, sz, t);
         const int steps = (tl.k1 - tl.k0) * (C::LOGIT ? 1 : __popc(tl.dw ? p.seg_h : p.seg_w));
         if (steps == 0) continue;  // the epilogue writes zeros by itself
         const int buf = nth & 1;
-        if (nth >= 2 && !(ok = mbar_wait(acc_free + buf, ((nth >> 1) - 1) & 1, g, 0x52))) break;
+        if (nth >= 2 && !(ok = __all_sync(0xffffffffu, mbar_wait(acc_free + buf, ((nth >> 1) - 1) & 1, g, 0x52)))) break;
         const uint32_t d = tmem + buf * 256;
         for (int k = 0; k < steps; ++k, ++it) {
           const int s = it % C::NSTAGE;
-          if (!ready && !(ok = mbar_wait(full + s, (it / C::NSTAGE) & 1, g, 0x53))) break;
+          if (!ready && !(ok = __all_sync(0xffffffffu, mbar_wait(full + s, (it / C::NSTAGE) & 1, g, 0x53)))) break;
           tc_fence_after();
           const uint32_t st = smem_u32(smem + s * C::STAGE);
           const uint64_t* next_full = full + (it + 1) % C::NSTAGE;
           const uint32_t next_par = ((it + 1) / C::NSTAGE) & 1;
+          if (leader) {
           if constexpr (C::DUAL) {
             const uint32_t a0 = st, a1 = st + C::TILE_A, b0 = st + 2 * C::TILE_A, b1 = b0 + C::TILE_B;
 #pragma unroll
@@ -400,13 +412,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
               umma_pair(d, desc_kmajor(st, C::ROWS_A, kk), db(st + C::TILE_A, kk), id_k, (k | kk) ? 1u : 0u);
           }
           commit_pair(empty + s);
-          ready = mbar_probe(next_full, next_par) != 0;
+          }
+          __syncwarp();
+          ready = __all_sync(0xffffffffu, mbar_probe(next_full, next_par) != 0);
         }
         if (!ok) break;
-        commit_pair(acc_full + buf);
+        if (leader) commit_pair(acc_full + buf);
+        __syncwarp();
         ++nth;
       }
-      commit_pair(drain);
+      if (leader) commit_pair(drain);
+      __syncwarp();
       mbar_drain(drain, 0);
     }
   } else if (go && warp < 8) {
