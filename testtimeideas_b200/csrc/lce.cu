@@ -249,19 +249,32 @@ __device__ __forceinline__ int row_kind(const RowArgs& a, int64_t i, float m) {
   return t >= 0 && t < a.vocab ? 1 : -1;
 }
 
-// Copies source row `row` (or zeros, row < 0) into slot `s`; one warp.
-__device__ __forceinline__ void copy_row(const RowArgs& a, int64_t row, int64_t s, int lane) {
+// Copies up to R source rows (row < 0: zeros) into slots (slot < 0: none); one warp,
+// the rows' loads in flight together.
+template <int R>
+__device__ __forceinline__ void copy_rows(const RowArgs& a, const int64_t (&row)[R], const int64_t (&slot)[R], int lane) {
   if (a.src == nullptr) return;
-  uint16_t* dst = a.dst + s * a.dim_pad;
-  const uint16_t* src = row < 0 ? nullptr : a.src + row * a.src_stride;
   if (a.wide) {
-#pragma unroll 4
-    for (int c = lane * 8; c < a.dim; c += 256)
-      *reinterpret_cast<uint4*>(dst + c) =
-          src == nullptr ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(src + c);
+#pragma unroll 2
+    for (int c = lane * 8; c < a.dim; c += 256) {
+      uint4 v[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        v[i] = slot[i] < 0 || row[i] < 0 ? make_uint4(0, 0, 0, 0)
+                                         : *reinterpret_cast<const uint4*>(a.src + row[i] * a.src_stride + c);
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (slot[i] >= 0) *reinterpret_cast<uint4*>(a.dst + slot[i] * a.dim_pad + c) = v[i];
+    }
   } else {
-#pragma unroll 4
-    for (int c = lane; c < a.dim; c += 32) dst[c] = src == nullptr ? 0 : src[c];
+    for (int c = lane; c < a.dim; c += 32) {
+      uint16_t v[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) v[i] = slot[i] < 0 || row[i] < 0 ? 0 : a.src[row[i] * a.src_stride + c];
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (slot[i] >= 0) a.dst[slot[i] * a.dim_pad + c] = v[i];
+    }
   }
 }
 
@@ -282,7 +295,7 @@ __global__ void __launch_bounds__(256) lce_list_kernel(const RowArgs a) {
   // participating rows before row0, and the mask's sum and largest magnitude over them
   int before = 0;
   float msum = 0.f, mmax = 0.f;
-#pragma unroll 4
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < row0; i += 256) {
     const float m = mask_weight(a, i);
     const bool in = row_kind(a, i, m) > 0;
@@ -324,13 +337,21 @@ __global__ void __launch_bounds__(256) lce_list_kernel(const RowArgs a) {
     if (lane == 0) total = base;
   }
   __syncthreads();
-  for (int j = warp; j < kListRows; j += 8)
-    if (slots[j] >= 0) copy_row(a, row0 + j, slots[j], lane);
+  {
+    int64_t from[4], to[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      from[i] = row0 + warp * 4 + i;
+      to[i] = slots[warp * 4 + i];
+    }
+    copy_rows<4>(a, from, to, lane);
+  }
   if (!last) return;
   const int n_active = total;
   const int end = min((n_active + ttt::kLceBM - 1) / ttt::kLceBM * ttt::kLceBM, a.n_pad);
   for (int s = n_active + warp; s < end; s += 8) {
-    copy_row(a, -1, s, lane);
+    const int64_t from[1] = {-1}, to[1] = {s};
+    copy_rows<1>(a, from, to, lane);
     if (lane == 0) a.st.idx[s] = -1, a.st.tgt[s] = -1, a.st.mw[s] = 0.f, a.st.lse2[s] = INFINITY;
   }
   msum = block_sum(msum, buf);
@@ -358,9 +379,11 @@ __global__ void __launch_bounds__(256) lce_coef_kernel(const RowArgs a) {
     if (a.reduction == TTT_LCE_NONE) return a.dloss[a.st.idx[s]] * a.st.mw[s];
     return *a.dloss * (a.st.mw[s] / a.st.head->denom);
   };
-  for (int s = blockIdx.x * 8 + warp; s < end; s += gridDim.x * 8) {
-    copy_row(a, s < n_active ? a.st.idx[s] : -1, s, lane);
-    if (lane == 0) a.coef[s] = s < n_active ? coef(s) : 0.f;
+  for (int s = (blockIdx.x * 8 + warp) * 2; s < end; s += gridDim.x * 16) {  // end is even
+    const int64_t from[2] = {s < n_active ? a.st.idx[s] : -1, s + 1 < n_active ? a.st.idx[s + 1] : -1};
+    const int64_t to[2] = {s, s + 1};
+    copy_rows<2>(a, from, to, lane);
+    if (lane < 2) a.coef[s + lane] = s + lane < n_active ? coef(s + lane) : 0.f;
   }
   if (blockIdx.x != 0) return;
   float big = 0.f;
@@ -406,15 +429,23 @@ __global__ void __launch_bounds__(32 * kShares) lce_lse_kernel(const State st, c
   const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
   const int s = blockIdx.x * 32 + lane, n_active = st.head->n_active;
   float m = -INFINITY, l = 0.f;
-  auto merge = [&](float2 o) {
-    const float top = fmaxf(m, o.x);
-    const float sub = top == -INFINITY ? 0.f : top;
-    l = l * exp2f(m - sub) + o.y * exp2f(o.x - sub);
-    m = top;
-  };
   if (s < n_active) {
-#pragma unroll 4
-    for (int i = share; i < parts; i += kShares) merge(part[static_cast<int64_t>(i) * n_pad + s]);
+    constexpr int U = 8;
+    for (int i0 = share; i0 < parts; i0 += U * kShares) {
+      float2 o[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        o[u] = i0 + u * kShares < parts ? part[static_cast<int64_t>(i0 + u * kShares) * n_pad + s]
+                                        : make_float2(-INFINITY, 0.f);
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) top = fmaxf(top, o[u].x);
+      const float sub = top == -INFINITY ? 0.f : top;
+      l *= exp2f(m - sub);
+#pragma unroll
+      for (int u = 0; u < U; ++u) l += o[u].y * exp2f(o[u].x - sub);
+      m = top;
+    }
   }
   sh[share][lane] = make_float2(m, l);
   __syncthreads();
@@ -446,7 +477,7 @@ __global__ void __launch_bounds__(32 * kShares) lce_rho_kernel(const State st, c
   const int s = blockIdx.x * 32 + lane, n_active = st.head->n_active;
   float sum = 0.f, big = 0.f;
   if (s < n_active) {
-#pragma unroll 4
+#pragma unroll 8
     for (int i = share; i < parts; i += kShares) {
       const float2 o = part[static_cast<int64_t>(i) * n_pad + s];
       sum += o.x;
@@ -613,26 +644,27 @@ __global__ void lce_zero_rows_kernel(const int* slot, int64_t n, float* out) {
   if (i < n && slot[i] < 0) out[i] = 0.f;
 }
 
-// dh[i] = sum over the splits (in order) of acc[split][slot_i] / scale, 0 for rows left out. One warp per row.
+// dh[i] = sum over the splits (in order) of acc[split][slot_i] / scale, 0 for rows left
+// out. Four columns a thread at a time, 64 threads a row.
 template <bool BF16>
 __global__ void __launch_bounds__(256) lce_scatter_kernel(const int* slot, const LceCoef coef, const float* acc,
                                                           int splits, int64_t n, int n_pad, int dim, int dim_pad,
-                                                          uint16_t* dh) {
+                                                          int width, uint16_t* dh) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int per = 256 / width;  // rows of a block
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / width;
   if (i >= n) return;
-  const int lane = threadIdx.x & 31;
   const int s = slot[i];
   const float inv = 1.f / coef.scale();
   uint16_t* dst = dh + i * dim;
-#pragma unroll 2
-  for (int c = lane * 4; c < dim; c += 128) {
+#pragma unroll 4
+  for (int c = (threadIdx.x % width) * 4; c < dim; c += width * 4) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (s >= 0) {
+      const float* src = acc + static_cast<int64_t>(s) * dim_pad + c;
 #pragma unroll 4
       for (int k = 0; k < splits; ++k) {
-        const float4 o =
-            *reinterpret_cast<const float4*>(acc + (static_cast<int64_t>(k) * n_pad + s) * dim_pad + c);
+        const float4 o = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(k) * n_pad * dim_pad);
         v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
       }
     }
@@ -810,10 +842,13 @@ int run_pieces(const Pass& p, const Weight& w, const Weight* uw, bool second, bo
       return TTT_ERR_TENSOR_MAP;
     TTT_TRY(p.run(t, ttt::kLceProd));
   }
-  if (outh != nullptr)
-    TTT_TRY(launch_early(p.bf16 ? lce_scatter_kernel<true> : lce_scatter_kernel<false>, (q.n + 7) / 8, 256, p.s,
-                         p.st.slot, p.coef, p.w.acc, q.splits, q.n, static_cast<int>(q.n_pad), q.dim, q.dim_pad,
-                         outh));
+  if (outh != nullptr) {
+    int width = 8;  // threads of a row
+    while (width < 64 && width * 4 < q.dim) width *= 2;
+    TTT_TRY(launch_early(p.bf16 ? lce_scatter_kernel<true> : lce_scatter_kernel<false>,
+                         (q.n + 256 / width - 1) / (256 / width), 256, p.s, p.st.slot, p.coef, p.w.acc, q.splits, q.n,
+                         static_cast<int>(q.n_pad), q.dim, q.dim_pad, width, outh));
+  }
   return TTT_OK;
 }
 

@@ -132,14 +132,21 @@ struct LceCfg {
   static constexpr bool DUAL = KIND == kLceDualStats || KIND == kLceDualGrad;
   static constexpr bool GRAD = KIND == kLceGrad || KIND == kLceDualGrad;
   static constexpr int BM = kLceBM, BN = DUAL ? kLceBNDual : kLceBN;
-  static constexpr int BK = DUAL ? kLcePanel : kLceBK, PANELS = BK / kLcePanel;  // of a stage's contraction
+  // Contraction of a stage, and staging boxes of an epilogue warp. kLceGrad is bound by
+  // shared memory: a pair's products read 64 bytes a cycle and their loads write 64 of
+  // the 128 that it moves, and the staged G comes on top. With two boxes per warp beside
+  // five short stages it keeps 84 % of the tensor pipe at dim 768, with one beside three
+  // long ones 78 %, and 16 epilogue warps add nothing; the dual gradient kind needs its
+  // fourth stage more than second boxes (87 % against 80 %).
+  static constexpr int BK = DUAL || KIND == kLceGrad ? kLcePanel : kLceBK, PANELS = BK / kLcePanel;
   static constexpr int ROWS_A = BM / 2, ROWS_B = BN / 2;  // of a CTA
   static constexpr int TILE_A = ROWS_A * BK * 2, TILE_B = ROWS_B * BK * 2;
   static constexpr int STAGE = (DUAL ? 2 : 1) * (TILE_A + TILE_B);
-  static constexpr int NSTAGE = 196608 / STAGE;  // 192 KB: 3 single or 4 dual stages
-  static constexpr int PANEL = 32 * 128;         // staging of one warp's [32 x 64] 16-bit store box
+  static constexpr int PANEL = 32 * 128;  // staging of one warp's [32 x 64] 16-bit store box
+  static constexpr int BOXES = KIND == kLceGrad ? 2 : 1;
+  static constexpr int NSTAGE = (232448 - 1024 - 256 - 8 * BOXES * PANEL) / STAGE;
   static constexpr int OFF_STORE = NSTAGE * STAGE;
-  static constexpr int OFF_BAR = OFF_STORE + 8 * PANEL;
+  static constexpr int OFF_BAR = OFF_STORE + 8 * BOXES * PANEL;
   static constexpr int NBAR = 2 * NSTAGE + 9;
   static constexpr int SMEM = OFF_BAR + NBAR * 8 + 32 + 1024;
   static constexpr int NTHREADS = 320, WARP_LOAD = 8, WARP_MMA = 9;
@@ -234,13 +241,17 @@ struct LceWalk {
   }
 };
 
-// Packs 64 columns of this warp's 32 rows into its staging panel and stores the box at (x, y).
-template <bool BF16>
-TTT_DEV void store_panel(uint8_t* panel, const CUtensorMap* map, int lane, int x, int y, const float (&v)[64]) {
+// Packs 64 columns of this warp's 32 rows into one of its BOXES staging boxes (in
+// turn: `turn` counts them) and stores it at (x, y).
+template <bool BF16, int BOXES>
+TTT_DEV void store_panel(uint8_t* panel, int& turn, const CUtensorMap* map, int lane, int x, int y, const float (&v)[64]) {
   uint32_t w[32];
 #pragma unroll
   for (int j = 0; j < 32; ++j) w[j] = pack2<BF16>(v[2 * j], v[2 * j + 1]);
-  if (lane == 0) bulk_wait_read();  // the previous store has left the panel
+  panel += (turn % BOXES) * 4096;
+  ++turn;
+  // the box's previous store has left it
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BOXES - 1) : "memory");
   __syncwarp();
 #pragma unroll
   for (int ch = 0; ch < 8; ++ch)
@@ -430,7 +441,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
     const int quarter = warp & 3, half = warp >> 2;
     const int r = static_cast<int>(rank) * C::ROWS_A + quarter * 32 + lane;  // row of the tile
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    uint8_t* panel = smem + C::OFF_STORE + warp * C::PANEL;
+    uint8_t* panel = smem + C::OFF_STORE + warp * C::BOXES * C::PANEL;
+    int turn = 0;
     const uint32_t free_leader = peer_addr(acc_free, 0);
     const float mul = C::GRAD ? p.coef.scale() : (KIND == kLceProd ? 1.f / p.coef.scale() : 1.f);
     int nth = 0;
@@ -537,7 +549,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
             release();
 #pragma unroll
             for (int j = 0; j < 64; ++j) d[j] = coef * v[j] * (d[j] - rho);
-            store_panel<BF16>(panel, &p.out[1], lane, cq, row0, d);
+            store_panel<BF16, C::BOXES>(panel, turn, &p.out[1], lane, cq, row0, d);
           } else if (q == C::HALF / 64 - 1) {
             release();
           }
@@ -549,7 +561,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
           }
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] *= coef;
-          store_panel<BF16>(panel, &p.out[0], lane, cq, row0, v);
+          store_panel<BF16, C::BOXES>(panel, turn, &p.out[0], lane, cq, row0, v);
         }
       } else if (!tl.dw) {
         float* dst = p.acc + (static_cast<int64_t>(tl.split) * p.n_pad + slot) * p.dim_pad;
@@ -593,7 +605,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
           for (int j = 0; j < 64; ++j) v[j] *= mul;
           if (cq >= p.dim || row0 >= p.cols) continue;
           if (boxes) {
-            store_panel<BF16>(panel, &p.dw_out, lane, cq, row0, v);
+            store_panel<BF16, C::BOXES>(panel, turn, &p.dw_out, lane, cq, row0, v);
           } else if (row < p.cols) {
             uint16_t* dst = p.dw + static_cast<int64_t>(row) * p.dim + cq;
 #pragma unroll
