@@ -508,11 +508,11 @@ __global__ void __launch_bounds__(32 * kShares) lce_rho_kernel(const State st, c
 }
 
 // Losses of a few rows without gradients (the score of a token): a product with so
-// few rows is bound by reading w once, so CUDA cores form it. Every warp takes four
-// vocabulary rows at a time (their loads in flight together), adds up its lanes'
-// products with the rows of h held in shared memory, and keeps a running (max, sum)
-// per row; blocks write theirs as one part each, which lce_lse_kernel merges. Block
-// 0 lists the rows. Against the tensor-core path (list, 256-row tiles, merge) at 1 x
+// few rows is bound by reading w once, so CUDA cores form it. Every warp has an equal
+// range of the vocabulary, takes four rows at a time (their loads in flight together),
+// adds up its lanes' products with the rows of h held in shared memory, and keeps a
+// running (max, sum) per row; blocks write theirs as one part each, which
+// lce_lse_kernel merges. Block 0 lists the rows. Against the tensor-core path (list, 256-row tiles, merge) at 1 x
 // 768 x 32000 bf16 this saves a launch and 10 us of 26.
 constexpr int kScoreRows = 4, kScoreWarps = 16, kScoreMaxDim = 8192;
 template <bool BF16, int NR>
@@ -523,6 +523,12 @@ __global__ void __launch_bounds__(32 * kScoreWarps) lce_score_kernel(const RowAr
   __shared__ int rows[NR], tgts[NR], count;
   asm volatile("griddepcontrol.launch_dependents;");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // this warp's vocabulary rows, on their way into L2 while the block lists the tokens
+  const int64_t wid = static_cast<int64_t>(blockIdx.x) * kScoreWarps + warp, warps = gridDim.x * kScoreWarps;
+  const int v_begin = static_cast<int>(a.vocab * wid / warps), v_end = static_cast<int>(a.vocab * (wid + 1) / warps);
+  for (int v = v_begin; v < v_end; ++v)
+    for (int c = lane * 64; c < a.dim; c += 2048)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(w + v * w_stride + c));
   if (warp == 0) {
     float m = 0.f;
     int kind = 0;
@@ -565,9 +571,8 @@ __global__ void __launch_bounds__(32 * kScoreWarps) lce_score_kernel(const RowAr
   float mx[NR], sum[NR];
 #pragma unroll
   for (int r = 0; r < NR; ++r) mx[r] = -INFINITY, sum[r] = 0.f;
-  const int vocab = static_cast<int>(a.vocab);
   constexpr int U = 4;
-  for (int v0 = (blockIdx.x * kScoreWarps + warp) * U; v0 < vocab; v0 += gridDim.x * kScoreWarps * U) {
+  for (int v0 = v_begin; v0 < v_end; v0 += U) {
     float z[NR][U];
 #pragma unroll
     for (int r = 0; r < NR; ++r)
@@ -578,7 +583,8 @@ __global__ void __launch_bounds__(32 * kScoreWarps) lce_score_kernel(const RowAr
       uint4 q[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        q[u] = __ldcs(reinterpret_cast<const uint4*>(w + min(v0 + u, vocab - 1) * w_stride + c));
+        q[u] = v0 + u < v_end ? __ldcs(reinterpret_cast<const uint4*>(w + (v0 + u) * w_stride + c))
+                              : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         const uint4 hq = *reinterpret_cast<const uint4*>(hs + r * a.dim + c);
@@ -605,7 +611,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps) lce_score_kernel(const RowAr
     }
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      if (lane == 0 && r < nr && tgts[r] >= v0 && tgts[r] < v0 + U) {
+      if (lane == 0 && r < nr && tgts[r] >= v0 && tgts[r] < min(v0 + U, v_end)) {
         float zt = z[r][0];
 #pragma unroll
         for (int u = 1; u < U; ++u) zt = tgts[r] == v0 + u ? z[r][u] : zt;
@@ -614,7 +620,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps) lce_score_kernel(const RowAr
       float top = mx[r];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        z[r][u] = v0 + u < vocab ? z[r][u] * kLog2e : -INFINITY;
+        z[r][u] = v0 + u < v_end ? z[r][u] * kLog2e : -INFINITY;
         top = fmaxf(top, z[r][u]);
       }
       const float sub = top == -INFINITY ? 0.f : top;
@@ -885,8 +891,9 @@ int ttt_lce_fwd(const ttt_lce_fwd_args* a, void* stream) {
   r.targets = a->targets, r.mask = a->mask, r.loss = a->loss;
   const Weight w(a->w, a->w_stride, pb);
   if (a->need_state == 0 && pb.n <= kScoreRows && pb.dim % 8 == 0 && pb.dim <= kScoreMaxDim) {
-    const int blocks = static_cast<int>(std::min<int64_t>((pb.vocab + 4 * kScoreWarps - 1) / (4 * kScoreWarps),
-                                                          std::min<int64_t>(p.sms, score_parts(pb.vocab))));
+    // two blocks fit on an SM with one row of h, one with more; no warp has less than two vocabulary rows
+    const int64_t fit = std::min<int64_t>(p.sms * (pb.n == 1 ? 2 : 1), score_parts(pb.vocab));
+    const int blocks = static_cast<int>(std::min((pb.vocab + 2 * kScoreWarps - 1) / (2 * kScoreWarps), fit));
     auto kern = p.bf16 ? (pb.n == 1 ? lce_score_kernel<true, 1> : lce_score_kernel<true, kScoreRows>)
                        : (pb.n == 1 ? lce_score_kernel<false, 1> : lce_score_kernel<false, kScoreRows>);
     const int smem = (pb.n == 1 ? 1 : kScoreRows) * pb.dim * 2;
