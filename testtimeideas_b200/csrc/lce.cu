@@ -897,7 +897,7 @@ int ttt_lce_fwd(const ttt_lce_fwd_args* a, void* stream) {
     auto kern = p.bf16 ? (pb.n == 1 ? lce_score_kernel<true, 1> : lce_score_kernel<true, kScoreRows>)
                        : (pb.n == 1 ? lce_score_kernel<false, 1> : lce_score_kernel<false, kScoreRows>);
     const int smem = (pb.n == 1 ? 1 : kScoreRows) * pb.dim * 2;
-    if (smem > 48 * 1024) TTT_TRY(launched(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)));
+    if (smem > 32 * 1024) TTT_TRY(launched(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)));
     kern<<<blocks, 32 * kScoreWarps, smem, p.s>>>(r, w.p, w.stride, p.w.part, p.w.ztgt);
     TTT_TRY(launched());
     return launch_early(lce_lse_kernel, 1, 32 * kShares, p.s, p.st, p.w.part, p.w.ztgt, blocks, static_cast<int>(p.q.n_pad),

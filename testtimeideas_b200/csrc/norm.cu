@@ -15,8 +15,9 @@
 // All three are bound by memory: 2, 3 and 5 passes over [rows, D]. A row is read
 // once and stays, packed as it came, in the registers of the NT threads that own
 // it: eight elements each up to 2048 (16 to 32 above), so that a thread needs few
-// registers and an SM holds enough rows in flight to cover the memory's latency
-// (32 elements a thread took 170 registers and ran at a quarter of the bandwidth).
+// registers (32 elements a thread took 170 and ran at a quarter of the bandwidth).
+// Rows come through shared memory up to three ahead of their turn (cp.async), which is
+// what covers the memory's latency.
 // Mean and variance are two sums over registers, and no statistic is a difference
 // of large sums. The threads of a row own fixed columns, so the parameter gradients
 // are summed in registers over all rows that a block meets; the blocks' sums (fp32)
@@ -202,6 +203,76 @@ __device__ __forceinline__ void row_sum(float (&v)[N], Sums<R>& sums, int& phase
   }
 }
 
+// Rows on their way through shared memory: T tensors, S rows ahead of the one being
+// summed (cp.async, 16 bytes a thread and piece). A thread reads back only what it
+// copied itself, so no barrier is needed. Rows that are not 16-byte aligned, or so wide
+// that fewer than two fit, are loaded into registers one row ahead instead (S = 0).
+template <class X, class R, int T, int PER_SM>
+struct Ring {
+  static constexpr int ROW = R::K * R::THREADS * 16;  // bytes of one tensor's rows of a block
+  static constexpr int FIT = (200 << 10) / (PER_SM * T * ROW);
+  static constexpr int S = R::VEC == 1 || FIT < 2 ? 0 : (FIT < 4 ? FIT : 4);
+  static constexpr int BYTES = S * T * ROW;
+  const X* src[T];
+  int64_t stride[T];
+  uint32_t base;
+  int t, D;
+
+  // Starts the copies of row `at` (none past the end) into stage `st`.
+  __device__ __forceinline__ void fetch(int64_t at, int64_t rows, int st) const {
+    if (at < rows) {
+#pragma unroll
+      for (int i = 0; i < T; ++i) {
+        if (src[i] == nullptr) continue;
+        const X* row = src[i] + at * stride[i];
+#pragma unroll
+        for (int k = 0; k < R::K; ++k) {
+          const int c = R::column(k, t);
+          if (c < D)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                             base + (st * T + i) * ROW + k * R::THREADS * 16),
+                         "l"(row + c)
+                         : "memory");
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // The oldest row's copies have landed (S - 1 newer rows may be on their way).
+  __device__ __forceinline__ void wait() const {
+    asm volatile("cp.async.wait_group %0;" ::"n"(S > 0 ? S - 1 : 0) : "memory");
+  }
+  __device__ __forceinline__ void read(int st, int i, Pack<X, R::EPT>& v) const {
+    constexpr int WORDS = 4;
+#pragma unroll
+    for (int k = 0; k < R::K; ++k) {
+      uint32_t* w = v.w + k * WORDS;
+      if (src[i] != nullptr && R::column(k, t) < D) {
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(base + (st * T + i) * ROW + k * R::THREADS * 16)
+                     : "memory");
+      } else {
+        w[0] = w[1] = w[2] = w[3] = 0;
+      }
+    }
+  }
+};
+template <class G>
+__device__ __forceinline__ G make_ring(uint8_t* smem, int t, int D) {
+  G g;
+  g.base = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + threadIdx.x * 16;
+  g.t = t;
+  g.D = D;
+  return g;
+}
+template <class X, class R>
+using FwdRing = Ring<X, R, 1, R::FWD_PER_SM>;
+template <class X, class R>
+using BwdRing = Ring<X, R, 2, R::BWD_PER_SM>;
+template <class X, class R>
+using Bwd2Ring = Ring<X, R, 3, R::BWD2_PER_SM>;
+
 template <class X, class P>
 struct NormArgs {
   const X *x, *dy, *ux;
@@ -219,6 +290,8 @@ struct NormArgs {
 template <class X, class P, class R>
 __global__ void __launch_bounds__(R::THREADS, R::FWD_PER_SM) norm_fwd_kernel(const NormArgs<X, P> a) {
   constexpr int EPT = R::EPT;
+  using G = FwdRing<X, R>;
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Sums<R> sums;
   int phase = 0;
   const int t = threadIdx.x % R::NT;
@@ -226,14 +299,30 @@ __global__ void __launch_bounds__(R::THREADS, R::FWD_PER_SM) norm_fwd_kernel(con
   const int64_t step = static_cast<int64_t>(gridDim.x) * R::GROUPS;
   int64_t row = static_cast<int64_t>(blockIdx.x) * R::GROUPS + threadIdx.x / R::NT;
   if (row >= a.rows) return;  // whole groups, which have their own barriers
-  Pack<X, EPT> xn;  // the next row, loaded while this one is summed
-  R::load(a.x + row * a.x_stride, t, a.D, xn);
+  G g = make_ring<G>(smem, t, a.D);
+  g.src[0] = a.x;
+  g.stride[0] = a.x_stride;
+  Pack<X, EPT> xn;  // S = 0: the next row
+  if constexpr (G::S > 0) {
+#pragma unroll
+    for (int i = 0; i < G::S - 1; ++i) g.fetch(row + i * step, a.rows, i);
+  } else {
+    R::load(a.x + row * a.x_stride, t, a.D, xn);
+  }
   Pack<P, EPT> w, b;
   R::load(a.w, t, a.D, w, 1.f);
   R::load(a.b, t, a.D, b, 0.f);
-  for (; row < a.rows; row += step) {
-    Pack<X, EPT> x = xn;
-    if (row + step < a.rows) R::load(a.x + (row + step) * a.x_stride, t, a.D, xn);
+  for (int st = 0; row < a.rows; row += step) {
+    Pack<X, EPT> x;
+    if constexpr (G::S > 0) {
+      g.fetch(row + (G::S - 1) * step, a.rows, (st + G::S - 1) % G::S);
+      g.wait();
+      g.read(st, 0, x);
+      st = (st + 1) % G::S;
+    } else {
+      x = xn;
+      if (row + step < a.rows) R::load(a.x + (row + step) * a.x_stride, t, a.D, xn);
+    }
     float s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < EPT; ++i) s[0] += x.at(i);
@@ -291,7 +380,9 @@ __device__ __forceinline__ void write_part(float* part, int which, int D, const 
 template <class X, class P, class R>
 __global__ void __launch_bounds__(R::THREADS, R::BWD_PER_SM) norm_bwd_kernel(const NormArgs<X, P> a) {
   constexpr int EPT = R::EPT;
-  extern __shared__ float cols[];
+  using G = BwdRing<X, R>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* cols = reinterpret_cast<float*>(smem + G::BYTES);
   __shared__ Sums<R> sums;
   int phase = 0;
   asm volatile("griddepcontrol.launch_dependents;");  // the parameter sums wait for this grid's end
@@ -304,20 +395,41 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD_PER_SM) norm_bwd_kernel(con
   R::load(a.w, t, a.D, w, 1.f);
   const int64_t step = static_cast<int64_t>(gridDim.x) * R::GROUPS;
   int64_t row = static_cast<int64_t>(blockIdx.x) * R::GROUPS + threadIdx.x / R::NT;
-  Pack<X, EPT> xn, dn;  // the next row, loaded while this one is summed
-  float mun = 0.f, rn = 0.f;
-  auto fetch = [&](int64_t at) {
-    if (at >= a.rows) return;
-    R::load(a.x + at * a.x_stride, t, a.D, xn);
-    R::load(a.dy + at * a.dy_stride, t, a.D, dn);
-    mun = a.mean[at];
-    rn = a.rstd[at];
+  G ring = make_ring<G>(smem, t, a.D);
+  ring.src[0] = a.x, ring.stride[0] = a.x_stride;
+  ring.src[1] = a.dy, ring.stride[1] = a.dy_stride;
+  Pack<X, EPT> xn, dn;  // S = 0: the next row
+  float mun[2], rn[2];  // statistics of the next two rows
+  auto fetch_stats = [&](int64_t at, int i) {
+    if (at < a.rows) mun[i] = a.mean[at], rn[i] = a.rstd[at];
   };
-  fetch(row);
-  for (; row < a.rows; row += step) {
-    Pack<X, EPT> x = xn, dy = dn;
-    const float mu = mun, r = rn;
-    fetch(row + step);
+  fetch_stats(row, 0);
+  fetch_stats(row + step, 1);
+  if constexpr (G::S > 0) {
+#pragma unroll
+    for (int i = 0; i < G::S - 1; ++i) ring.fetch(row + i * step, a.rows, i);
+  } else if (row < a.rows) {
+    R::load(a.x + row * a.x_stride, t, a.D, xn);
+    R::load(a.dy + row * a.dy_stride, t, a.D, dn);
+  }
+  for (int st = 0; row < a.rows; row += step) {
+    Pack<X, EPT> x, dy;
+    const float mu = mun[0], r = rn[0];
+    mun[0] = mun[1], rn[0] = rn[1];
+    fetch_stats(row + 2 * step, 1);
+    if constexpr (G::S > 0) {
+      ring.fetch(row + (G::S - 1) * step, a.rows, (st + G::S - 1) % G::S);
+      ring.wait();
+      ring.read(st, 0, x);
+      ring.read(st, 1, dy);
+      st = (st + 1) % G::S;
+    } else {
+      x = xn, dy = dn;
+      if (row + step < a.rows) {
+        R::load(a.x + (row + step) * a.x_stride, t, a.D, xn);
+        R::load(a.dy + (row + step) * a.dy_stride, t, a.D, dn);
+      }
+    }
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
@@ -348,7 +460,9 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD_PER_SM) norm_bwd_kernel(con
 template <class X, class P, class R>
 __global__ void __launch_bounds__(R::THREADS, R::BWD2_PER_SM) norm_bwd2_kernel(const NormArgs<X, P> a) {
   constexpr int EPT = R::EPT;
-  extern __shared__ float cols[];
+  using G = Bwd2Ring<X, R>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* cols = reinterpret_cast<float*>(smem + G::BYTES);
   __shared__ Sums<R> sums;
   int phase = 0;
   asm volatile("griddepcontrol.launch_dependents;");
@@ -362,12 +476,33 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD2_PER_SM) norm_bwd2_kernel(c
   R::load(a.uw, t, a.D, uw);
   R::load(a.ub, t, a.D, ub);
   const int64_t step = static_cast<int64_t>(gridDim.x) * R::GROUPS;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * R::GROUPS + threadIdx.x / R::NT; row < a.rows; row += step) {
-    const float mu = a.mean[row], r = a.rstd[row];
+  int64_t row = static_cast<int64_t>(blockIdx.x) * R::GROUPS + threadIdx.x / R::NT;
+  G ring = make_ring<G>(smem, t, a.D);
+  ring.src[0] = a.x, ring.stride[0] = a.x_stride;
+  ring.src[1] = a.dy, ring.stride[1] = a.dy_stride;
+  ring.src[2] = a.ux, ring.stride[2] = a.ux_stride;
+  float mun = 0.f, rn = 0.f;
+  if (row < a.rows) mun = a.mean[row], rn = a.rstd[row];
+  if constexpr (G::S > 0) {
+#pragma unroll
+    for (int i = 0; i < G::S - 1; ++i) ring.fetch(row + i * step, a.rows, i);
+  }
+  for (int st = 0; row < a.rows; row += step) {
+    const float mu = mun, r = rn;
+    if (row + step < a.rows) mun = a.mean[row + step], rn = a.rstd[row + step];
     Pack<X, EPT> x, dy, u;
-    R::load(a.x + row * a.x_stride, t, a.D, x);
-    R::load(a.dy + row * a.dy_stride, t, a.D, dy);
-    R::load(a.ux == nullptr ? nullptr : a.ux + row * a.ux_stride, t, a.D, u);
+    if constexpr (G::S > 0) {
+      ring.fetch(row + (G::S - 1) * step, a.rows, (st + G::S - 1) % G::S);
+      ring.wait();
+      ring.read(st, 0, x);
+      ring.read(st, 1, dy);
+      ring.read(st, 2, u);
+      st = (st + 1) % G::S;
+    } else {
+      R::load(a.x + row * a.x_stride, t, a.D, x);
+      R::load(a.dy + row * a.dy_stride, t, a.D, dy);
+      R::load(a.ux == nullptr ? nullptr : a.ux + row * a.ux_stride, t, a.D, u);
+    }
     float s[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // g, u, g xh, u xh, h, h xh
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
@@ -484,17 +619,22 @@ enum Pass { kFwd, kBwd, kBwd2 };
 
 template <class X, class P, class R>
 cudaError_t launch_rows(const NormArgs<X, P>& a, Pass pass, int blocks, int sms, cudaStream_t s) {
+  auto launch = [&](auto kern, int64_t grid, int smem) {
+    if (smem > 32 * 1024) {  // 48 KB, the kernels' static shared memory included, need no permission
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return e;
+    }
+    kern<<<static_cast<unsigned>(grid), R::THREADS, smem, s>>>(a);
+    return cudaGetLastError();
+  };
   if (pass == kFwd) {
     const int64_t need = (a.rows + R::GROUPS - 1) / R::GROUPS, fit = static_cast<int64_t>(sms) * R::FWD_PER_SM;
-    norm_fwd_kernel<X, P, R><<<static_cast<unsigned>(std::min(need, fit)), R::THREADS, 0, s>>>(a);
-    return cudaGetLastError();
+    return launch(norm_fwd_kernel<X, P, R>, std::min(need, fit), FwdRing<X, R>::BYTES);
   }
-  const size_t smem = R::GROUPS > 1 ? sizeof(float) * R::GROUPS * a.D : 0;  // at most 16 KB: D <= 8 * NT
-  if (pass == kBwd)
-    norm_bwd_kernel<X, P, R><<<blocks, R::THREADS, smem, s>>>(a);
-  else
-    norm_bwd2_kernel<X, P, R><<<blocks, R::THREADS, smem, s>>>(a);
-  return cudaGetLastError();
+  // several rows a block: their column sums, at most 8 KB (D <= 8 NT, 256 threads)
+  const int cols = R::GROUPS > 1 ? static_cast<int>(sizeof(float)) * R::GROUPS * a.D : 0;
+  if (pass == kBwd) return launch(norm_bwd_kernel<X, P, R>, blocks, BwdRing<X, R>::BYTES + cols);
+  return launch(norm_bwd2_kernel<X, P, R>, blocks, Bwd2Ring<X, R>::BYTES + cols);
 }
 
 template <class X, class P, bool WIDE>
