@@ -181,16 +181,16 @@ def _register_fakes() -> None:
     @torch.library.register_fake("ttt::layer_norm")
     def _ln(x, w, b, eps, need_stats):
         stats = x.new_empty((2, x.numel() // x.shape[-1] if need_stats else 0), dtype=torch.float32)
-        return x.new_empty(x.shape), stats[0], stats[1]
+        return x.new_empty(x.shape), stats
 
     @torch.library.register_fake("ttt::layer_norm_bwd")
-    def _ln_bwd(dy, x, w, mean, rstd, need_dx, need_dw, need_db, p_type):
+    def _ln_bwd(dy, x, w, stats, need_dx, need_dw, need_db, p_type):
         d = x.shape[-1]
         return (x.new_empty(x.shape if need_dx else (0,)), x.new_empty((d if need_dw else 0,), dtype=p_type),
                 x.new_empty((d if need_db else 0,), dtype=p_type))
 
     @torch.library.register_fake("ttt::layer_norm_bwd2")
-    def _ln_bwd2(dy, x, w, mean, rstd, ux, uw, ub):
+    def _ln_bwd2(dy, x, w, stats, ux, uw, ub):
         gw = x.new_empty((0,)) if w is None else w.new_empty(w.shape)
         return x.new_empty(x.shape), x.new_empty(x.shape), gw
 

@@ -33,11 +33,33 @@ int type_code(at::ScalarType t) {
 
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 
-// x as [rows, dim] with unit column stride: a view where the layout allows one, else a copy.
-at::Tensor as_rows(const at::Tensor& x, int64_t dim) {
-  at::Tensor r = x.reshape({-1, dim});
-  return (r.size(0) == 0 || dim == 1 || r.stride(1) == 1) && (r.size(0) < 2 || r.stride(0) >= 0) ? r : r.contiguous();
-}
+// A tensor's last dimension as rows of unit column stride: the tensor itself where its
+// layout is one row stride over all leading dimensions, else a contiguous copy.
+struct Rows {
+  at::Tensor keep;
+  void* p = nullptr;
+  int64_t stride = 0;
+  Rows() = default;
+  Rows(const at::Tensor& x, int64_t dim) : keep(x), stride(dim) {
+    bool ok = dim == 1 || x.stride(-1) == 1;
+    if (ok && !x.is_contiguous()) {
+      int64_t inner = -1;  // row stride; every outer dimension must step over whole inner ones
+      int64_t span = 1;
+      for (int64_t d = x.dim() - 2; d >= 0 && ok; --d) {
+        if (x.size(d) == 1) continue;
+        if (inner < 0) inner = x.stride(d);
+        ok = x.stride(d) == inner * span && inner >= 0;
+        span *= x.size(d);
+      }
+      if (inner >= 0) stride = inner;
+    }
+    if (!ok) {
+      keep = x.contiguous();
+      stride = dim;
+    }
+    if (keep.numel() > 0) p = keep.data_ptr();
+  }
+};
 
 void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
@@ -78,69 +100,68 @@ ttt_norm_problem norm_problem(const at::Tensor& x, const OptTensor& w, const Opt
 
 at::Tensor vec(const OptTensor& p) { return p.has_value() ? p->contiguous() : at::Tensor(); }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> op_layer_norm(const at::Tensor& x_, const OptTensor& w_,
-                                                             const OptTensor& b_, double eps, bool need_stats) {
+std::tuple<at::Tensor, at::Tensor> op_layer_norm(const at::Tensor& x_, const OptTensor& w_, const OptTensor& b_,
+                                                 double eps, bool need_stats) {
   const ttt_norm_problem pb = norm_problem(x_, w_, b_, eps);
   c10::cuda::CUDAGuard guard(x_.device());
   at::Tensor word = error_word_for(x_.get_device());
   raise_if_pending(x_.get_device(), word);
-  const at::Tensor x = as_rows(x_, pb.dim), w = vec(w_), b = vec(b_);
+  const Rows x(x_, pb.dim);
+  const at::Tensor w = vec(w_), b = vec(b_);
   at::Tensor y = at::empty(x_.sizes(), x_.options());
   at::Tensor stats = at::empty({2, need_stats ? pb.rows : 0}, x_.options().dtype(at::kFloat));
-  at::Tensor mean = stats.select(0, 0), rstd = stats.select(0, 1);
   ttt_norm_fwd_args a{};
   a.pb = pb;
-  a.x = ptr(x);
-  a.x_stride = x.stride(0);
+  a.x = x.p;
+  a.x_stride = x.stride;
   a.w = ptr(w);
   a.b = ptr(b);
   a.y = y.data_ptr();
-  if (need_stats) {
-    a.mean = mean.data_ptr<float>();
-    a.rstd = rstd.data_ptr<float>();
-    if (pb.rows == 0) a.mean = a.rstd = nullptr;
+  if (need_stats && pb.rows > 0) {
+    a.mean = stats.data_ptr<float>();
+    a.rstd = a.mean + pb.rows;
   }
   check(ttt_norm_fwd(&a, stream()), "ttt::layer_norm");
-  return {y, mean, rstd};
+  return {y, stats};
 }
 
 // The gradient inputs of both gradients: dy, ux as rows of x's dtype.
-at::Tensor grad_rows(const at::Tensor& g, const at::Tensor& x, int64_t dim, const char* what) {
+Rows grad_rows(const at::Tensor& g, const at::Tensor& x, int64_t dim, const char* what) {
   TORCH_CHECK(g.sizes() == x.sizes(), "layer norm: ", what, " must have x's shape");
   TORCH_CHECK(g.device() == x.device(), "layer norm: ", what, " must be on x's device");
-  return as_rows(g.to(x.scalar_type()), dim);
+  return Rows(g.scalar_type() == x.scalar_type() ? g : g.to(x.scalar_type()), dim);
 }
 
-void check_stats(const at::Tensor& mean, const at::Tensor& rstd, int64_t rows) {
-  for (const at::Tensor* s : {&mean, &rstd})
-    TORCH_CHECK(s->is_cuda() && s->scalar_type() == at::kFloat && s->numel() == rows && s->is_contiguous(),
-                "layer norm: mean and rstd must be the forward's fp32 [rows]");
+void check_stats(const at::Tensor& stats, int64_t rows) {
+  TORCH_CHECK(stats.is_cuda() && stats.scalar_type() == at::kFloat && stats.numel() == 2 * rows && stats.is_contiguous(),
+              "layer norm: stats must be the forward's fp32 [2, rows]");
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> op_layer_norm_bwd(const at::Tensor& dy_, const at::Tensor& x_,
-                                                                 const OptTensor& w_, const at::Tensor& mean,
-                                                                 const at::Tensor& rstd, bool need_dx, bool need_dw,
-                                                                 bool need_db, at::ScalarType p_type) {
+                                                                 const OptTensor& w_, const at::Tensor& stats,
+                                                                 bool need_dx, bool need_dw, bool need_db,
+                                                                 at::ScalarType p_type) {
   ttt_norm_problem pb = norm_problem(x_, w_, std::nullopt, 0.0);
   pb.p_dtype = type_code(p_type);
   c10::cuda::CUDAGuard guard(x_.device());
   at::Tensor word = error_word_for(x_.get_device());
   raise_if_pending(x_.get_device(), word);
-  check_stats(mean, rstd, pb.rows);
-  const at::Tensor x = as_rows(x_, pb.dim), dy = grad_rows(dy_, x_, pb.dim, "dy"), w = vec(w_);
+  check_stats(stats, pb.rows);
+  const Rows x(x_, pb.dim), dy = grad_rows(dy_, x_, pb.dim, "dy");
+  const at::Tensor w = vec(w_);
   const auto po = x_.options().dtype(p_type);
   at::Tensor dx = need_dx ? at::empty(x_.sizes(), x_.options()) : at::empty({0}, x_.options());
   at::Tensor dw = at::empty({need_dw ? pb.dim : 0}, po), db = at::empty({need_db ? pb.dim : 0}, po);
   at::Tensor work = need_dw || need_db ? scratch(ttt_norm_work_bytes(&pb), x_) : at::Tensor();
   ttt_norm_bwd_args a{};
   a.pb = pb;
-  a.x = ptr(x);
-  a.dy = ptr(dy);
-  a.x_stride = x.stride(0);
-  a.dy_stride = dy.stride(0);
+  a.x = x.p;
+  a.dy = dy.p;
+  a.x_stride = x.stride;
+  a.dy_stride = dy.stride;
   a.w = ptr(w);
-  a.mean = mean.data_ptr<float>();
-  a.rstd = rstd.data_ptr<float>();
+  a.mean = stats.data_ptr<float>();
+  a.rstd = a.mean + pb.rows;
   a.dx = need_dx ? dx.data_ptr() : nullptr;
   a.dw = need_dw ? dw.data_ptr() : nullptr;
   a.db = need_db ? db.data_ptr() : nullptr;
@@ -151,17 +172,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_layer_norm_bwd(const at::Tenso
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> op_layer_norm_bwd2(const at::Tensor& dy_, const at::Tensor& x_,
-                                                                  const OptTensor& w_, const at::Tensor& mean,
-                                                                  const at::Tensor& rstd, const OptTensor& ux_,
-                                                                  const OptTensor& uw_, const OptTensor& ub_) {
+                                                                  const OptTensor& w_, const at::Tensor& stats,
+                                                                  const OptTensor& ux_, const OptTensor& uw_,
+                                                                  const OptTensor& ub_) {
   const ttt_norm_problem pb = norm_problem(x_, w_, std::nullopt, 0.0);
   c10::cuda::CUDAGuard guard(x_.device());
   at::Tensor word = error_word_for(x_.get_device());
   raise_if_pending(x_.get_device(), word);
-  check_stats(mean, rstd, pb.rows);
+  check_stats(stats, pb.rows);
   const auto pt = w_.has_value() ? w_->scalar_type() : x_.scalar_type();
-  const at::Tensor x = as_rows(x_, pb.dim), dy = grad_rows(dy_, x_, pb.dim, "dy"), w = vec(w_);
-  const at::Tensor ux = ux_.has_value() ? grad_rows(*ux_, x_, pb.dim, "ux") : at::Tensor();
+  const Rows x(x_, pb.dim), dy = grad_rows(dy_, x_, pb.dim, "dy");
+  const at::Tensor w = vec(w_);
+  const Rows ux = ux_.has_value() ? grad_rows(*ux_, x_, pb.dim, "ux") : Rows();
   at::Tensor up[2];
   for (int i = 0; i < 2; ++i) {
     const OptTensor& u = i == 0 ? uw_ : ub_;
@@ -175,17 +197,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_layer_norm_bwd2(const at::Tens
   at::Tensor work = w_.has_value() ? scratch(ttt_norm_work_bytes(&pb), x_) : at::Tensor();
   ttt_norm_bwd2_args a{};
   a.pb = pb;
-  a.x = ptr(x);
-  a.dy = ptr(dy);
-  a.ux = ptr(ux);
-  a.x_stride = x.stride(0);
-  a.dy_stride = dy.stride(0);
-  a.ux_stride = ux.defined() ? ux.stride(0) : 0;
+  a.x = x.p;
+  a.dy = dy.p;
+  a.ux = ux.p;
+  a.x_stride = x.stride;
+  a.dy_stride = dy.stride;
+  a.ux_stride = ux.stride;
   a.w = ptr(w);
   a.uw = ptr(up[0]);
   a.ub = ptr(up[1]);
-  a.mean = mean.data_ptr<float>();
-  a.rstd = rstd.data_ptr<float>();
+  a.mean = stats.data_ptr<float>();
+  a.rstd = a.mean + pb.rows;
   a.gx = gx.data_ptr();
   a.gw = w_.has_value() ? gw.data_ptr() : nullptr;
   a.gdy = gdy.data_ptr();
@@ -256,7 +278,8 @@ std::tuple<at::Tensor, at::Tensor> op_linear_ce(const at::Tensor& h_, const at::
     mask = (u8 ? *mask_ : mask_->to(at::kFloat)).contiguous();
     pb.mask_kind = u8 ? TTT_LCE_MASK_U8 : TTT_LCE_MASK_F32;
   }
-  const at::Tensor h = as_rows(h_, pb.dim), w = weight_rows(w_);
+  const Rows h(h_, pb.dim);
+  const at::Tensor w = weight_rows(w_);
   const at::Tensor targets = targets_.to(at::kLong).contiguous();
   const auto f32 = h_.options().dtype(at::kFloat);
   at::Tensor loss = reduction == TTT_LCE_NONE ? at::empty(targets_.sizes(), f32) : at::empty({}, f32);
@@ -264,8 +287,8 @@ std::tuple<at::Tensor, at::Tensor> op_linear_ce(const at::Tensor& h_, const at::
   at::Tensor work = lce_work(pb, 0, h_);
   ttt_lce_fwd_args a{};
   a.pb = pb;
-  a.h = h.numel() > 0 ? h.data_ptr() : nullptr;
-  a.h_stride = h.stride(0);
+  a.h = h.p;
+  a.h_stride = h.stride;
   a.w = w.data_ptr();
   a.w_stride = w.stride(0);
   a.targets = pb.n > 0 ? targets.data_ptr<int64_t>() : nullptr;
@@ -300,14 +323,15 @@ std::tuple<at::Tensor, at::Tensor> op_linear_ce_bwd(const at::Tensor& dloss_, co
   at::Tensor word = error_word_for(h_.get_device());
   raise_if_pending(h_.get_device(), word);
   check_state(state, pb);
-  const at::Tensor h = as_rows(h_, pb.dim), w = weight_rows(w_), dloss = lce_upstream(dloss_, h_, pb);
+  const Rows h(h_, pb.dim);
+  const at::Tensor w = weight_rows(w_), dloss = lce_upstream(dloss_, h_, pb);
   at::Tensor dh = need_dh ? at::empty(h_.sizes(), h_.options()) : at::empty({0}, h_.options());
   at::Tensor dw = need_dw ? at::empty(w_.sizes(), w_.options()) : at::empty({0}, w_.options());
   at::Tensor work = lce_work(pb, 1, h_);
   ttt_lce_bwd_args a{};
   a.pb = pb;
-  a.h = h.numel() > 0 ? h.data_ptr() : nullptr;
-  a.h_stride = h.stride(0);
+  a.h = h.p;
+  a.h_stride = h.stride;
   a.w = w.data_ptr();
   a.w_stride = w.stride(0);
   a.state = state.data_ptr();
@@ -331,12 +355,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_linear_ce_bwd2(const at::Tenso
   at::Tensor word = error_word_for(h_.get_device());
   raise_if_pending(h_.get_device(), word);
   check_state(state, pb);
-  const at::Tensor h = as_rows(h_, pb.dim), w = weight_rows(w_), dloss = lce_upstream(dloss_, h_, pb);
-  at::Tensor uh, uw;
+  const Rows h(h_, pb.dim);
+  const at::Tensor w = weight_rows(w_), dloss = lce_upstream(dloss_, h_, pb);
+  Rows uh;
+  at::Tensor uw;
   if (uh_.has_value()) {
     TORCH_CHECK(uh_->sizes() == h_.sizes() && uh_->device() == h_.device(),
                 "linear cross entropy: uh must have hidden's shape and device");
-    uh = as_rows(uh_->to(h_.scalar_type()), pb.dim);
+    uh = Rows(uh_->to(h_.scalar_type()), pb.dim);
   }
   if (uw_.has_value()) {
     TORCH_CHECK(uw_->sizes() == w_.sizes() && uw_->device() == h_.device(),
@@ -349,12 +375,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_linear_ce_bwd2(const at::Tenso
   at::Tensor work = lce_work(pb, 2, h_);
   ttt_lce_bwd2_args a{};
   a.pb = pb;
-  a.h = h.numel() > 0 ? h.data_ptr() : nullptr;
-  a.h_stride = h.stride(0);
+  a.h = h.p;
+  a.h_stride = h.stride;
   a.w = w.data_ptr();
   a.w_stride = w.stride(0);
-  a.uh = uh.defined() && pb.n > 0 ? uh.data_ptr() : nullptr;
-  a.uh_stride = uh.defined() ? uh.stride(0) : 0;
+  a.uh = uh.p;
+  a.uh_stride = uh.stride;
   a.uw = uw.defined() ? uw.data_ptr() : nullptr;
   a.uw_stride = uw.defined() ? uw.stride(0) : 0;
   a.state = state.data_ptr();
@@ -429,22 +455,22 @@ void mark_last(variable_list& outs, variable_list inputs) {
 // (dy, x, w) -> (dx, dw, db); `need` has a bit per output.
 struct LayerNormBwdFn : torch::autograd::Function<LayerNormBwdFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& dy, const at::Tensor& x, const OptTensor& w,
-                               const at::Tensor& mean, const at::Tensor& rstd, int64_t need, int64_t p_type) {
+                               const at::Tensor& stats, int64_t need, int64_t p_type) {
     at::AutoDispatchBelowADInplaceOrView below;
-    ctx->save_for_backward({dy, x, defined_or(w), mean, rstd});
+    ctx->save_for_backward({dy, x, defined_or(w), stats});
     ctx->set_materialize_grads(false);
-    auto [dx, dw, db] = raw_layer_norm_bwd().call(dy, x, w, mean, rstd, (need & 1) != 0, (need & 2) != 0,
-                                                  (need & 4) != 0, static_cast<at::ScalarType>(p_type));
+    auto [dx, dw, db] = raw_layer_norm_bwd().call(dy, x, w, stats, (need & 1) != 0, (need & 2) != 0, (need & 4) != 0,
+                                                  static_cast<at::ScalarType>(p_type));
     return {dx, dw, db};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& up) {
     const variable_list v = ctx->get_saved_variables();
-    variable_list g(7);
+    variable_list g(6);
     if (!up[0].defined() && !up[1].defined() && !up[2].defined()) return g;
     {
       at::AutoDispatchBelowADInplaceOrView below;
       std::tie(g[0], g[1], g[2]) =
-          raw_layer_norm_bwd2().call(v[0], v[1], opt(v[2]), v[3], v[4], opt(up[0]), opt(up[1]), opt(up[2]));
+          raw_layer_norm_bwd2().call(v[0], v[1], opt(v[2]), v[3], opt(up[0]), opt(up[1]), opt(up[2]));
       g[0] = g[0].to(v[0].scalar_type());
       if (!v[2].defined()) g[2] = at::Tensor();
     }
@@ -457,8 +483,8 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& w, const OptTensor& b,
                             double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [y, mean, rstd] = raw_layer_norm().call(x, w, b, eps, true);
-    ctx->save_for_backward({x, defined_or(w), mean, rstd});
+    auto [y, stats] = raw_layer_norm().call(x, w, b, eps, true);
+    ctx->save_for_backward({x, defined_or(w), stats});
     ctx->set_materialize_grads(false);
     ctx->saved_data["p_type"] = static_cast<int64_t>((w.has_value() ? *w : (b.has_value() ? *b : x)).scalar_type());
     ctx->saved_data["has_b"] = b.has_value();
@@ -476,12 +502,11 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     if (has_b && ctx->needs_input_grad(has_w ? 2 : 1)) need |= 4;
     variable_list out;
     if (at::GradMode::is_enabled()) {
-      out = LayerNormBwdFn::apply(up[0], v[0], opt(v[1]), v[2], v[3], need, p_type);
+      out = LayerNormBwdFn::apply(up[0], v[0], opt(v[1]), v[2], need, p_type);
     } else {
       at::AutoDispatchBelowADInplaceOrView below;
-      auto [dx, dw, db] = raw_layer_norm_bwd().call(up[0], v[0], opt(v[1]), v[2], v[3], (need & 1) != 0,
-                                                    (need & 2) != 0, (need & 4) != 0,
-                                                    static_cast<at::ScalarType>(p_type));
+      auto [dx, dw, db] = raw_layer_norm_bwd().call(up[0], v[0], opt(v[1]), v[2], (need & 1) != 0, (need & 2) != 0,
+                                                    (need & 4) != 0, static_cast<at::ScalarType>(p_type));
       out = {dx, dw, db};
     }
     for (int i = 0; i < 3; ++i)
@@ -574,14 +599,13 @@ at::Tensor op_linear_ce_ad(const at::Tensor& h, const at::Tensor& w, const at::T
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(ttt, m) {
-  // mean and rstd (fp32 [rows]) are empty unless need_stats.
-  m.def("layer_norm(Tensor x, Tensor? w, Tensor? b, float eps, bool need_stats) -> (Tensor y, Tensor mean, "
-        "Tensor rstd)");
+  // stats: fp32 [2, rows], mean and 1/std of each row; [2, 0] unless need_stats.
+  m.def("layer_norm(Tensor x, Tensor? w, Tensor? b, float eps, bool need_stats) -> (Tensor y, Tensor stats)");
   // An output that is not needed is empty; dw and db have dtype p_type.
-  m.def("layer_norm_bwd(Tensor dy, Tensor x, Tensor? w, Tensor mean, Tensor rstd, bool need_dx, bool need_dw, "
+  m.def("layer_norm_bwd(Tensor dy, Tensor x, Tensor? w, Tensor stats, bool need_dx, bool need_dw, "
         "bool need_db, ScalarType p_type) -> (Tensor dx, Tensor dw, Tensor db)");
-  m.def("layer_norm_bwd2(Tensor dy, Tensor x, Tensor? w, Tensor mean, Tensor rstd, Tensor? ux, Tensor? uw, "
-        "Tensor? ub) -> (Tensor gdy, Tensor gx, Tensor gw)");
+  m.def("layer_norm_bwd2(Tensor dy, Tensor x, Tensor? w, Tensor stats, Tensor? ux, Tensor? uw, Tensor? ub) "
+        " -> (Tensor gdy, Tensor gx, Tensor gw)");
   // reduction: 0 none, 1 mean, 2 sum; state (bytes) is what the gradients need of the forward
   // (filled only with need_state).
   m.def("linear_ce(Tensor h, Tensor w, Tensor targets, Tensor? mask, int reduction, int ignore_index, bool "
