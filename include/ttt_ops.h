@@ -178,6 +178,11 @@ typedef struct {
 } ttt_lce_bwd2_args;
 int ttt_lce_bwd2(const ttt_lce_bwd2_args* a, void* stream);
 
+/* Copies a [vocab, dim] 16-bit matrix with any row stride into rows that the entry
+ * points above accept: dst_stride >= dim, a multiple of 8, dst 16-byte aligned. */
+int ttt_lce_pad_weight(const void* src, int64_t src_stride, void* dst, int64_t dst_stride, int64_t vocab, int32_t dim,
+                       void* stream);
+
 int64_t ttt_lce_state_bytes(const ttt_lce_problem* pb);
 /* pass: 0 forward, 1 gradient, 2 second gradient. The gradients keep the
  * derivative of the logits of one piece of the vocabulary at a time in 16 bits

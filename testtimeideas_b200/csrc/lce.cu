@@ -267,6 +267,7 @@ __device__ __forceinline__ void copy_rows(const RowArgs& a, const int64_t (&row)
         if (slot[i] >= 0) *reinterpret_cast<uint4*>(a.dst + slot[i] * a.dim_pad + c) = v[i];
     }
   } else {
+#pragma unroll 4
     for (int c = lane; c < a.dim; c += 32) {
       uint16_t v[R];
 #pragma unroll
@@ -686,6 +687,26 @@ __global__ void __launch_bounds__(256) lce_scatter_kernel(const int* slot, const
   }
 }
 
+// Rows of unaligned 16-bit elements into aligned rows; a warp per row, consecutive lanes on
+// consecutive elements, so that both sides move whole sectors.
+__global__ void __launch_bounds__(256) lce_pad_kernel(const uint16_t* src, int64_t src_stride, uint16_t* dst,
+                                                      int64_t dst_stride, int64_t rows, int dim) {
+  const int lane = threadIdx.x & 31;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); r < rows; r += step) {
+    const uint16_t* from = src + r * src_stride;
+    uint16_t* to = dst + r * dst_stride;
+    for (int c0 = lane; c0 < dim; c0 += 256) {
+      uint16_t v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = c0 + u * 32 < dim ? from[c0 + u * 32] : 0;
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (c0 + u * 32 < dim) to[c0 + u * 32] = v[u];
+    }
+  }
+}
+
 // ---------------------------------------------------------------- host side
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
@@ -863,6 +884,18 @@ int zero(void* p, int64_t bytes, cudaStream_t s) { return launched(cudaMemsetAsy
 }  // namespace
 
 extern "C" {
+
+int ttt_lce_pad_weight(const void* src, int64_t src_stride, void* dst, int64_t dst_stride, int64_t vocab, int32_t dim,
+                       void* stream) {
+  if (src == nullptr || dst == nullptr) return TTT_ERR_NULL;
+  if (vocab < 1 || vocab > (1 << 24) || dim < 1 || dim > 65536) return TTT_ERR_SHAPE;
+  if (src_stride < 0 || dst_stride < dim || dst_stride % 8 != 0) return TTT_ERR_STRIDE;
+  if (!aligned(dst, 16)) return TTT_ERR_ALIGN;
+  const int64_t grid = std::min<int64_t>((vocab + 7) / 8, static_cast<int64_t>(device_sms()) * 8);
+  lce_pad_kernel<<<static_cast<unsigned>(grid), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint16_t*>(src), src_stride, static_cast<uint16_t*>(dst), dst_stride, vocab, dim);
+  return launched();
+}
 
 int64_t ttt_lce_state_bytes(const ttt_lce_problem* pb) {
   if (pb == nullptr || check_lce(*pb) != TTT_OK) return 0;

@@ -241,22 +241,27 @@ struct LceWalk {
   }
 };
 
-// Packs 64 columns of this warp's 32 rows into one of its BOXES staging boxes (in
-// turn: `turn` counts them) and stores it at (x, y).
-template <bool BF16, int BOXES>
-TTT_DEV void store_panel(uint8_t* panel, int& turn, const CUtensorMap* map, int lane, int x, int y, const float (&v)[64]) {
+// Packs 64 columns of this warp's 32 rows into a staging box (128-byte swizzle).
+template <bool BF16>
+TTT_DEV void write_box(uint8_t* box, int lane, const float (&v)[64]) {
   uint32_t w[32];
 #pragma unroll
   for (int j = 0; j < 32; ++j) w[j] = pack2<BF16>(v[2 * j], v[2 * j + 1]);
+#pragma unroll
+  for (int ch = 0; ch < 8; ++ch)
+    *reinterpret_cast<uint4*>(box + lane * 128 + ((ch ^ (lane & 7)) << 4)) =
+        make_uint4(w[4 * ch], w[4 * ch + 1], w[4 * ch + 2], w[4 * ch + 3]);
+}
+// ... into one of the warp's BOXES staging boxes (in turn: `turn` counts them), stored at (x, y).
+template <bool BF16, int BOXES>
+TTT_DEV void store_panel(uint8_t* panel, int& turn, const CUtensorMap* map, int lane, int x, int y,
+                         const float (&v)[64]) {
   panel += (turn % BOXES) * 4096;
   ++turn;
   // the box's previous store has left it
   if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BOXES - 1) : "memory");
   __syncwarp();
-#pragma unroll
-  for (int ch = 0; ch < 8; ++ch)
-    *reinterpret_cast<uint4*>(panel + lane * 128 + ((ch ^ (lane & 7)) << 4)) =
-        make_uint4(w[4 * ch], w[4 * ch + 1], w[4 * ch + 2], w[4 * ch + 3]);
+  write_box<BF16>(panel, lane, v);
   fence_async_smem();
   __syncwarp();
   if (lane == 0) {
@@ -586,7 +591,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
         }
       } else {
         const bool boxes = (p.dim & 7) == 0;  // else the rows are not aligned for tensor-map stores
-        const int row = tl.m * C::BM + r;
         const int row0 = tl.m * C::BM + static_cast<int>(rank) * C::ROWS_A + quarter * 32;
 #pragma unroll 1
         for (int q = 0; q < C::HALF / 64; ++q) {
@@ -606,13 +610,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
           if (cq >= p.dim || row0 >= p.cols) continue;
           if (boxes) {
             store_panel<BF16, C::BOXES>(panel, turn, &p.dw_out, lane, cq, row0, v);
-          } else if (row < p.cols) {
-            uint16_t* dst = p.dw + static_cast<int64_t>(row) * p.dim + cq;
-#pragma unroll
-            for (int j = 0; j < 64; j += 2) {
-              const uint32_t w = pack2<BF16>(v[j], v[j + 1]);
-              if (cq + j < p.dim) dst[j] = static_cast<uint16_t>(w);
-              if (cq + j + 1 < p.dim) dst[j + 1] = static_cast<uint16_t>(w >> 16);
+          } else {
+            // through the staging box as well, then row by row: consecutive lanes write
+            // consecutive columns, a pair each where rows start on 4 bytes
+            __syncwarp();
+            write_box<BF16>(panel, lane, v);
+            __syncwarp();
+            auto at = [&](int i, int c) { return panel + i * 128 + (((c >> 3) ^ (i & 7)) << 4) + (c & 7) * 2; };
+            const int rows = min(32, p.cols - row0), cols = min(64, p.dim - cq);
+            uint16_t* dst = p.dw + static_cast<int64_t>(row0) * p.dim + cq;
+            if ((p.dim & 1) == 0) {
+              if (2 * lane < cols) {
+#pragma unroll 8
+                for (int i = 0; i < rows; ++i)
+                  *reinterpret_cast<uint32_t*>(dst + static_cast<int64_t>(i) * p.dim + 2 * lane) =
+                      *reinterpret_cast<const uint32_t*>(at(i, 2 * lane));
+              }
+            } else {
+#pragma unroll 8
+              for (int i = 0; i < rows; ++i) {
+                uint16_t* to = dst + static_cast<int64_t>(i) * p.dim + lane;
+                if (lane < cols) to[0] = *reinterpret_cast<const uint16_t*>(at(i, lane));
+                if (lane + 32 < cols) to[32] = *reinterpret_cast<const uint16_t*>(at(i, lane + 32));
+              }
             }
           }
         }

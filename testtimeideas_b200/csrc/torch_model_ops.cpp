@@ -223,11 +223,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_layer_norm_bwd2(const at::Tens
 at::Tensor weight_rows(const at::Tensor& w) {
   const bool ok = w.stride(1) == 1 && (reinterpret_cast<uintptr_t>(w.data_ptr()) & 15u) == 0 &&
                   (w.size(0) == 1 || (w.stride(0) >= w.size(1) && w.stride(0) % 8 == 0)) &&
-                  (w.size(0) > 1 || w.size(1) % 8 == 0);
+                  (w.size(0) > 1 || w.size(1) % 8 == 0);  // one row: any stride, but whole 16-byte pieces
   if (ok) return w;
   at::Tensor buf = at::empty({w.size(0), (w.size(1) + 7) / 8 * 8}, w.options());
   at::Tensor r = buf.narrow(1, 0, w.size(1));
-  r.copy_(w);
+  if (w.size(1) > 1 && w.stride(1) != 1) {
+    r.copy_(w);
+  } else {
+    check(ttt_lce_pad_weight(w.data_ptr(), w.stride(0), buf.data_ptr(), buf.stride(0), w.size(0),
+                             static_cast<int32_t>(w.size(1)), stream()),
+          "ttt::linear_ce");
+  }
   return r;
 }
 
@@ -529,26 +535,39 @@ at::Tensor op_layer_norm_ad(const at::Tensor& x, const OptTensor& w_, const OptT
   return std::get<0>(raw_layer_norm().call(x, w_, b_, eps, false));
 }
 
+// Weights that the kernels cannot read in place (odd widths) are copied once, in the
+// forward, and the copy (`rows`, else undefined) is kept for both gradients.
+at::Tensor kept_rows(const at::Tensor& w) {
+  if (!w.is_cuda() || w.dim() != 2 || w.numel() == 0 || w.scalar_type() == at::kFloat ||
+      w.key_set().has(c10::DispatchKey::Python))
+    return at::Tensor();  // refused by the operator, or being traced
+  c10::cuda::CUDAGuard guard(w.device());
+  const at::Tensor r = weight_rows(w);
+  return r.is_same(w) ? at::Tensor() : r;
+}
+const at::Tensor& rows_or(const at::Tensor& rows, const at::Tensor& w) { return rows.defined() ? rows : w; }
+
 // (dloss, h, w) -> (dh, dw); `need` has a bit per output.
 struct LinearCEBwdFn : torch::autograd::Function<LinearCEBwdFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& dloss, const at::Tensor& h, const at::Tensor& w,
-                               const at::Tensor& state, int64_t reduction, int64_t need) {
+                               const at::Tensor& state, const OptTensor& rows, int64_t reduction, int64_t need) {
     at::AutoDispatchBelowADInplaceOrView below;
-    ctx->save_for_backward({dloss, h, w, state});
+    ctx->save_for_backward({dloss, h, w, state, defined_or(rows)});
     ctx->set_materialize_grads(false);
     ctx->saved_data["reduction"] = reduction;
-    auto [dh, dw] = raw_linear_ce_bwd().call(dloss, h, w, state, reduction, (need & 1) != 0, (need & 2) != 0);
+    auto [dh, dw] = raw_linear_ce_bwd().call(dloss, h, rows_or(defined_or(rows), w), state, reduction,
+                                             (need & 1) != 0, (need & 2) != 0);
     return {dh, dw};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& up) {
     const variable_list v = ctx->get_saved_variables();
-    variable_list g(6);
+    variable_list g(7);
     if (!up[0].defined() && !up[1].defined()) return g;
     bool need[3];
     for (int i = 0; i < 3; ++i) need[i] = ctx->needs_input_grad(i);
     {
       at::AutoDispatchBelowADInplaceOrView below;
-      std::tie(g[0], g[1], g[2]) = raw_linear_ce_bwd2().call(v[0], v[1], v[2], v[3],
+      std::tie(g[0], g[1], g[2]) = raw_linear_ce_bwd2().call(v[0], v[1], rows_or(v[4], v[2]), v[3],
                                                              ctx->saved_data["reduction"].toInt(), opt(up[0]),
                                                              opt(up[1]), need[0], need[1], need[2]);
       for (int i = 0; i < 3; ++i)
@@ -563,8 +582,9 @@ struct LinearCEFn : torch::autograd::Function<LinearCEFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& targets,
                             const OptTensor& mask, int64_t reduction, int64_t ignore_index) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [loss, state] = raw_linear_ce().call(h, w, targets, mask, reduction, ignore_index, true);
-    ctx->save_for_backward({h, w, state});
+    const at::Tensor rows = kept_rows(w);
+    auto [loss, state] = raw_linear_ce().call(h, rows_or(rows, w), targets, mask, reduction, ignore_index, true);
+    ctx->save_for_backward({h, w, state, rows});
     ctx->set_materialize_grads(false);
     ctx->saved_data["reduction"] = reduction;
     return loss;
@@ -577,10 +597,11 @@ struct LinearCEFn : torch::autograd::Function<LinearCEFn> {
     const int64_t need = (ctx->needs_input_grad(0) ? 1 : 0) | (ctx->needs_input_grad(1) ? 2 : 0);
     variable_list out;
     if (at::GradMode::is_enabled()) {
-      out = LinearCEBwdFn::apply(up[0], v[0], v[1], v[2], reduction, need);
+      out = LinearCEBwdFn::apply(up[0], v[0], v[1], v[2], opt(v[3]), reduction, need);
     } else {
       at::AutoDispatchBelowADInplaceOrView below;
-      auto [dh, dw] = raw_linear_ce_bwd().call(up[0], v[0], v[1], v[2], reduction, (need & 1) != 0, (need & 2) != 0);
+      auto [dh, dw] = raw_linear_ce_bwd().call(up[0], v[0], rows_or(v[3], v[1]), v[2], reduction, (need & 1) != 0,
+                                               (need & 2) != 0);
       out = {dh, dw};
     }
     for (int i = 0; i < 2; ++i)
