@@ -368,8 +368,8 @@ __global__ void __launch_bounds__(256) lce_list_kernel(const RowArgs a) {
   }
 }
 
-// Lists the row coefficients c and gathers uh into slots; block 0 also finds the
-// largest |c| (the second gradient raises it in lce_rho_kernel).
+// Lists the row coefficients and gathers uh into slots; block 0 also finds the
+// largest magnitude (the second gradient raises it in lce_rho_kernel).
 __global__ void __launch_bounds__(256) lce_coef_kernel(const RowArgs a) {
   __shared__ float buf[8];
   asm volatile("griddepcontrol.launch_dependents;");
@@ -377,8 +377,7 @@ __global__ void __launch_bounds__(256) lce_coef_kernel(const RowArgs a) {
   const int n_active = a.st.head->n_active;
   const int end = min((n_active + ttt::kLceBM - 1) / ttt::kLceBM * ttt::kLceBM, a.n_pad);
   auto coef = [&](int s) {
-    if (a.reduction == TTT_LCE_NONE) return a.dloss[a.st.idx[s]] * a.st.mw[s];
-    return *a.dloss * (a.st.mw[s] / a.st.head->denom);
+    return a.reduction == TTT_LCE_NONE ? a.dloss[a.st.idx[s]] * a.st.mw[s] : a.st.mw[s];
   };
   for (int s = (blockIdx.x * 8 + warp) * 2; s < end; s += gridDim.x * 16) {  // end is even
     const int64_t from[2] = {s < n_active ? a.st.idx[s] : -1, s + 1 < n_active ? a.st.idx[s + 1] : -1};
@@ -651,7 +650,7 @@ __global__ void lce_zero_rows_kernel(const int* slot, int64_t n, float* out) {
   if (i < n && slot[i] < 0) out[i] = 0.f;
 }
 
-// dh[i] = sum over the splits (in order) of acc[split][slot_i] / scale, 0 for rows left
+// dh[i] = sum over the splits (in order) of acc[split][slot_i] times the outputs' factor, 0 for rows left
 // out. Four columns a thread at a time, 64 threads a row.
 template <bool BF16>
 __global__ void __launch_bounds__(256) lce_scatter_kernel(const int* slot, const LceCoef coef, const float* acc,
@@ -662,7 +661,7 @@ __global__ void __launch_bounds__(256) lce_scatter_kernel(const int* slot, const
   const int64_t i = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / width;
   if (i >= n) return;
   const int s = slot[i];
-  const float inv = 1.f / coef.scale();
+  const float mul = coef.out();
   uint16_t* dst = dh + i * dim;
 #pragma unroll 4
   for (int c = (threadIdx.x % width) * 4; c < dim; c += width * 4) {
@@ -675,7 +674,7 @@ __global__ void __launch_bounds__(256) lce_scatter_kernel(const int* slot, const
         v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
       }
     }
-    const uint32_t lo = ttt::pack2<BF16>(v.x * inv, v.y * inv), hi = ttt::pack2<BF16>(v.z * inv, v.w * inv);
+    const uint32_t lo = ttt::pack2<BF16>(v.x * mul, v.y * mul), hi = ttt::pack2<BF16>(v.z * mul, v.w * mul);
     if ((dim & 3) == 0) {
       *reinterpret_cast<uint2*>(dst + c) = make_uint2(lo, hi);
     } else {
@@ -764,6 +763,7 @@ struct Pass {
   State st;
   Work w;
   LceCoef coef;
+  const float* upstream;
   int sms;
   bool bf16;
   int* err;
@@ -778,7 +778,9 @@ struct Pass {
     state_layout(p, const_cast<void*>(state), &st);
     work_layout(q, pass, work, &w);
     const bool listed = pass == 2 || (pass == 1 && p.reduction == TTT_LCE_NONE);
-    coef = {st.head, dloss, st.mw, listed ? w.coef : nullptr, w.counters + 1};
+    coef = {st.head, p.reduction == TTT_LCE_NONE ? nullptr : dloss, st.mw, listed ? w.coef : nullptr,
+            listed ? w.counters + 1 : nullptr};
+    upstream = dloss;
   }
   // Row kernels; src is gathered into dst when given.
   RowArgs row_args(const void* src, int64_t stride, uint16_t* dst) const {
@@ -790,7 +792,7 @@ struct Pass {
     a.src = static_cast<const uint16_t*>(src), a.src_stride = stride, a.dst = dst;
     a.wide = q.dim % 8 == 0 && aligned(src, 16) && stride % 8 == 0;
     a.st = st;
-    a.dloss = coef.dloss, a.coef = w.coef, a.counters = w.counters;
+    a.dloss = upstream, a.coef = w.coef, a.counters = w.counters;
     a.err = err, a.err_host = err_host;
     return a;
   }

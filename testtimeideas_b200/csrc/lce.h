@@ -17,26 +17,29 @@ struct LceHead {
   unsigned ticket;  // blocks of the forward's last kernel that are done
 };
 
-// Where the row coefficients c of a gradient come from: listed (per-row upstream
-// gradients, and the second gradient), or formed from the one upstream value.
+// The row coefficients c of a gradient. One upstream value for all rows (mean, sum)
+// multiplies the outputs in fp32, and the stored derivatives carry the mask weights
+// only: with weights of 1 the entry of a target is then p - 1, which 16 bits hold far
+// better than a multiple of 1 / N (1 / 6144 alone is off by 0.2 % in bf16). Per-row
+// upstream values are part of what is stored.
 struct LceCoef {
   const LceHead* head;
-  const float* dloss;        // one value (unused when coef is set)
+  const float* dloss;        // the one upstream value, or null
   const float* mw;           // mask weights by slot
-  const float* coef;         // c by slot, or null
-  const unsigned* max_bits;  // with coef: bits of the largest magnitude to store
+  const float* coef;         // stored coefficients by slot, or null: the mask weights
+  const unsigned* max_bits;  // bits of the largest magnitude to store, or null: the largest weight
 
-  __device__ __forceinline__ float row(int slot) const {
-    return coef != nullptr ? coef[slot] : *dloss * (mw[slot] / head->denom);
-  }
+  __device__ __forceinline__ float row(int slot) const { return coef != nullptr ? coef[slot] : mw[slot]; }
   // Power of two that brings the largest magnitude to store near 2^13 (1 for 0, inf and NaN).
   __device__ __forceinline__ float scale() const {
-    const float big = coef != nullptr ? __uint_as_float(*max_bits) : fabsf(*dloss) * (head->mw_max / head->denom);
+    const float big = max_bits != nullptr ? __uint_as_float(*max_bits) : head->mw_max;
     if (!(big > 0.f && big < INFINITY)) return 1.f;
     int e;
     frexpf(big, &e);  // big < 2^e
     return ldexpf(1.f, max(-100, min(100, 13 - e)));
   }
+  // What the sums over stored derivatives are multiplied by.
+  __device__ __forceinline__ float out() const { return (dloss != nullptr ? *dloss / head->denom : 1.f) / scale(); }
 };
 
 // A tile is formed by a pair of CTAs: 256 rows, 128 in each CTA. Rows are tokens

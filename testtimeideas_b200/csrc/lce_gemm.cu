@@ -449,7 +449,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
     uint8_t* panel = smem + C::OFF_STORE + warp * C::BOXES * C::PANEL;
     int turn = 0;
     const uint32_t free_leader = peer_addr(acc_free, 0);
-    const float mul = C::GRAD ? p.coef.scale() : (KIND == kLceProd ? 1.f / p.coef.scale() : 1.f);
+    const float mul = C::GRAD ? p.coef.scale() : (KIND == kLceProd ? p.coef.out() : 1.f);
     int nth = 0;
     for (int t; (t = walk.template next<kWarp>(g)) >= 0;) {
       const LceTile tl = lce_tile<KIND>(p, sz, t);
