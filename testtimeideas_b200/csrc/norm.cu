@@ -15,7 +15,8 @@
 // All three are bound by memory: 2, 3 and 5 passes over [rows, D]. A row is read
 // once and stays, packed as it came, in the registers of the NT threads that own
 // it: eight elements each up to 2048 (16 to 32 above), so that a thread needs few
-// registers (32 elements a thread took 170 and ran at a quarter of the bandwidth).
+// registers (32 elements a thread took 170 and ran at a quarter of the bandwidth), and
+// about as many threads as the row needs (8 lanes for 64 columns, three warps for 768).
 // Rows come through shared memory up to three ahead of their turn (cp.async), which is
 // what covers the memory's latency.
 // Mean and variance are two sums over registers, and no statistic is a difference
@@ -95,19 +96,20 @@ __device__ __forceinline__ void stay_packed(Pack<T, EPT>& v) {
   for (auto& w : v.w) asm volatile("" : "+r"(w));
 }
 
-// The layout of a row: NT threads, each with K pieces of VEC elements; piece k of
-// thread t starts at column (k * NT + t) * VEC. VEC is 16 bytes of X, or 1 for rows
-// that are not 16-byte aligned. A block holds GROUPS rows at a time.
-template <class X, int NT_, int EPT_, bool WIDE>
+// The layout of a row: NT threads (part of a warp, or whole warps), each with K pieces of
+// VEC elements; piece k of thread t starts at column (k * NT + t) * VEC. VEC is 16 bytes
+// of X, or 4 bytes, or one element, as the rows are aligned. A block holds GROUPS rows at
+// a time. NT is a constant: with a number of threads known only at run time the kernels
+// issue enough more instructions to lose a third of their speed.
+template <class X, int NT_, int EPT_, int VEC_>
 struct Row {
-  static constexpr int NT = NT_, EPT = EPT_;
-  static constexpr int VEC = WIDE ? 16 / static_cast<int>(sizeof(X)) : 1;
-  static constexpr int K = EPT / VEC;
-  static constexpr int THREADS = NT > 256 ? NT : 256, GROUPS = THREADS / NT;
+  static constexpr int NT = NT_, EPT = EPT_, VEC = VEC_, K = EPT / VEC;
+  static constexpr int PIECE = VEC * static_cast<int>(sizeof(X));  // bytes
+  static constexpr int GROUPS = NT > 256 ? 1 : 256 / NT, THREADS = GROUPS * NT;
   // Blocks that an SM holds: 64 registers a thread in the forward, 80 in the gradient of
   // eight 16-bit elements, else 128.
   static constexpr int FWD_PER_SM = 1024 / THREADS;
-  static constexpr int BWD_PER_SM = EPT == 8 && sizeof(X) == 2 ? 3 : 512 / THREADS;
+  static constexpr int BWD_PER_SM = (EPT == 8 && sizeof(X) == 2 ? 768 : 512) / THREADS;
   static constexpr int BWD2_PER_SM = 512 / THREADS;
 
   static __device__ __forceinline__ int column(int k, int t) { return (k * NT + t) * VEC; }
@@ -128,6 +130,17 @@ struct Row {
           v.set_bits(k, *reinterpret_cast<const uint32_t*>(&e));
         else
           v.set_bits(k, *reinterpret_cast<const uint16_t*>(&e));
+      } else if constexpr (PIECE == 4) {
+        static_assert(VEC == 2 && sizeof(X) == 2, "pairs of 16-bit elements");
+        v.set2(k * 2, fill, fill);
+        if (in) {
+          if constexpr (sizeof(T) == 2) {
+            v.w[k] = *reinterpret_cast<const uint32_t*>(row + c);
+          } else {
+            v.w[2 * k] = __float_as_uint(row[c]);
+            v.w[2 * k + 1] = __float_as_uint(row[c + 1]);
+          }
+        }
       } else if (in) {
 #pragma unroll
         for (int q = 0; q < WORDS / 4; ++q) {
@@ -153,6 +166,8 @@ struct Row {
           reinterpret_cast<uint32_t*>(row)[c] = v.bits(k);
         else
           reinterpret_cast<uint16_t*>(row)[c] = static_cast<uint16_t>(v.bits(k));
+      } else if constexpr (PIECE == 4) {
+        *reinterpret_cast<uint32_t*>(row + c) = v.w[k];
       } else {
 #pragma unroll
         for (int q = 0; q < WORDS / 4; ++q) {
@@ -168,15 +183,21 @@ struct Row {
 // several warps go through shared memory and a barrier of their own; `phase`
 // alternates between two halves of the buffer so that one barrier is enough.
 constexpr int kMaxSums = 6;
+// The block's row of this thread's first lane: where several rows share a warp, the warp
+// goes on together for as long as its first row exists.
+template <class R>
+__device__ __forceinline__ int lead_row() {
+  return R::NT < 32 ? static_cast<int>(threadIdx.x & ~31u) / R::NT : static_cast<int>(threadIdx.x) / R::NT;
+}
 template <class R>
 struct Sums {
-  static constexpr int W = R::NT / 32;
-  float red[R::GROUPS][2][kMaxSums][W];
+  static constexpr int W = R::NT > 32 ? R::NT / 32 : 1, ROWS = R::NT > 32 ? R::GROUPS : 1;
+  float red[ROWS][2][kMaxSums][W];
 };
 template <class R, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], Sums<R>& sums, int& phase) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = (R::NT < 32 ? R::NT : 32) / 2; o > 0; o >>= 1) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   }
@@ -211,7 +232,7 @@ template <class X, class R, int T, int PER_SM>
 struct Ring {
   static constexpr int ROW = R::K * R::THREADS * 16;  // bytes of one tensor's rows of a block
   static constexpr int FIT = (200 << 10) / (PER_SM * T * ROW);
-  static constexpr int S = R::VEC == 1 || FIT < 2 ? 0 : (FIT < 4 ? FIT : 4);
+  static constexpr int S = R::PIECE < 16 || FIT < 2 ? 0 : (FIT < 4 ? FIT : 4);
   static constexpr int BYTES = S * T * ROW;
   const X* src[T];
   int64_t stride[T];
@@ -242,12 +263,13 @@ struct Ring {
   __device__ __forceinline__ void wait() const {
     asm volatile("cp.async.wait_group %0;" ::"n"(S > 0 ? S - 1 : 0) : "memory");
   }
-  __device__ __forceinline__ void read(int st, int i, Pack<X, R::EPT>& v) const {
+  // Tensor i of the row in stage `st`; zeros outside it, and where there is no such row.
+  __device__ __forceinline__ void read(int st, int i, bool exists, Pack<X, R::EPT>& v) const {
     constexpr int WORDS = 4;
 #pragma unroll
     for (int k = 0; k < R::K; ++k) {
       uint32_t* w = v.w + k * WORDS;
-      if (src[i] != nullptr && R::column(k, t) < D) {
+      if (exists && src[i] != nullptr && R::column(k, t) < D) {
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                      : "r"(base + (st * T + i) * ROW + k * R::THREADS * 16)
@@ -298,7 +320,7 @@ __global__ void __launch_bounds__(R::THREADS, R::FWD_PER_SM) norm_fwd_kernel(con
   const float inv = 1.f / static_cast<float>(a.D);
   const int64_t step = static_cast<int64_t>(gridDim.x) * R::GROUPS;
   int64_t row = static_cast<int64_t>(blockIdx.x) * R::GROUPS + threadIdx.x / R::NT;
-  if (row >= a.rows) return;  // whole groups, which have their own barriers
+  int64_t lead = static_cast<int64_t>(blockIdx.x) * R::GROUPS + lead_row<R>();
   G g = make_ring<G>(smem, t, a.D);
   g.src[0] = a.x;
   g.stride[0] = a.x_stride;
@@ -307,21 +329,22 @@ __global__ void __launch_bounds__(R::THREADS, R::FWD_PER_SM) norm_fwd_kernel(con
 #pragma unroll
     for (int i = 0; i < G::S - 1; ++i) g.fetch(row + i * step, a.rows, i);
   } else {
-    R::load(a.x + row * a.x_stride, t, a.D, xn);
+    R::load(row < a.rows ? a.x + row * a.x_stride : nullptr, t, a.D, xn);
   }
   Pack<P, EPT> w, b;
   R::load(a.w, t, a.D, w, 1.f);
   R::load(a.b, t, a.D, b, 0.f);
-  for (int st = 0; row < a.rows; row += step) {
+  for (int st = 0; (R::NT < 32 ? lead : row) < a.rows; row += step, lead += step) {
+    const bool exists = R::NT >= 32 || row < a.rows;
     Pack<X, EPT> x;
     if constexpr (G::S > 0) {
       g.fetch(row + (G::S - 1) * step, a.rows, (st + G::S - 1) % G::S);
       g.wait();
-      g.read(st, 0, x);
+      g.read(st, 0, exists, x);
       st = (st + 1) % G::S;
     } else {
       x = xn;
-      if (row + step < a.rows) R::load(a.x + (row + step) * a.x_stride, t, a.D, xn);
+      R::load(row + step < a.rows ? a.x + (row + step) * a.x_stride : nullptr, t, a.D, xn);
     }
     float s[1] = {0.f};
 #pragma unroll
@@ -339,10 +362,12 @@ __global__ void __launch_bounds__(R::THREADS, R::FWD_PER_SM) norm_fwd_kernel(con
 #pragma unroll
     for (int i = 0; i < EPT; i += 2)
       x.set2(i, (x.at(i) - mu) * r * w.at(i) + b.at(i), (x.at(i + 1) - mu) * r * w.at(i + 1) + b.at(i + 1));
-    R::store(a.y + row * a.D, t, a.D, x);
-    if (t == 0 && a.mean != nullptr) {
-      a.mean[row] = mu;
-      a.rstd[row] = r;
+    if (exists) {
+      R::store(a.y + row * a.D, t, a.D, x);
+      if (t == 0 && a.mean != nullptr) {
+        a.mean[row] = mu;
+        a.rstd[row] = r;
+      }
     }
   }
 }
@@ -370,7 +395,7 @@ __device__ __forceinline__ void write_part(float* part, int which, int D, const 
     __syncthreads();
     for (int c = threadIdx.x; c < D; c += R::THREADS) {
       float s = 0.f;
-#pragma unroll
+#pragma unroll 8
       for (int gi = 0; gi < R::GROUPS; ++gi) s += cols[gi * D + c];
       dst[c] = s;
     }
@@ -395,24 +420,29 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD_PER_SM) norm_bwd_kernel(con
   R::load(a.w, t, a.D, w, 1.f);
   const int64_t step = static_cast<int64_t>(gridDim.x) * R::GROUPS;
   int64_t row = static_cast<int64_t>(blockIdx.x) * R::GROUPS + threadIdx.x / R::NT;
+  int64_t lead = static_cast<int64_t>(blockIdx.x) * R::GROUPS + lead_row<R>();
   G ring = make_ring<G>(smem, t, a.D);
   ring.src[0] = a.x, ring.stride[0] = a.x_stride;
   ring.src[1] = a.dy, ring.stride[1] = a.dy_stride;
   Pack<X, EPT> xn, dn;  // S = 0: the next row
-  float mun[2], rn[2];  // statistics of the next two rows
+  float mun[2] = {0.f, 0.f}, rn[2] = {0.f, 0.f};  // statistics of the next two rows
   auto fetch_stats = [&](int64_t at, int i) {
     if (at < a.rows) mun[i] = a.mean[at], rn[i] = a.rstd[at];
+  };
+  auto fetch_rows = [&](int64_t at) {
+    R::load(at < a.rows ? a.x + at * a.x_stride : nullptr, t, a.D, xn);
+    R::load(at < a.rows ? a.dy + at * a.dy_stride : nullptr, t, a.D, dn);
   };
   fetch_stats(row, 0);
   fetch_stats(row + step, 1);
   if constexpr (G::S > 0) {
 #pragma unroll
     for (int i = 0; i < G::S - 1; ++i) ring.fetch(row + i * step, a.rows, i);
-  } else if (row < a.rows) {
-    R::load(a.x + row * a.x_stride, t, a.D, xn);
-    R::load(a.dy + row * a.dy_stride, t, a.D, dn);
+  } else {
+    fetch_rows(row);
   }
-  for (int st = 0; row < a.rows; row += step) {
+  for (int st = 0; (R::NT < 32 ? lead : row) < a.rows; row += step, lead += step) {
+    const bool exists = R::NT >= 32 || row < a.rows;
     Pack<X, EPT> x, dy;
     const float mu = mun[0], r = rn[0];
     mun[0] = mun[1], rn[0] = rn[1];
@@ -420,20 +450,17 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD_PER_SM) norm_bwd_kernel(con
     if constexpr (G::S > 0) {
       ring.fetch(row + (G::S - 1) * step, a.rows, (st + G::S - 1) % G::S);
       ring.wait();
-      ring.read(st, 0, x);
-      ring.read(st, 1, dy);
+      ring.read(st, 0, exists, x);
+      ring.read(st, 1, exists, dy);
       st = (st + 1) % G::S;
     } else {
       x = xn, dy = dn;
-      if (row + step < a.rows) {
-        R::load(a.x + (row + step) * a.x_stride, t, a.D, xn);
-        R::load(a.dy + (row + step) * a.dy_stride, t, a.D, dn);
-      }
+      fetch_rows(row + step);
     }
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-      // dy is zero outside the row, so nothing else has to be
+      // dy is zero outside the row (and past the last row), so nothing else has to be
       const float xh = (x.at(i) - mu) * r, d = dy.at(i), g = d * w.at(i);
       aw[i] += d * xh;
       ab[i] += d;
@@ -444,7 +471,7 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD_PER_SM) norm_bwd_kernel(con
     stay_packed(x);
     stay_packed(dy);
     stay_packed(w);
-    if (a.dx != nullptr) {
+    if (a.dx != nullptr && exists) {
       const float mg = s[0] * inv, ma = s[1] * inv;
 #pragma unroll
       for (int i = 0; i < EPT; i += 2)
@@ -477,6 +504,7 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD2_PER_SM) norm_bwd2_kernel(c
   R::load(a.ub, t, a.D, ub);
   const int64_t step = static_cast<int64_t>(gridDim.x) * R::GROUPS;
   int64_t row = static_cast<int64_t>(blockIdx.x) * R::GROUPS + threadIdx.x / R::NT;
+  int64_t lead = static_cast<int64_t>(blockIdx.x) * R::GROUPS + lead_row<R>();
   G ring = make_ring<G>(smem, t, a.D);
   ring.src[0] = a.x, ring.stride[0] = a.x_stride;
   ring.src[1] = a.dy, ring.stride[1] = a.dy_stride;
@@ -487,21 +515,22 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD2_PER_SM) norm_bwd2_kernel(c
 #pragma unroll
     for (int i = 0; i < G::S - 1; ++i) ring.fetch(row + i * step, a.rows, i);
   }
-  for (int st = 0; row < a.rows; row += step) {
+  for (int st = 0; (R::NT < 32 ? lead : row) < a.rows; row += step, lead += step) {
+    const bool exists = R::NT >= 32 || row < a.rows;
     const float mu = mun, r = rn;
     if (row + step < a.rows) mun = a.mean[row + step], rn = a.rstd[row + step];
     Pack<X, EPT> x, dy, u;
     if constexpr (G::S > 0) {
       ring.fetch(row + (G::S - 1) * step, a.rows, (st + G::S - 1) % G::S);
       ring.wait();
-      ring.read(st, 0, x);
-      ring.read(st, 1, dy);
-      ring.read(st, 2, u);
+      ring.read(st, 0, exists, x);
+      ring.read(st, 1, exists, dy);
+      ring.read(st, 2, exists, u);
       st = (st + 1) % G::S;
     } else {
-      R::load(a.x + row * a.x_stride, t, a.D, x);
-      R::load(a.dy + row * a.dy_stride, t, a.D, dy);
-      R::load(a.ux == nullptr ? nullptr : a.ux + row * a.ux_stride, t, a.D, u);
+      R::load(exists ? a.x + row * a.x_stride : nullptr, t, a.D, x);
+      R::load(exists ? a.dy + row * a.dy_stride : nullptr, t, a.D, dy);
+      R::load(exists && a.ux != nullptr ? a.ux + row * a.ux_stride : nullptr, t, a.D, u);
     }
     float s[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // g, u, g xh, u xh, h, h xh
 #pragma unroll
@@ -553,8 +582,10 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD2_PER_SM) norm_bwd2_kernel(c
       dy.set2(i, gd[0], gd[1]);
       x.set2(i, gx[0], gx[1]);
     }
-    R::store(a.gdy + row * a.D, t, a.D, dy);
-    R::store(a.gx + row * a.D, t, a.D, x);
+    if (exists) {
+      R::store(a.gdy + row * a.D, t, a.D, dy);
+      R::store(a.gx + row * a.D, t, a.D, x);
+    }
   }
   if (a.want_dw) write_part<R>(a.part, 0, a.D, agw, cols);
 }
@@ -593,19 +624,26 @@ int sm_count() {
   return n < 1 ? 1 : n;
 }
 
-// Threads of a row: 32 to 256 with eight elements each, then 256 or 512 with 16, 512 with 32.
-int row_threads(int D) {
+// Threads of a row: eight elements each up to 2048 columns, then 16 and 32. Aligned rows
+// have 8 to 256 threads with steps of a half between 64 and 256, others powers of two
+// from a warp up (which keeps the number of kernels down).
+int row_threads(int D, bool wide) {
+  if (D > 4096) return 512;
+  if (D > 2048) return 256;
+  if (wide)
+    for (const int nt : {8, 16, 32, 64, 96, 128, 192})
+      if (nt * 8 >= D) return nt;
   int nt = 32;
-  while (nt < 256 && nt * 8 < D) nt *= 2;
-  return D <= 4096 ? nt : 512;
+  while (nt * 8 < D) nt *= 2;
+  return nt;
 }
 
 // Blocks of the gradient kernels: all that fit on the SMs at once, or as many as there are rows for.
-int grad_blocks(const ttt_norm_problem& pb, bool second, int sms) {
-  const int nt = row_threads(pb.dim), threads = nt > 256 ? nt : 256;
-  const int64_t groups = threads / nt, need = (pb.rows + groups - 1) / groups;
-  const int per_sm = pb.dim <= 2048 && pb.dtype != TTT_F32 && !second ? 3 : 512 / threads;
-  return static_cast<int>(std::min<int64_t>(std::max<int64_t>(need, 1), static_cast<int64_t>(sms) * per_sm));
+int grad_blocks(const ttt_norm_problem& pb, bool second, bool wide, int sms) {
+  const int nt = row_threads(pb.dim, wide), groups = nt > 256 ? 1 : 256 / nt, threads = groups * nt;
+  const int64_t res = pb.dim <= 2048 && pb.dtype != TTT_F32 && !second ? 768 : 512;
+  return static_cast<int>(
+      std::min<int64_t>(std::max<int64_t>((pb.rows + groups - 1) / groups, 1), sms * (res / threads)));
 }
 
 int check_norm(const ttt_norm_problem& pb) {
@@ -637,15 +675,31 @@ cudaError_t launch_rows(const NormArgs<X, P>& a, Pass pass, int blocks, int sms,
   return launch(norm_bwd2_kernel<X, P, R>, blocks, Bwd2Ring<X, R>::BYTES + cols);
 }
 
-template <class X, class P, bool WIDE>
+template <class X, class P, int VEC>
 cudaError_t launch_width(const NormArgs<X, P>& a, Pass pass, int blocks, int sms, cudaStream_t s) {
-  if (a.D <= 256) return launch_rows<X, P, Row<X, 32, 8, WIDE>>(a, pass, blocks, sms, s);
-  if (a.D <= 512) return launch_rows<X, P, Row<X, 64, 8, WIDE>>(a, pass, blocks, sms, s);
-  if (a.D <= 1024) return launch_rows<X, P, Row<X, 128, 8, WIDE>>(a, pass, blocks, sms, s);
-  if (a.D <= 2048) return launch_rows<X, P, Row<X, 256, 8, WIDE>>(a, pass, blocks, sms, s);
-  if (a.D <= 4096) return launch_rows<X, P, Row<X, 256, 16, WIDE>>(a, pass, blocks, sms, s);
-  if (a.D <= 8192) return launch_rows<X, P, Row<X, 512, 16, WIDE>>(a, pass, blocks, sms, s);
-  return launch_rows<X, P, Row<X, 512, 32, WIDE>>(a, pass, blocks, sms, s);
+  constexpr bool WIDE = VEC * sizeof(X) == 16;
+  if (a.D > 8192) return launch_rows<X, P, Row<X, 512, 32, VEC>>(a, pass, blocks, sms, s);
+  if (a.D > 4096) return launch_rows<X, P, Row<X, 512, 16, VEC>>(a, pass, blocks, sms, s);
+  if (a.D > 2048) return launch_rows<X, P, Row<X, 256, 16, VEC>>(a, pass, blocks, sms, s);
+  switch (row_threads(a.D, WIDE)) {
+    case 8:
+      if constexpr (WIDE) return launch_rows<X, P, Row<X, 8, 8, VEC>>(a, pass, blocks, sms, s);
+      break;
+    case 16:
+      if constexpr (WIDE) return launch_rows<X, P, Row<X, 16, 8, VEC>>(a, pass, blocks, sms, s);
+      break;
+    case 96:
+      if constexpr (WIDE) return launch_rows<X, P, Row<X, 96, 8, VEC>>(a, pass, blocks, sms, s);
+      break;
+    case 192:
+      if constexpr (WIDE) return launch_rows<X, P, Row<X, 192, 8, VEC>>(a, pass, blocks, sms, s);
+      break;
+    case 32: return launch_rows<X, P, Row<X, 32, 8, VEC>>(a, pass, blocks, sms, s);
+    case 64: return launch_rows<X, P, Row<X, 64, 8, VEC>>(a, pass, blocks, sms, s);
+    case 128: return launch_rows<X, P, Row<X, 128, 8, VEC>>(a, pass, blocks, sms, s);
+    default: return launch_rows<X, P, Row<X, 256, 8, VEC>>(a, pass, blocks, sms, s);
+  }
+  return cudaErrorInvalidValue;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -659,21 +713,30 @@ int run_norm(NormArgs<X, P> a, const ttt_norm_problem& pb, Pass pass, void* dw, 
   a.want_dw = dw != nullptr;
   a.want_db = db != nullptr;
   const int sms = sm_count();
-  const int blocks = pass == kFwd ? 0 : grad_blocks(pb, pass == kBwd2, sms);
+  // 16-byte pieces need every row and every parameter vector on a 16-byte boundary, 4-byte
+  // pieces the rows on a 4-byte one
+  constexpr int V = 16 / static_cast<int>(sizeof(X)), H = 4 / static_cast<int>(sizeof(X));
+  const void* rows_at[] = {a.x, a.dy, a.ux, a.y, a.dx, a.gx, a.gdy};
+  const void* params_at[] = {a.w, a.b, a.uw, a.ub};
+  uintptr_t row_bits = 0, param_bits = 0;
+  for (const void* p : rows_at) row_bits |= reinterpret_cast<uintptr_t>(p);
+  for (const void* p : params_at) param_bits |= reinterpret_cast<uintptr_t>(p);
+  const int64_t steps = pb.dim | a.x_stride | a.dy_stride | a.ux_stride;
+  const bool wide = ((row_bits | param_bits) & 15) == 0 && steps % V == 0;
+  const int blocks = pass == kFwd ? 0 : grad_blocks(pb, pass == kBwd2, wide, sms);
   if (a.want_dw || a.want_db) {
     if (work == nullptr || !aligned16(work) || work_bytes < static_cast<int64_t>(blocks) * 2 * pb.dim * 4)
       return TTT_ERR_SCRATCH;
     a.part = static_cast<float*>(work);
   }
   if (pb.rows > 0 || pass != kFwd) {
-    // 16-byte pieces need every row and every parameter vector on a 16-byte boundary
-    constexpr int V = 16 / static_cast<int>(sizeof(X));
-    bool wide = pb.dim % V == 0;
-    const void* rows_at[] = {a.x, a.dy, a.ux, a.w, a.b, a.uw, a.ub, a.y, a.dx, a.gx, a.gdy};
-    for (const void* p : rows_at) wide = wide && aligned16(p);
-    wide = wide && a.x_stride % V == 0 && a.dy_stride % V == 0 && a.ux_stride % V == 0;
-    const cudaError_t e = wide ? launch_width<X, P, true>(a, pass, blocks, sms, s)
-                               : launch_width<X, P, false>(a, pass, blocks, sms, s);
+    cudaError_t e;
+    if (wide)
+      e = launch_width<X, P, V>(a, pass, blocks, sms, s);
+    else if (H == 2 && (row_bits & 3) == 0 && steps % H == 0)
+      e = launch_width<X, P, H>(a, pass, blocks, sms, s);
+    else
+      e = launch_width<X, P, 1>(a, pass, blocks, sms, s);
     if (e != cudaSuccess) return TTT_ERR_LAUNCH;
   }
   if (a.want_dw || a.want_db) {
@@ -709,7 +772,9 @@ extern "C" {
 
 int64_t ttt_norm_work_bytes(const ttt_norm_problem* pb) {
   if (pb == nullptr || check_norm(*pb) != TTT_OK) return 0;
-  return static_cast<int64_t>(grad_blocks(*pb, false, sm_count())) * 2 * pb->dim * 4;
+  const int sms = sm_count();  // the gradient's blocks, in whichever layout has more of them
+  return static_cast<int64_t>(std::max(grad_blocks(*pb, false, true, sms), grad_blocks(*pb, false, false, sms))) * 2 *
+         pb->dim * 4;
 }
 
 int ttt_norm_fwd(const ttt_norm_fwd_args* g, void* stream) {
