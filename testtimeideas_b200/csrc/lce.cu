@@ -221,7 +221,7 @@ __device__ __forceinline__ float block_max(float v, float* buf) {
 
 struct RowArgs {
   int64_t n, vocab, ignore_index;
-  int n_pad, dim, dim_pad, mask_kind, reduction;
+  int n_pad, dim, dim_pad, mask_kind, reduction, list_rows;
   const int64_t* targets;
   const void* mask;
   const uint16_t* src;  // h (forward) or uh
@@ -249,14 +249,15 @@ __device__ __forceinline__ int row_kind(const RowArgs& a, int64_t i, float m) {
   return t >= 0 && t < a.vocab ? 1 : -1;
 }
 
-// Copies up to R source rows (row < 0: zeros) into slots (slot < 0: none); one warp,
-// the rows' loads in flight together.
+// Copies up to R source rows (row < 0: zeros) into slots (slot < 0: none), the rows'
+// loads in flight together; by `count` threads, of which this is number `me`.
 template <int R>
-__device__ __forceinline__ void copy_rows(const RowArgs& a, const int64_t (&row)[R], const int64_t (&slot)[R], int lane) {
+__device__ __forceinline__ void copy_rows(const RowArgs& a, const int64_t (&row)[R], const int64_t (&slot)[R], int me,
+                                          int count) {
   if (a.src == nullptr) return;
   if (a.wide) {
 #pragma unroll 2
-    for (int c = lane * 8; c < a.dim; c += 256) {
+    for (int c = me * 8; c < a.dim; c += count * 8) {
       uint4 v[R];
 #pragma unroll
       for (int i = 0; i < R; ++i)
@@ -268,7 +269,7 @@ __device__ __forceinline__ void copy_rows(const RowArgs& a, const int64_t (&row)
     }
   } else {
 #pragma unroll 4
-    for (int c = lane; c < a.dim; c += 32) {
+    for (int c = me; c < a.dim; c += count) {
       uint16_t v[R];
 #pragma unroll
       for (int i = 0; i < R; ++i) v[i] = slot[i] < 0 || row[i] < 0 ? 0 : a.src[row[i] * a.src_stride + c];
@@ -279,25 +280,38 @@ __device__ __forceinline__ void copy_rows(const RowArgs& a, const int64_t (&row)
   }
 }
 
-// Lists the participating rows and gathers h. Block b owns rows [32 b, 32 b + 32);
-// it counts the participating rows before them itself (n / 2 reads of 8 to 12 bytes
-// on average, from L2), so that one launch does without a scan across blocks. The
-// last block also knows the totals and clears the slots up to the next whole tile.
-constexpr int kListRows = 32;
+// Clears row slot `s`; one warp.
+__device__ __forceinline__ void clear_slot(const RowArgs& a, int64_t s, int lane) {
+  for (int c = lane * 8; c < a.dim_pad; c += 256)
+    *reinterpret_cast<uint4*>(a.dst + s * a.dim_pad + c) = make_uint4(0, 0, 0, 0);
+  if (lane == 0) a.st.idx[s] = -1, a.st.tgt[s] = -1, a.st.mw[s] = 0.f, a.st.lse2[s] = INFINITY;
+}
+
+// Lists the participating rows and gathers h. Block b owns a range of a.list_rows rows,
+// 32 at a time; it counts the participating rows before the range itself (n / 2 reads of
+// 8 to 12 bytes on average, from L2, by at most 512 blocks), so that one launch does
+// without a scan across blocks. The last of them also knows the totals and clears the
+// slots up to the next whole tile; the slots past the last row, which no row can take,
+// have blocks of their own.
 __global__ void __launch_bounds__(256) lce_list_kernel(const RowArgs a) {
   __shared__ float buf[8];
   __shared__ int cnt[8];
-  __shared__ int slots[kListRows];
+  __shared__ int slots[32];
   __shared__ int total;
   asm volatile("griddepcontrol.launch_dependents;");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kListRows;
-  const bool last = blockIdx.x == gridDim.x - 1;
-  // participating rows before row0, and the mask's sum and largest magnitude over them
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * a.list_rows;
+  if (first >= a.n) {
+    const int64_t s0 = a.n + (blockIdx.x - (a.n + a.list_rows - 1) / a.list_rows) * 32;
+    for (int64_t s = s0 + warp; s < s0 + 32 && s < a.n_pad; s += 8) clear_slot(a, s, lane);
+    return;
+  }
+  const int64_t past = min(first + a.list_rows, a.n);
+  // participating rows before the range, and the mask's sum and largest magnitude over them
   int before = 0;
   float msum = 0.f, mmax = 0.f;
 #pragma unroll 8
-  for (int64_t i = threadIdx.x; i < row0; i += 256) {
+  for (int64_t i = threadIdx.x; i < first; i += 256) {
     const float m = mask_weight(a, i);
     const bool in = row_kind(a, i, m) > 0;
     before += in;
@@ -308,53 +322,56 @@ __global__ void __launch_bounds__(256) lce_list_kernel(const RowArgs a) {
   for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
   if (lane == 0) cnt[warp] = before;
   __syncthreads();
-  if (warp == 0) {
-    int base = 0;
-    for (int i = 0; i < 8; ++i) base += cnt[i];
-    const int64_t i = row0 + lane;
-    float m = 0.f;
-    int kind = 0;
-    if (i < a.n) {
-      m = mask_weight(a, i);
-      kind = row_kind(a, i, m);
-      if (kind < 0) ttt::report_error(a.err, a.err_host, TTT_ERR_WORD_TARGET | (static_cast<int>(i) & 0xffffff));
-      msum += m;
-      mmax = kind > 0 ? fmaxf(mmax, fabsf(m)) : mmax;
-    }
-    const unsigned bits = __ballot_sync(0xffffffffu, kind > 0);
-    const int s = kind > 0 ? base + __popc(bits & ((1u << lane) - 1)) : -1;
-    base += __popc(bits);
-    slots[lane] = s;
-    if (i < a.n) {
-      a.st.slot[i] = s;
-      if (s >= 0) {
-        a.st.idx[s] = static_cast<int>(i);
-        a.st.tgt[s] = static_cast<int>(a.targets[i]);
-        a.st.mw[s] = m;
-      } else if (a.reduction == TTT_LCE_NONE) {
-        a.loss[i] = 0.f;
+  int base = 0;
+  for (int i = 0; i < 8; ++i) base += cnt[i];
+  for (int64_t row0 = first; row0 < past; row0 += 32) {
+    if (warp == 0) {
+      const int64_t i = row0 + lane;
+      float m = 0.f;
+      int kind = 0;
+      if (i < past) {
+        m = mask_weight(a, i);
+        kind = row_kind(a, i, m);
+        if (kind < 0) ttt::report_error(a.err, a.err_host, TTT_ERR_WORD_TARGET | (static_cast<int>(i) & 0xffffff));
+        msum += m;
+        mmax = kind > 0 ? fmaxf(mmax, fabsf(m)) : mmax;
       }
+      const unsigned bits = __ballot_sync(0xffffffffu, kind > 0);
+      const int s = kind > 0 ? base + __popc(bits & ((1u << lane) - 1)) : -1;
+      base += __popc(bits);
+      slots[lane] = s;
+      if (i < past) {
+        a.st.slot[i] = s;
+        if (s >= 0) {
+          a.st.idx[s] = static_cast<int>(i);
+          a.st.tgt[s] = static_cast<int>(a.targets[i]);
+          a.st.mw[s] = m;
+        } else if (a.reduction == TTT_LCE_NONE) {
+          a.loss[i] = 0.f;
+        }
+      }
+      if (lane == 0) total = base;
     }
-    if (lane == 0) total = base;
-  }
-  __syncthreads();
-  {
-    int64_t from[4], to[4];
+    __syncthreads();
+    // aligned rows four to a warp, others (one element a load) four to the block
+    for (int j = a.wide ? warp : 0; j < (a.wide ? warp + 1 : 8); ++j) {
+      int64_t from[4], to[4];
+      bool any = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      from[i] = row0 + warp * 4 + i;
-      to[i] = slots[warp * 4 + i];
+      for (int i = 0; i < 4; ++i) {
+        const int at = a.wide ? j + 8 * i : j * 4 + i;
+        from[i] = row0 + at;
+        to[i] = slots[at];
+        any = any || to[i] >= 0;
+      }
+      if (any) copy_rows<4>(a, from, to, a.wide ? lane : threadIdx.x, a.wide ? 32 : 256);
     }
-    copy_rows<4>(a, from, to, lane);
+    __syncthreads();
   }
-  if (!last) return;
+  if (past < a.n) return;
   const int n_active = total;
-  const int end = min((n_active + ttt::kLceBM - 1) / ttt::kLceBM * ttt::kLceBM, a.n_pad);
-  for (int s = n_active + warp; s < end; s += 8) {
-    const int64_t from[1] = {-1}, to[1] = {s};
-    copy_rows<1>(a, from, to, lane);
-    if (lane == 0) a.st.idx[s] = -1, a.st.tgt[s] = -1, a.st.mw[s] = 0.f, a.st.lse2[s] = INFINITY;
-  }
+  const int64_t end = min(static_cast<int64_t>((n_active + ttt::kLceBM - 1) / ttt::kLceBM * ttt::kLceBM), a.n);
+  for (int64_t s = n_active + warp; s < end; s += 8) clear_slot(a, s, lane);
   msum = block_sum(msum, buf);
   mmax = block_max(mmax, buf);
   if (threadIdx.x == 0) {
@@ -382,7 +399,7 @@ __global__ void __launch_bounds__(256) lce_coef_kernel(const RowArgs a) {
   for (int s = (blockIdx.x * 8 + warp) * 2; s < end; s += gridDim.x * 16) {  // end is even
     const int64_t from[2] = {s < n_active ? a.st.idx[s] : -1, s + 1 < n_active ? a.st.idx[s + 1] : -1};
     const int64_t to[2] = {s, s + 1};
-    copy_rows<2>(a, from, to, lane);
+    copy_rows<2>(a, from, to, lane, 32);
     if (lane < 2) a.coef[s + lane] = s + lane < n_active ? coef(s + lane) : 0.f;
   }
   if (blockIdx.x != 0) return;
@@ -418,9 +435,9 @@ __device__ __forceinline__ void total_rows(float v, float* sums, unsigned* ticke
   if (threadIdx.x == 0) *out = t / denom;
 }
 
-// Merges the half tiles' (max, sum) of a row: 32 rows and 16 shares of the tiles per
+// Merges the half tiles' (max, sum) of a row: 32 rows and 32 shares of the tiles per
 // block, shares in order. Writes lse2 and the row's weighted loss.
-constexpr int kShares = 16;
+constexpr int kShares = 32;
 __global__ void __launch_bounds__(32 * kShares) lce_lse_kernel(const State st, const float2* part, const float* ztgt,
                                                                int parts, int n_pad, int reduction, float* sums,
                                                                float* loss) {
@@ -651,7 +668,7 @@ __global__ void lce_zero_rows_kernel(const int* slot, int64_t n, float* out) {
 }
 
 // dh[i] = sum over the splits (in order) of acc[split][slot_i] times the outputs' factor, 0 for rows left
-// out. Four columns a thread at a time, 64 threads a row.
+// out. Four columns a thread at a time, `width` threads a row.
 template <bool BF16>
 __global__ void __launch_bounds__(256) lce_scatter_kernel(const int* slot, const LceCoef coef, const float* acc,
                                                           int splits, int64_t n, int n_pad, int dim, int dim_pad,
@@ -872,8 +889,8 @@ int run_pieces(const Pass& p, const Weight& w, const Weight* uw, bool second, bo
     TTT_TRY(p.run(t, ttt::kLceProd));
   }
   if (outh != nullptr) {
-    int width = 8;  // threads of a row
-    while (width < 64 && width * 4 < q.dim) width *= 2;
+    int width = 8;  // threads of a row: with few rows a whole block
+    while (width < (q.n < 512 ? 256 : 64) && width * 4 < q.dim) width *= 2;
     TTT_TRY(launch_early(p.bf16 ? lce_scatter_kernel<true> : lce_scatter_kernel<false>,
                          (q.n + 256 / width - 1) / (256 / width), 256, p.s, p.st.slot, p.coef, p.w.acc, q.splits, q.n,
                          static_cast<int>(q.n_pad), q.dim, q.dim_pad, width, outh));
@@ -938,7 +955,10 @@ int ttt_lce_fwd(const ttt_lce_fwd_args* a, void* stream) {
     return launch_early(lce_lse_kernel, 1, 32 * kShares, p.s, p.st, p.w.part, p.w.ztgt, blocks, static_cast<int>(p.q.n_pad),
                         pb.reduction, p.w.sums, a->loss);
   }
-  lce_list_kernel<<<static_cast<unsigned>((pb.n + kListRows - 1) / kListRows), 256, 0, p.s>>>(r);
+  r.list_rows = static_cast<int>(std::max<int64_t>(32, up((pb.n + 511) / 512, 32)));
+  const int64_t row_blocks = (pb.n + r.list_rows - 1) / r.list_rows;
+  const int64_t pad_blocks = (p.q.n_pad - pb.n + 31) / 32;
+  lce_list_kernel<<<static_cast<unsigned>(row_blocks + pad_blocks), 256, 0, p.s>>>(r);
   TTT_TRY(launched());
   ttt::LceGemm g = p.gemm(0, pb.vocab);
   if (!p.map_rows(&g.a[0], p.st.hc) || !p.map_weight(&g.b[0], w, g, ttt::kLceBN)) return TTT_ERR_TENSOR_MAP;
