@@ -102,7 +102,9 @@ int64_t makespan(int64_t pairs, int64_t n_long, int64_t len, int64_t n_short, in
     const int64_t a = x > full ? (x - full) / slen : 0, b = x > k * len ? (x - k * len) / slen : 0;
     return r > 0 ? r * a + (pairs - r) * b : pairs * b;
   };
-  int64_t lo = full, hi = full + (n_short / pairs + 1) * slen;
+  // between a perfect fill and one short tile more
+  int64_t lo = std::max(full, (n_short * slen + r * full + (pairs - r) * k * len + pairs - 1) / pairs);
+  int64_t hi = lo + slen;
   while (lo < hi) {
     const int64_t mid = (lo + hi) / 2;
     if (room(mid) >= n_short)
@@ -126,7 +128,7 @@ int plan_splits(const Plan& q, int segs, int64_t pairs) {
   const int64_t dw_len = q.n_pad / 64 * segs + 8;
   int best = 1;
   double best_time = 0;
-  for (const int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
+  for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
     if (s > 1 && kt / s < 8) break;
     const int64_t dh_len = (kt + s - 1) / s * segs + 8;
     const int64_t steps = dh_len > dw_len ? makespan(pairs, n_dh * s, dh_len, n_dw, dw_len)
@@ -152,7 +154,7 @@ Plan make_plan(const ttt_lce_problem& pb, int pass, int sms) {
   const int64_t most = std::max<int64_t>(2048, budget / std::max<int64_t>(per_col, 1));
   const int64_t pieces = (q.vocab + most - 1) / most;
   q.piece = up((q.vocab + pieces - 1) / pieces, 256);
-  q.splits = plan_splits(q, pass == 2 ? 2 : 1, std::max(1, sms / 2));
+  q.splits = pass == 0 ? 1 : plan_splits(q, pass, std::max(1, sms / 2));
   return q;
 }
 
@@ -162,8 +164,7 @@ int64_t score_parts(int64_t vocab) { return std::max<int64_t>(2 * ((vocab + ttt:
 struct Work {
   float2* part;        // statistics of half tiles, [2 * tiles][n_pad]
   float* ztgt;         // [n_pad]
-  float* rows;         // [n_pad] row losses (forward), derivatives by c (second)
-  float* sums;         // [n_pad / 32] their sums by block
+  float* sums;         // [n_pad / 32] sums of the row losses (or derivatives by c) by block
   unsigned* counters;  // [0] ticket of the products, [1] max_bits, [2] ticket of the row sums
   uint16_t* uc;        // gathered uh, [n_pad][dim_pad]
   float* coef;         // [n_pad]
@@ -180,7 +181,6 @@ int64_t work_layout(const Plan& q, int pass, void* base, Work* w) {
     const int64_t parts = pass == 0 ? score_parts(q.vocab) : 2 * ((q.vocab + ttt::kLceBNDual - 1) / ttt::kLceBNDual);
     t.part = a.take<float2>(parts * rows);
     t.ztgt = a.take<float>(rows);
-    t.rows = a.take<float>(rows);
     t.sums = a.take<float>(rows / 32);
   }
   if (pass != 0) {
@@ -781,6 +781,7 @@ struct Pass {
   Work w;
   LceCoef coef;
   const float* upstream;
+  int64_t work_need;
   int sms;
   bool bf16;
   int* err;
@@ -793,7 +794,7 @@ struct Pass {
         err_host(e != nullptr ? ttt::registered_error_mirror() : nullptr), s(static_cast<cudaStream_t>(stream)) {
     q = make_plan(p, pass, sms);
     state_layout(p, const_cast<void*>(state), &st);
-    work_layout(q, pass, work, &w);
+    work_need = work_layout(q, pass, work, &w);
     const bool listed = pass == 2 || (pass == 1 && p.reduction == TTT_LCE_NONE);
     coef = {st.head, p.reduction == TTT_LCE_NONE ? nullptr : dloss, st.mw, listed ? w.coef : nullptr,
             listed ? w.counters + 1 : nullptr};
@@ -936,9 +937,10 @@ int ttt_lce_fwd(const ttt_lce_fwd_args* a, void* stream) {
     return pb.reduction == TTT_LCE_NONE ? TTT_OK : zero(a->loss, 4, static_cast<cudaStream_t>(stream));
   if (a->h == nullptr || a->targets == nullptr) return TTT_ERR_NULL;
   if ((a->mask == nullptr) != (pb.mask_kind == TTT_LCE_MASK_NONE)) return TTT_ERR_NULL;
-  if (a->work == nullptr || a->work_bytes < ttt_lce_work_bytes(&pb, 0)) return TTT_ERR_SCRATCH;
+  if (a->work == nullptr) return TTT_ERR_SCRATCH;
   if (!aligned(a->work, 256) || !aligned(a->state, 256)) return TTT_ERR_ALIGN;
   Pass p(pb, 0, a->state, a->work, nullptr, a->err, stream);
+  if (a->work_bytes < p.work_need) return TTT_ERR_SCRATCH;
   RowArgs r = p.row_args(a->h, a->h_stride, p.st.hc);
   r.targets = a->targets, r.mask = a->mask, r.loss = a->loss;
   const Weight w(a->w, a->w_stride, pb);
@@ -978,9 +980,10 @@ int ttt_lce_bwd(const ttt_lce_bwd_args* a, void* stream) {
   if (pb.n == 0)
     return a->dw != nullptr ? zero(a->dw, pb.vocab * pb.dim * 2, static_cast<cudaStream_t>(stream)) : TTT_OK;
   if (a->h == nullptr) return TTT_ERR_NULL;
-  if (a->work == nullptr || a->work_bytes < ttt_lce_work_bytes(&pb, 1)) return TTT_ERR_SCRATCH;
+  if (a->work == nullptr) return TTT_ERR_SCRATCH;
   if (!aligned(a->work, 256) || !aligned(a->state, 256)) return TTT_ERR_ALIGN;
   Pass p(pb, 1, a->state, a->work, a->dloss, a->err, stream);
+  if (a->work_bytes < p.work_need) return TTT_ERR_SCRATCH;
   if (p.coef.coef != nullptr) TTT_TRY(p.list_coef(nullptr, 0));
   return run_pieces(p, Weight(a->w, a->w_stride, pb), nullptr, false, false, static_cast<uint16_t*>(a->dh),
                     static_cast<uint16_t*>(a->dw));
@@ -1003,9 +1006,10 @@ int ttt_lce_bwd2(const ttt_lce_bwd2_args* a, void* stream) {
     return TTT_OK;
   }
   if (a->h == nullptr) return TTT_ERR_NULL;
-  if (a->work == nullptr || a->work_bytes < ttt_lce_work_bytes(&pb, 2)) return TTT_ERR_SCRATCH;
+  if (a->work == nullptr) return TTT_ERR_SCRATCH;
   if (!aligned(a->work, 256) || !aligned(a->state, 256)) return TTT_ERR_ALIGN;
   Pass p(pb, 2, a->state, a->work, a->dloss, a->err, stream);
+  if (a->work_bytes < p.work_need) return TTT_ERR_SCRATCH;
   TTT_TRY(p.list_coef(a->uh, a->uh_stride));
   const Weight w(a->w, a->w_stride, pb);
   const Weight uw = a->uw != nullptr ? Weight(a->uw, a->uw_stride, pb) : w;
