@@ -19,6 +19,12 @@
 // The logits never leave the chip: the statistics kinds reduce them to two floats
 // per row and half tile, the gradient kinds turn them into the 16-bit derivative of
 // the logits of one piece of the vocabulary, which kLceProd contracts with w and h.
+//
+// Measured at 8192 x 768 x 32000 bf16, each launch on its own: statistics 217 us (1.85
+// PFLOP/s, tensor pipe 95 % active), G 258 us, both products 523 us (1.54), statistics of
+// (z, A) 694 us (1.74, 99 %), G and D 773 us (85 %), their four products 1080 us (1.49).
+// Back to back the GPU's power cap holds the clock near 1.35 GHz and the whole sequence
+// runs at 1.25 PFLOP/s (cuBLAS sustains 1.38 there), so what is left is energy, not issue.
 #include "attn_pipe.cuh"
 #include "lce.h"
 
@@ -376,8 +382,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
   } else if (go && warp == C::WARP_MMA && rank == 0) {
     // ------------------------------------------------------------ MMA issuer
     // The whole warp walks along, so that the compiler keeps descriptors and addresses in
-    // uniform registers; one thread issues. (A single thread on its own took ~96 cycles a
-    // product, more than a 128-wide one lasts.)
+    // uniform registers; one thread issues. A single thread on its own took ~96 cycles a
+    // product, more than a 128-wide one lasts: statistics of (z, A) 944 us, 727 like this.
     {
       const bool leader = elect_one();
       constexpr bool B_MN = !C::LOGIT;
