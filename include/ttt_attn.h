@@ -191,7 +191,9 @@ enum ttt_kernel_kind {
   TTT_K_BWD2_Q = 5,      /* dd_q (+ dd_dout) */
   TTT_K_BWD2_KV = 6,     /* dd_k, dd_v */
   TTT_K_FROM_P = 7,      /* passes over materialized P */
-  TTT_K_COUNT = 8
+  TTT_K_NORM = 8,        /* a call of ttt_norm_* (ttt_ops.h) */
+  TTT_K_LOSS = 9,        /* a call of ttt_lce_* (ttt_ops.h), its launches together */
+  TTT_K_COUNT = 10
 };
 
 /* Profiling hook (no reference counterpart; the reference times whole steps

@@ -40,8 +40,14 @@ def test_meta_step_and_scores_match_the_plain_model(window, suffix, chunk, pfilt
         return inner.item(), outer.item(), {n: p.grad for n, p in model.named_parameters() if p.grad is not None}, scores
 
     ri, ro, rg, rs = run(cpu, "cpu")
+    _lib.profile_collect()
+    _lib.profile_enable(True)
     gi, go, gg, gs = run(gpu, "cuda")
+    torch.cuda.synchronize()
+    _lib.profile_enable(False)
+    prof = _lib.profile_collect()
     _lib.check_device_errors()
+    assert prof["norm"][0] > 0 and prof["loss"][0] > 0 and prof["loss"][1] > 0.0
     assert abs(gi - ri) < 2e-2 * abs(ri) and abs(go - ro) < 2e-2 * abs(ro)
     assert set(gg) == set(rg)
     num = sum(float((gg[n].double().cpu() - rg[n]).pow(2).sum()) for n in rg)

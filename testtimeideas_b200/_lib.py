@@ -84,7 +84,8 @@ NOALLOC_MAX_ROWS = 1 << 20  # TTT_ATTN_NOALLOC_MAX_ROWS
 # Every symbol include/ttt_ops.h declares.
 EXPORTED_OPS = ("ttt_norm_fwd", "ttt_norm_bwd", "ttt_norm_bwd2", "ttt_norm_work_bytes", "ttt_lce_fwd", "ttt_lce_bwd",
                 "ttt_lce_bwd2", "ttt_lce_pad_weight", "ttt_lce_state_bytes", "ttt_lce_work_bytes")
-KERNEL_KINDS = ("fwd", "delta", "bwd_kv", "bwd_q", "bwd2_stats", "bwd2_q", "bwd2_kv", "from_p")
+KERNEL_KINDS = ("fwd", "delta", "bwd_kv", "bwd_q", "bwd2_stats", "bwd2_q", "bwd2_kv", "from_p", "norm",
+                "loss")
 
 _lib = None
 _lib_lock = threading.Lock()

@@ -7,11 +7,13 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <new>
 #include <vector>
 
 #include "ttt_attn.h"
 #include "host_ctx.h"
 #include "kernels.h"
+#include "prof.h"
 
 namespace {
 
@@ -447,6 +449,15 @@ namespace ttt {
 // For the operators of ttt_ops.h (lce.cu): the registered mirror, and a 2-D
 // 16-bit tensor map with 128-byte swizzle, elements outside read as zero.
 int32_t* registered_error_mirror() { return error_mirror(); }
+
+void* prof_begin(int kind, cudaStream_t stream) {
+  {
+    std::lock_guard<std::mutex> lk(g_prof_mu);
+    if (!g_prof_on) return nullptr;
+  }
+  return new (std::nothrow) ProfScope(kind, stream);
+}
+void prof_end(void* span) { delete static_cast<ProfScope*>(span); }
 
 bool encode_2d(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64_t rows, int64_t stride, int box_cols,
                int box_rows) {

@@ -23,6 +23,7 @@
 
 #include "host_ctx.h"
 #include "lce.h"
+#include "prof.h"
 #include "tc100.cuh"
 #include "ttt_ops.h"
 
@@ -941,6 +942,7 @@ int ttt_lce_fwd(const ttt_lce_fwd_args* a, void* stream) {
   if (!aligned(a->work, 256) || !aligned(a->state, 256)) return TTT_ERR_ALIGN;
   Pass p(pb, 0, a->state, a->work, nullptr, a->err, stream);
   if (a->work_bytes < p.work_need) return TTT_ERR_SCRATCH;
+  ttt::ProfSpan prof(TTT_K_LOSS, stream);
   RowArgs r = p.row_args(a->h, a->h_stride, p.st.hc);
   r.targets = a->targets, r.mask = a->mask, r.loss = a->loss;
   const Weight w(a->w, a->w_stride, pb);
@@ -984,6 +986,7 @@ int ttt_lce_bwd(const ttt_lce_bwd_args* a, void* stream) {
   if (!aligned(a->work, 256) || !aligned(a->state, 256)) return TTT_ERR_ALIGN;
   Pass p(pb, 1, a->state, a->work, a->dloss, a->err, stream);
   if (a->work_bytes < p.work_need) return TTT_ERR_SCRATCH;
+  ttt::ProfSpan prof(TTT_K_LOSS, stream);
   if (p.coef.coef != nullptr) TTT_TRY(p.list_coef(nullptr, 0));
   return run_pieces(p, Weight(a->w, a->w_stride, pb), nullptr, false, false, static_cast<uint16_t*>(a->dh),
                     static_cast<uint16_t*>(a->dw));
@@ -1010,6 +1013,7 @@ int ttt_lce_bwd2(const ttt_lce_bwd2_args* a, void* stream) {
   if (!aligned(a->work, 256) || !aligned(a->state, 256)) return TTT_ERR_ALIGN;
   Pass p(pb, 2, a->state, a->work, a->dloss, a->err, stream);
   if (a->work_bytes < p.work_need) return TTT_ERR_SCRATCH;
+  ttt::ProfSpan prof(TTT_K_LOSS, stream);
   TTT_TRY(p.list_coef(a->uh, a->uh_stride));
   const Weight w(a->w, a->w_stride, pb);
   const Weight uw = a->uw != nullptr ? Weight(a->uw, a->uw_stride, pb) : w;

@@ -32,6 +32,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "prof.h"
 #include "ttt_ops.h"
 
 namespace {
@@ -783,6 +784,7 @@ int ttt_norm_fwd(const ttt_norm_fwd_args* g, void* stream) {
   if (g->pb.rows > 0 && (g->x == nullptr || g->y == nullptr)) return TTT_ERR_NULL;
   if ((g->mean == nullptr) != (g->rstd == nullptr)) return TTT_ERR_NULL;
   if (g->x_stride < 0) return TTT_ERR_STRIDE;
+  ttt::ProfSpan prof(TTT_K_NORM, stream);
   return with_types(g->pb, [&](auto xt, auto pt) {
     using X = decltype(xt);
     using P = decltype(pt);
@@ -804,6 +806,7 @@ int ttt_norm_bwd(const ttt_norm_bwd_args* g, void* stream) {
   if (g->pb.rows > 0 && (g->x == nullptr || g->dy == nullptr || g->mean == nullptr || g->rstd == nullptr))
     return TTT_ERR_NULL;
   if (g->x_stride < 0 || g->dy_stride < 0) return TTT_ERR_STRIDE;
+  ttt::ProfSpan prof(TTT_K_NORM, stream);
   return with_types(g->pb, [&](auto xt, auto pt) {
     using X = decltype(xt);
     using P = decltype(pt);
@@ -827,6 +830,7 @@ int ttt_norm_bwd2(const ttt_norm_bwd2_args* g, void* stream) {
                          g->gx == nullptr || g->gdy == nullptr))
     return TTT_ERR_NULL;
   if (g->x_stride < 0 || g->dy_stride < 0 || g->ux_stride < 0) return TTT_ERR_STRIDE;
+  ttt::ProfSpan prof(TTT_K_NORM, stream);
   return with_types(g->pb, [&](auto xt, auto pt) {
     using X = decltype(xt);
     using P = decltype(pt);
