@@ -97,6 +97,24 @@ __device__ __forceinline__ void stay_packed(Pack<T, EPT>& v) {
   for (auto& w : v.w) asm volatile("" : "+r"(w));
 }
 
+// Threads that an SM holds, which leaves 65536 / threads registers to each: as many as hide
+// the memory's latency without registers spilled inside the loop over the rows.
+// Forward: 1024, but 512 where a thread has 32 elements (6710x10000 in fp32: 92 us against
+// 231 with 1024) and 768 where it has 16 that it loads in small pieces (22362x3001 in bf16:
+// 92 us against 118); with 8 elements fewer threads are slower (66974x1002: 62 against 67).
+constexpr int fwd_threads(int ept, int piece_bytes) {
+  return ept == 32 ? 512 : ept == 16 && piece_bytes < 16 ? 768 : 1024;
+}
+// Gradient: 512, but 768 where a thread has eight 16-bit elements, two sums a column among
+// its registers all the same. Times of a forward and gradient, 768 against 512 threads:
+// 43690x1536 143 and 173 us, 262144x256 136 and 151. Three layouts spill at 768: 128 threads
+// a row (65536x1024: 170 and 147), 96 (87381x768: 172, 186, and 165 with 576) and rows loaded
+// element by element (133949x501: 303 and 217; but 43662x1537, 256 threads: 240 and 266).
+constexpr int grad_threads(int ept, int elem_bytes, int vec, int nt) {
+  if (ept > 8 || elem_bytes > 2 || nt == 128 || (vec == 1 && nt < 256)) return 512;
+  return nt == 96 ? 576 : 768;
+}
+
 // The layout of a row: NT threads (part of a warp, or whole warps), each with K pieces of
 // VEC elements; piece k of thread t starts at column (k * NT + t) * VEC. VEC is 16 bytes
 // of X, or 4 bytes, or one element, as the rows are aligned. A block holds GROUPS rows at
@@ -107,10 +125,9 @@ struct Row {
   static constexpr int NT = NT_, EPT = EPT_, VEC = VEC_, K = EPT / VEC;
   static constexpr int PIECE = VEC * static_cast<int>(sizeof(X));  // bytes
   static constexpr int GROUPS = NT > 256 ? 1 : 256 / NT, THREADS = GROUPS * NT;
-  // Blocks that an SM holds: 64 registers a thread in the forward, 80 in the gradient of
-  // eight 16-bit elements, else 128.
-  static constexpr int FWD_PER_SM = 1024 / THREADS;
-  static constexpr int BWD_PER_SM = (EPT == 8 && sizeof(X) == 2 ? 768 : 512) / THREADS;
+  // Blocks that an SM holds.
+  static constexpr int FWD_PER_SM = fwd_threads(EPT, PIECE) / THREADS;
+  static constexpr int BWD_PER_SM = grad_threads(EPT, sizeof(X), VEC, NT) / THREADS;
   static constexpr int BWD2_PER_SM = 512 / THREADS;
 
   static __device__ __forceinline__ int column(int k, int t) { return (k * NT + t) * VEC; }
@@ -640,11 +657,12 @@ int row_threads(int D, bool wide) {
 }
 
 // Blocks of the gradient kernels: all that fit on the SMs at once, or as many as there are rows for.
-int grad_blocks(const ttt_norm_problem& pb, bool second, bool wide, int sms) {
-  const int nt = row_threads(pb.dim, wide), groups = nt > 256 ? 1 : 256 / nt, threads = groups * nt;
-  const int64_t res = pb.dim <= 2048 && pb.dtype != TTT_F32 && !second ? 768 : 512;
+int grad_blocks(const ttt_norm_problem& pb, bool second, int vec, int sms) {
+  const int elem = pb.dtype == TTT_F32 ? 4 : 2;
+  const int nt = row_threads(pb.dim, vec * elem == 16), groups = nt > 256 ? 1 : 256 / nt, threads = groups * nt;
+  const int64_t fit = second ? 512 : grad_threads(pb.dim <= 2048 ? 8 : 16, elem, vec, nt);
   return static_cast<int>(
-      std::min<int64_t>(std::max<int64_t>((pb.rows + groups - 1) / groups, 1), sms * (res / threads)));
+      std::min<int64_t>(std::max<int64_t>((pb.rows + groups - 1) / groups, 1), sms * (fit / threads)));
 }
 
 int check_norm(const ttt_norm_problem& pb) {
@@ -723,8 +741,10 @@ int run_norm(NormArgs<X, P> a, const ttt_norm_problem& pb, Pass pass, void* dw, 
   for (const void* p : rows_at) row_bits |= reinterpret_cast<uintptr_t>(p);
   for (const void* p : params_at) param_bits |= reinterpret_cast<uintptr_t>(p);
   const int64_t steps = pb.dim | a.x_stride | a.dy_stride | a.ux_stride;
-  const bool wide = ((row_bits | param_bits) & 15) == 0 && steps % V == 0;
-  const int blocks = pass == kFwd ? 0 : grad_blocks(pb, pass == kBwd2, wide, sms);
+  const int vec = ((row_bits | param_bits) & 15) == 0 && steps % V == 0 ? V
+                  : (row_bits & 3) == 0 && steps % H == 0               ? H
+                                                                        : 1;
+  const int blocks = pass == kFwd ? 0 : grad_blocks(pb, pass == kBwd2, vec, sms);
   if (a.want_dw || a.want_db) {
     if (work == nullptr || !aligned16(work) || work_bytes < static_cast<int64_t>(blocks) * 2 * pb.dim * 4)
       return TTT_ERR_SCRATCH;
@@ -732,9 +752,9 @@ int run_norm(NormArgs<X, P> a, const ttt_norm_problem& pb, Pass pass, void* dw, 
   }
   if (pb.rows > 0 || pass != kFwd) {
     cudaError_t e;
-    if (wide)
+    if (vec == V)
       e = launch_width<X, P, V>(a, pass, blocks, sms, s);
-    else if (H == 2 && (row_bits & 3) == 0 && steps % H == 0)
+    else if (vec == H && H == 2)
       e = launch_width<X, P, H>(a, pass, blocks, sms, s);
     else
       e = launch_width<X, P, 1>(a, pass, blocks, sms, s);
@@ -773,9 +793,11 @@ extern "C" {
 
 int64_t ttt_norm_work_bytes(const ttt_norm_problem* pb) {
   if (pb == nullptr || check_norm(*pb) != TTT_OK) return 0;
-  const int sms = sm_count();  // the gradient's blocks, in whichever layout has more of them
-  return static_cast<int64_t>(std::max(grad_blocks(*pb, false, true, sms), grad_blocks(*pb, false, false, sms))) * 2 *
-         pb->dim * 4;
+  const int sms = sm_count();
+  int blocks = 0;  // the gradient's, in whichever layout has most of them
+  for (const int vec : {1, 2, 4, 8})
+    for (const bool second : {false, true}) blocks = std::max(blocks, grad_blocks(*pb, second, vec, sms));
+  return static_cast<int64_t>(blocks) * 2 * pb->dim * 4;
 }
 
 int ttt_norm_fwd(const ttt_norm_fwd_args* g, void* stream) {
