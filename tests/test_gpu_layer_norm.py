@@ -106,6 +106,13 @@ def test_no_rows():
     assert y.shape == dx.shape == x.shape and torch.equal(dw, torch.zeros_like(w))
 
 
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32))
+@pytest.mark.parametrize("d", (4096, 5001, 8200, 9001, 9002, 16384))
+def test_several_wide_rows_a_block(d, dtype):
+    # more rows than blocks that fit on the SMs: the column sums run over a block's rows
+    _check(_inputs(640, d, dtype, dtype, seed=d))
+
+
 @pytest.mark.parametrize("weight,bias", [(True, False), (False, True), (False, False)])
 def test_optional_parameters(weight, bias):
     inp = _inputs(40, 300, torch.float16, torch.float16, seed=3)

@@ -130,6 +130,15 @@ struct Row {
   static constexpr int BWD_PER_SM = grad_threads(EPT, sizeof(X), VEC, NT) / THREADS;
   static constexpr int BWD2_PER_SM = 512 / THREADS;
 
+  // Column sums in shared memory, each thread its own, where the loop over the rows spills with
+  // them in registers. Forward and gradient: 8184x8200 in fp32 720 -> 302 us, 4096x16384 in bf16
+  // 225 -> 173. Forward and both gradients, all in bf16: 16384x4096 374 -> 311, 8192x8192
+  // 422 -> 366, 4096x16384 893 -> 440.
+  static constexpr bool SHARED_SUMS = EPT == 32;
+  static constexpr int SUM_BYTES = SHARED_SUMS ? 2 * EPT * THREADS * static_cast<int>(sizeof(float)) : 0;
+  static constexpr bool SHARED_SUMS2 = EPT >= 16;
+  static constexpr int SUM2_BYTES = SHARED_SUMS2 ? EPT * THREADS * static_cast<int>(sizeof(float)) : 0;
+
   static __device__ __forceinline__ int column(int k, int t) { return (k * NT + t) * VEC; }
   static __device__ __forceinline__ bool inside(int i, int t, int D) { return column(i / VEC, t) < D; }
 
@@ -246,10 +255,10 @@ __device__ __forceinline__ void row_sum(float (&v)[N], Sums<R>& sums, int& phase
 // summed (cp.async, 16 bytes a thread and piece). A thread reads back only what it
 // copied itself, so no barrier is needed. Rows that are not 16-byte aligned, or so wide
 // that fewer than two fit, are loaded into registers one row ahead instead (S = 0).
-template <class X, class R, int T, int PER_SM>
+template <class X, class R, int T, int PER_SM, int TAKEN = 0>
 struct Ring {
   static constexpr int ROW = R::K * R::THREADS * 16;  // bytes of one tensor's rows of a block
-  static constexpr int FIT = (200 << 10) / (PER_SM * T * ROW);
+  static constexpr int FIT = ((200 << 10) - PER_SM * TAKEN) / (PER_SM * T * ROW);
   static constexpr int S = R::PIECE < 16 || FIT < 2 ? 0 : (FIT < 4 ? FIT : 4);
   static constexpr int BYTES = S * T * ROW;
   const X* src[T];
@@ -309,9 +318,9 @@ __device__ __forceinline__ G make_ring(uint8_t* smem, int t, int D) {
 template <class X, class R>
 using FwdRing = Ring<X, R, 1, R::FWD_PER_SM>;
 template <class X, class R>
-using BwdRing = Ring<X, R, 2, R::BWD_PER_SM>;
+using BwdRing = Ring<X, R, 2, R::BWD_PER_SM, R::SUM_BYTES>;
 template <class X, class R>
-using Bwd2Ring = Ring<X, R, 3, R::BWD2_PER_SM>;
+using Bwd2Ring = Ring<X, R, 3, R::BWD2_PER_SM, R::SUM2_BYTES>;
 
 template <class X, class P>
 struct NormArgs {
@@ -432,8 +441,12 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD_PER_SM) norm_bwd_kernel(con
   const int t = threadIdx.x % R::NT;
   const float inv = 1.f / static_cast<float>(a.D);
   float aw[EPT], ab[EPT];
+  float* own = cols + threadIdx.x;  // SHARED_SUMS: element i of aw at own[i * THREADS], then ab's
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) aw[i] = ab[i] = 0.f;
+  for (int i = 0; i < EPT; ++i) {
+    aw[i] = ab[i] = 0.f;
+    if constexpr (R::SHARED_SUMS) own[i * R::THREADS] = own[(EPT + i) * R::THREADS] = 0.f;
+  }
   Pack<P, EPT> w;
   R::load(a.w, t, a.D, w, 1.f);
   const int64_t step = static_cast<int64_t>(gridDim.x) * R::GROUPS;
@@ -442,7 +455,10 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD_PER_SM) norm_bwd_kernel(con
   G ring = make_ring<G>(smem, t, a.D);
   ring.src[0] = a.x, ring.stride[0] = a.x_stride;
   ring.src[1] = a.dy, ring.stride[1] = a.dy_stride;
-  Pack<X, EPT> xn, dn;  // S = 0: the next row
+  // S = 0: the next row, where there are registers for it (rows of 32 elements: 16-bit ones in
+  // wide pieces; 7455x9001 in bf16 531 us with it, 348 without)
+  Pack<X, EPT> xn, dn;
+  constexpr bool AHEAD = EPT < 32 || R::PIECE * sizeof(X) == 32;
   float mun[2] = {0.f, 0.f}, rn[2] = {0.f, 0.f};  // statistics of the next two rows
   auto fetch_stats = [&](int64_t at, int i) {
     if (at < a.rows) mun[i] = a.mean[at], rn[i] = a.rstd[at];
@@ -456,7 +472,7 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD_PER_SM) norm_bwd_kernel(con
   if constexpr (G::S > 0) {
 #pragma unroll
     for (int i = 0; i < G::S - 1; ++i) ring.fetch(row + i * step, a.rows, i);
-  } else {
+  } else if constexpr (AHEAD) {
     fetch_rows(row);
   }
   for (int st = 0; (R::NT < 32 ? lead : row) < a.rows; row += step, lead += step) {
@@ -472,16 +488,22 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD_PER_SM) norm_bwd_kernel(con
       ring.read(st, 1, exists, dy);
       st = (st + 1) % G::S;
     } else {
+      if constexpr (!AHEAD) fetch_rows(row);
       x = xn, dy = dn;
-      fetch_rows(row + step);
+      if constexpr (AHEAD) fetch_rows(row + step);
     }
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
       // dy is zero outside the row (and past the last row), so nothing else has to be
       const float xh = (x.at(i) - mu) * r, d = dy.at(i), g = d * w.at(i);
-      aw[i] += d * xh;
-      ab[i] += d;
+      if constexpr (R::SHARED_SUMS) {
+        own[i * R::THREADS] += d * xh;
+        own[(EPT + i) * R::THREADS] += d;
+      } else {
+        aw[i] += d * xh;
+        ab[i] += d;
+      }
       s[0] += g;
       s[1] += g * xh;
     }
@@ -497,6 +519,10 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD_PER_SM) norm_bwd_kernel(con
                r * (dy.at(i + 1) * w.at(i + 1) - mg - (x.at(i + 1) - mu) * r * ma));
       R::store(a.dx + row * a.D, t, a.D, x);
     }
+  }
+  if constexpr (R::SHARED_SUMS) {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) aw[i] = own[i * R::THREADS], ab[i] = own[(EPT + i) * R::THREADS];
   }
   if (a.want_dw) write_part<R>(a.part, 0, a.D, aw, cols);
   if (a.want_db) write_part<R>(a.part, 1, a.D, ab, cols);
@@ -514,12 +540,19 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD2_PER_SM) norm_bwd2_kernel(c
   const int t = threadIdx.x % R::NT;
   const float inv = 1.f / static_cast<float>(a.D);
   float agw[EPT];
+  float* own = cols + threadIdx.x;  // SHARED_SUMS2: element i of agw at own[i * THREADS]
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) agw[i] = 0.f;
+  for (int i = 0; i < EPT; ++i) {
+    agw[i] = 0.f;
+    if constexpr (R::SHARED_SUMS2) own[i * R::THREADS] = 0.f;
+  }
   Pack<P, EPT> w, uw, ub;
-  R::load(a.w, t, a.D, w, 1.f);
-  R::load(a.uw, t, a.D, uw);
-  R::load(a.ub, t, a.D, ub);
+  constexpr bool RELOAD = EPT == 32;  // the parameters, for each pass over the row: no registers to keep them
+  if constexpr (!RELOAD) {
+    R::load(a.w, t, a.D, w, 1.f);
+    R::load(a.uw, t, a.D, uw);
+    R::load(a.ub, t, a.D, ub);
+  }
   const int64_t step = static_cast<int64_t>(gridDim.x) * R::GROUPS;
   int64_t row = static_cast<int64_t>(blockIdx.x) * R::GROUPS + threadIdx.x / R::NT;
   int64_t lead = static_cast<int64_t>(blockIdx.x) * R::GROUPS + lead_row<R>();
@@ -550,6 +583,10 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD2_PER_SM) norm_bwd2_kernel(c
       R::load(exists ? a.dy + row * a.dy_stride : nullptr, t, a.D, dy);
       R::load(exists && a.ux != nullptr ? a.ux + row * a.ux_stride : nullptr, t, a.D, u);
     }
+    if constexpr (RELOAD) {
+      R::load(a.w, t, a.D, w, 1.f);
+      R::load(a.uw, t, a.D, uw);
+    }
     float s[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // g, u, g xh, u xh, h, h xh
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
@@ -571,6 +608,7 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD2_PER_SM) norm_bwd2_kernel(c
     stay_packed(uw);
     const float mg = s[0] * inv, mu_u = s[1] * inv, ma = s[2] * inv, mc = s[3] * inv;
     float q[1] = {0.f};
+    if constexpr (RELOAD) R::load(a.w, t, a.D, w, 1.f);
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
       const float xh = (x.at(i) - mu) * r;
@@ -582,6 +620,11 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD2_PER_SM) norm_bwd2_kernel(c
     stay_packed(u);
     stay_packed(w);
     const float ms = q[0] * inv;
+    if constexpr (RELOAD) {
+      R::load(a.w, t, a.D, w, 1.f);
+      R::load(a.uw, t, a.D, uw);
+      R::load(a.ub, t, a.D, ub);
+    }
     // v = h - r (c g + a u): its mean and its mean against xh
     const float mv = s[4] * inv - r * (mc * mg + ma * mu_u);
     const float mvx = s[5] * inv - 2.f * r * ma * mc;
@@ -593,7 +636,10 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD2_PER_SM) norm_bwd2_kernel(c
         const float xh = (x.at(i + j) - mu) * r, d = dy.at(i + j);
         const float pu = r * (u.at(i + j) - mu_u - xh * mc);
         const float v = d * uw.at(i + j) - r * (mc * d * w.at(i + j) + ma * u.at(i + j));
-        agw[i + j] += d * pu;
+        if constexpr (R::SHARED_SUMS2)
+          own[(i + j) * R::THREADS] += d * pu;
+        else
+          agw[i + j] += d * pu;
         gd[j] = w.at(i + j) * pu + xh * uw.at(i + j) + ub.at(i + j);
         gx[j] = r * (v - mv - xh * mvx) - r * r * ms * xh;
       }
@@ -604,6 +650,10 @@ __global__ void __launch_bounds__(R::THREADS, R::BWD2_PER_SM) norm_bwd2_kernel(c
       R::store(a.gdy + row * a.D, t, a.D, dy);
       R::store(a.gx + row * a.D, t, a.D, x);
     }
+  }
+  if constexpr (R::SHARED_SUMS2) {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) agw[i] = own[i * R::THREADS];
   }
   if (a.want_dw) write_part<R>(a.part, 0, a.D, agw, cols);
 }
@@ -690,8 +740,8 @@ cudaError_t launch_rows(const NormArgs<X, P>& a, Pass pass, int blocks, int sms,
   }
   // several rows a block: their column sums, at most 8 KB (D <= 8 NT, 256 threads)
   const int cols = R::GROUPS > 1 ? static_cast<int>(sizeof(float)) * R::GROUPS * a.D : 0;
-  if (pass == kBwd) return launch(norm_bwd_kernel<X, P, R>, blocks, BwdRing<X, R>::BYTES + cols);
-  return launch(norm_bwd2_kernel<X, P, R>, blocks, Bwd2Ring<X, R>::BYTES + cols);
+  if (pass == kBwd) return launch(norm_bwd_kernel<X, P, R>, blocks, BwdRing<X, R>::BYTES + R::SUM_BYTES + cols);
+  return launch(norm_bwd2_kernel<X, P, R>, blocks, Bwd2Ring<X, R>::BYTES + R::SUM2_BYTES + cols);
 }
 
 template <class X, class P, int VEC>
