@@ -21,8 +21,8 @@
 // what covers the memory's latency.
 // Mean and variance are two sums over registers, and no statistic is a difference
 // of large sums. The threads of a row own fixed columns, so the parameter gradients
-// are summed in registers over all rows that a block meets; the blocks' sums (fp32)
-// are added in block order by a second small kernel, launched ahead of the first
+// are summed in registers (wide rows: in shared memory, see Row) over all rows that a
+// block meets; the blocks' sums (fp32) are added in block order by a second small kernel, launched ahead of the first
 // one's end. Everything is computed in fp32 and rounded once on the way out.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
