@@ -232,6 +232,22 @@ def test_more_than_one_piece():
     _check(inp, _mask(70000, "bool", 42), "sum", up=1.0)
 
 
+@pytest.mark.parametrize("n,d,v", [(32768, 64, 253953), (16384, 24, 253953), (16384, 512, 262208)])
+def test_last_piece_shorter_than_its_shares(n, d, v):
+    """The hidden gradient is cut into shares of a piece's columns, two (or three) here, and the last
+    piece is a single column (or 64): shares without columns leave the sums alone. First gradient for
+    the first size, second for the others. Few rows are kept, which the plan does not look at."""
+    inp = _inputs(n, d, v, torch.bfloat16, seed=v + d)
+    m = torch.zeros(n, device="cuda")
+    m[:: n // 130] = 1.0
+    dl = torch.full((), 64.0, device="cuda")
+    got = _all(lambda h, w: tb.linear_cross_entropy(h, w, inp["t"], m), inp["h"], inp["w"], dl, inp["uh"], inp["uw"])
+    ref = _all(lambda h, w: _definition(h, w, inp["t"], m, "mean"), inp["h"].double(), inp["w"].double(), dl.double(),
+               inp["uh"].double(), inp["uw"].double())
+    _compare(got, ref, torch.bfloat16)
+    _lib.check_device_errors()
+
+
 def test_few_rows_split_the_vocabulary():
     """One token tile, a long vocabulary: the dh product is shared between CTAs."""
     _check(_inputs(3, 160, 40000, torch.bfloat16, seed=43), up=4.0)

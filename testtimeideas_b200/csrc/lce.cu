@@ -130,7 +130,7 @@ int plan_splits(const Plan& q, int segs, int64_t pairs) {
   int best = 1;
   double best_time = 0;
   for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-    if (s > 1 && kt / s < 8) break;
+    if (s > 1 && kt / s < 8) break;  // of the first piece; the last one may leave shares without columns
     const int64_t dh_len = (kt + s - 1) / s * segs + 8;
     const int64_t steps = dh_len > dw_len ? makespan(pairs, n_dh * s, dh_len, n_dw, dw_len)
                                           : makespan(pairs, n_dw, dw_len, n_dh * s, dh_len);

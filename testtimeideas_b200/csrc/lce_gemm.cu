@@ -397,7 +397,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
       for (int t; ok && (t = walk.template next<kWarp>(g)) >= 0;) {
         const LceTile tl = lce_tile<KIND>(p, sz, t);
         const int steps = (tl.k1 - tl.k0) * (C::LOGIT ? 1 : __popc(tl.dw ? p.seg_h : p.seg_w));
-        if (steps == 0) continue;  // the epilogue writes zeros by itself
+        if (steps == 0) continue;  // the epilogue does without the accumulators
         const int buf = nth & 1;
         if (nth >= 2 && !(ok = __all_sync(0xffffffffu, mbar_wait(acc_free + buf, ((nth >> 1) - 1) & 1, g, 0x52)))) break;
         const uint32_t d = tmem + buf * 256;
@@ -575,6 +575,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
           store_panel<BF16, C::BOXES>(panel, turn, &p.out[0], lane, cq, row0, v);
         }
       } else if (!tl.dw) {
+        // A share without columns adds nothing to the partial rows. Only a last piece can be that
+        // short (the plan gives every share of the first one some steps), and an earlier piece
+        // has written them.
+        if (!have) continue;
         float* dst = p.acc + (static_cast<int64_t>(tl.split) * p.n_pad + slot) * p.dim_pad;
 #pragma unroll 1
         for (int q = 0; q < C::HALF / 32; ++q) {
