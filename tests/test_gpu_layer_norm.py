@@ -148,6 +148,24 @@ def test_layouts(dtype):
     _compare({"dx": dx, "dw": dw}, {"dx": rx, "dw": rw})
 
 
+@pytest.mark.parametrize("d", (64, 258, 301, 520, 768, 2050, 9002))
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_parameters_inside_a_flat_buffer(dtype, d):
+    """16-bit weight, bias and their upstream gradients as slices at odd and even offsets: aligned
+    rows beside parameters on 2-byte, 4-byte and 8-byte boundaries, alone and together."""
+    inp = _inputs(70, d, dtype, dtype, seed=d)
+    names = ("w", "b", "uw", "ub")
+
+    def at(v, off):
+        flat = torch.zeros(d + 16, dtype=dtype, device="cuda")
+        flat[off:off + d] = v.cuda()
+        return flat[off:off + d]
+
+    for off in (1, 2, 4, 7):
+        for moved in (names, ("w",), ("b",), ("uw",), ("ub",)):
+            _check(inp, **{k: at(inp[k], off) for k in moved})
+
+
 def test_batched_shape():
     inp = _inputs(24, 128, torch.bfloat16, torch.bfloat16, seed=1)
     x = inp["x"].cuda()

@@ -783,7 +783,7 @@ int run_norm(NormArgs<X, P> a, const ttt_norm_problem& pb, Pass pass, void* dw, 
   a.want_db = db != nullptr;
   const int sms = sm_count();
   // 16-byte pieces need every row and every parameter vector on a 16-byte boundary, 4-byte
-  // pieces the rows on a 4-byte one
+  // pieces (two 16-bit elements) the rows and 16-bit parameters on a 4-byte one
   constexpr int V = 16 / static_cast<int>(sizeof(X)), H = 4 / static_cast<int>(sizeof(X));
   const void* rows_at[] = {a.x, a.dy, a.ux, a.y, a.dx, a.gx, a.gdy};
   const void* params_at[] = {a.w, a.b, a.uw, a.ub};
@@ -791,9 +791,9 @@ int run_norm(NormArgs<X, P> a, const ttt_norm_problem& pb, Pass pass, void* dw, 
   for (const void* p : rows_at) row_bits |= reinterpret_cast<uintptr_t>(p);
   for (const void* p : params_at) param_bits |= reinterpret_cast<uintptr_t>(p);
   const int64_t steps = pb.dim | a.x_stride | a.dy_stride | a.ux_stride;
-  const int vec = ((row_bits | param_bits) & 15) == 0 && steps % V == 0 ? V
-                  : (row_bits & 3) == 0 && steps % H == 0               ? H
-                                                                        : 1;
+  const int vec = ((row_bits | param_bits) & 15) == 0 && steps % V == 0  ? V
+                  : ((row_bits | param_bits) & 3) == 0 && steps % H == 0 ? H
+                                                                         : 1;
   const int blocks = pass == kFwd ? 0 : grad_blocks(pb, pass == kBwd2, vec, sms);
   if (a.want_dw || a.want_db) {
     if (work == nullptr || !aligned16(work) || work_bytes < static_cast<int64_t>(blocks) * 2 * pb.dim * 4)
