@@ -430,3 +430,15 @@ def test_refusals():
         tb.linear_cross_entropy(h, w, t, torch.ones(4, device="cuda"))
     with pytest.raises(RuntimeError, match="CUDA tensors|device"):
         tb.linear_cross_entropy(h, w.cpu(), t)
+
+
+@pytest.mark.parametrize("dtype", (torch.uint8, torch.int8, torch.bool, torch.float8_e4m3fn, torch.float64, torch.int64))
+def test_weights_of_other_types_are_refused_with_gradients(dtype):
+    """Before the copy into aligned rows, which an odd width asks for and which moves 16-bit elements."""
+    inp = _inputs(8, 33, 40, torch.bfloat16, seed=66)
+    h = inp["h"].requires_grad_(True)
+    w = torch.ones(40, 33, device="cuda").to(dtype)
+    with pytest.raises(RuntimeError, match="share one dtype"):
+        tb.linear_cross_entropy(h, w, inp["t"])
+    with pytest.raises(RuntimeError, match="expected hidden"):
+        tb.linear_cross_entropy(h, torch.ones(40, 31, device="cuda", dtype=torch.bfloat16), inp["t"])

@@ -536,11 +536,13 @@ at::Tensor op_layer_norm_ad(const at::Tensor& x, const OptTensor& w_, const OptT
 }
 
 // Weights that the kernels cannot read in place (odd widths) are copied once, in the
-// forward, and the copy (`rows`, else undefined) is kept for both gradients.
-at::Tensor kept_rows(const at::Tensor& w) {
-  if (!w.is_cuda() || w.dim() != 2 || w.numel() == 0 || w.scalar_type() == at::kFloat ||
+// forward, and the copy (`rows`, else undefined) is kept for both gradients. The copy moves
+// 16-bit elements, so what the operator refuses is refused before it.
+at::Tensor kept_rows(const at::Tensor& h, const at::Tensor& w) {
+  if (!h.is_cuda() || !w.is_cuda() || h.key_set().has(c10::DispatchKey::Python) ||
       w.key_set().has(c10::DispatchKey::Python))
     return at::Tensor();  // refused by the operator, or being traced
+  lce_problem(h, w, TTT_LCE_NONE, 0);
   c10::cuda::CUDAGuard guard(w.device());
   const at::Tensor r = weight_rows(w);
   return r.is_same(w) ? at::Tensor() : r;
@@ -582,7 +584,7 @@ struct LinearCEFn : torch::autograd::Function<LinearCEFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& targets,
                             const OptTensor& mask, int64_t reduction, int64_t ignore_index) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const at::Tensor rows = kept_rows(w);
+    const at::Tensor rows = kept_rows(h, w);
     auto [loss, state] = raw_linear_ce().call(h, rows_or(rows, w), targets, mask, reduction, ignore_index, true);
     ctx->save_for_backward({h, w, state, rows});
     ctx->set_materialize_grads(false);
