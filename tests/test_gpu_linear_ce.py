@@ -442,3 +442,14 @@ def test_weights_of_other_types_are_refused_with_gradients(dtype):
         tb.linear_cross_entropy(h, w, inp["t"])
     with pytest.raises(RuntimeError, match="expected hidden"):
         tb.linear_cross_entropy(h, torch.ones(40, 31, device="cuda", dtype=torch.bfloat16), inp["t"])
+
+
+@pytest.mark.parametrize("n,d,v", [(2, 2**32, 3), (2, 2**32 + 8, 3), (2, 65537, 3), (2**24 + 1, 1, 3), (2, 1, 2**24 + 1)])
+@pytest.mark.parametrize("grad", (False, True))
+def test_sizes_past_the_limits_are_refused(n, d, v, grad):
+    """Broadcast tensors: no memory behind the sizes, 2^32 columns among them."""
+    h = torch.zeros(1, 1, dtype=torch.bfloat16, device="cuda").expand(n, d).requires_grad_(grad)
+    w = torch.zeros(1, 1, dtype=torch.bfloat16, device="cuda").expand(v, d)
+    t = torch.zeros(1, dtype=torch.long, device="cuda").expand(n)
+    with pytest.raises(RuntimeError, match="at most 2\\^24 rows"):
+        tb.linear_cross_entropy(h, w, t)

@@ -248,11 +248,11 @@ ttt_lce_problem lce_problem(const at::Tensor& h, const at::Tensor& w, int64_t re
               "linear cross entropy: expected hidden [..., dim] and weight [vocab, dim], got ", h.sizes(), " and ",
               w.sizes());
   ttt_lce_problem pb{};
-  pb.dim = static_cast<int32_t>(w.size(1));
-  pb.n = h.numel() / pb.dim;
+  pb.n = h.numel() / w.size(1);
   pb.vocab = w.size(0);
-  TORCH_CHECK(pb.dim <= 65536 && pb.n <= (1 << 24) && pb.vocab <= (1 << 24),
+  TORCH_CHECK(w.size(1) <= 65536 && pb.n <= (1 << 24) && pb.vocab <= (1 << 24),
               "linear cross entropy takes at most 2^24 rows, 2^24 vocabulary entries and 65536 columns");
+  pb.dim = static_cast<int32_t>(w.size(1));
   pb.dtype = type_code(t);
   TORCH_CHECK(reduction >= 0 && reduction <= 2, "linear cross entropy: unknown reduction ", reduction);
   pb.reduction = static_cast<int32_t>(reduction);
