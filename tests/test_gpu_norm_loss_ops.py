@@ -163,3 +163,27 @@ def test_vocabulary_past_32_bit_offsets():
     tol = 4 * 2.0**-9  # as in test_gpu_linear_ce.py
     assert float((dh.double() - ref_dh).abs().max() / ref_dh.abs().max()) <= tol
     assert float((dw[-300:].double() - ref_dw).abs().max() / ref_dw.abs().max()) <= tol
+
+
+def test_gradients_refuse_what_is_not_the_forwards():
+    """The bytes and statistics that a gradient reads: not those of a forward without them, of another
+    size, type or device, or strided."""
+    x, ops = _inputs(n=5, d=64, v=90), torch.ops.ttt
+    for n in (5, 2):  # the second takes the path of a few rows
+        h, t = x["h"][:n], x["t"][:n]
+        loss, none = ops.linear_ce(h, x["w"], t, None, 1, -100, False)
+        _, state = ops.linear_ce(h, x["w"], t, None, 1, -100, True)
+        assert none.numel() == 0 and none.dtype == state.dtype
+        one = torch.ones_like(loss)
+        for bad in (none, state[:-256], state.cpu(), state.float(), state.repeat_interleave(2)[::2]):
+            with pytest.raises(RuntimeError, match="state must be"):
+                ops.linear_ce_bwd(one, h, x["w"], bad, 1, True, True)
+            with pytest.raises(RuntimeError, match="state must be"):
+                ops.linear_ce_bwd2(one, h, x["w"], bad, 1, h, x["w"], True, True, True)
+    _, stats = ops.layer_norm(x["h"], None, None, 1e-5, True)
+    _, none = ops.layer_norm(x["h"], None, None, 1e-5, False)
+    for bad in (none, stats[:, :4], stats.cpu(), stats.double(), stats.repeat_interleave(2, 1)[:, ::2]):
+        with pytest.raises(RuntimeError, match="stats must be"):
+            ops.layer_norm_bwd(x["h"], x["h"], None, bad, True, False, False, torch.bfloat16)
+        with pytest.raises(RuntimeError, match="stats must be"):
+            ops.layer_norm_bwd2(x["h"], x["h"], None, bad, x["h"], None, None)

@@ -198,7 +198,8 @@ def _register_fakes() -> None:
     @torch.library.register_fake("ttt::linear_ce")
     def _lce(h, w, targets, mask, reduction, ignore_index, need_state):
         loss = h.new_empty(targets.shape if reduction == 0 else (), dtype=torch.float32)
-        return loss, h.new_empty((_lce_state_bytes(targets.numel(), h.shape[-1]),), dtype=torch.uint8)
+        bytes_ = _lce_state_bytes(targets.numel(), h.shape[-1]) if need_state else 0
+        return loss, h.new_empty((bytes_,), dtype=torch.uint8)
 
     @torch.library.register_fake("ttt::linear_ce_bwd")
     def _lce_bwd(dloss, h, w, state, reduction, need_dh, need_dw):

@@ -132,9 +132,10 @@ Rows grad_rows(const at::Tensor& g, const at::Tensor& x, int64_t dim, const char
   return Rows(g.scalar_type() == x.scalar_type() ? g : g.to(x.scalar_type()), dim);
 }
 
-void check_stats(const at::Tensor& stats, int64_t rows) {
-  TORCH_CHECK(stats.is_cuda() && stats.scalar_type() == at::kFloat && stats.numel() == 2 * rows && stats.is_contiguous(),
-              "layer norm: stats must be the forward's fp32 [2, rows]");
+void check_stats(const at::Tensor& stats, const at::Tensor& x, int64_t rows) {
+  TORCH_CHECK(stats.device() == x.device() && stats.scalar_type() == at::kFloat && stats.numel() == 2 * rows &&
+                  stats.is_contiguous(),
+              "layer norm: stats must be the forward's fp32 [2, rows] on x's device");
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> op_layer_norm_bwd(const at::Tensor& dy_, const at::Tensor& x_,
@@ -146,7 +147,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_layer_norm_bwd(const at::Tenso
   c10::cuda::CUDAGuard guard(x_.device());
   at::Tensor word = error_word_for(x_.get_device());
   raise_if_pending(x_.get_device(), word);
-  check_stats(stats, pb.rows);
+  check_stats(stats, x_, pb.rows);
   const Rows x(x_, pb.dim), dy = grad_rows(dy_, x_, pb.dim, "dy");
   const at::Tensor w = vec(w_);
   const auto po = x_.options().dtype(p_type);
@@ -179,7 +180,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_layer_norm_bwd2(const at::Tens
   c10::cuda::CUDAGuard guard(x_.device());
   at::Tensor word = error_word_for(x_.get_device());
   raise_if_pending(x_.get_device(), word);
-  check_stats(stats, pb.rows);
+  check_stats(stats, x_, pb.rows);
   const auto pt = w_.has_value() ? w_->scalar_type() : x_.scalar_type();
   const Rows x(x_, pb.dim), dy = grad_rows(dy_, x_, pb.dim, "dy");
   const at::Tensor w = vec(w_);
@@ -307,6 +308,8 @@ std::tuple<at::Tensor, at::Tensor> op_linear_ce(const at::Tensor& h_, const at::
   a.work = ptr(work);
   a.work_bytes = work.defined() ? work.numel() : 0;
   check(ttt_lce_fwd(&a, stream()), "ttt::linear_ce");
+  // without need_state the buffer was scratch, which no gradient may read
+  if (!need_state) state = at::empty({0}, state.options());
   return {loss, state};
 }
 
@@ -316,9 +319,10 @@ at::Tensor lce_upstream(const at::Tensor& dloss, const at::Tensor& h, const ttt_
               "linear cross entropy: dloss must have the loss's shape, got ", dloss.sizes());
   return dloss.to(at::kFloat).contiguous();
 }
-void check_state(const at::Tensor& state, const ttt_lce_problem& pb) {
-  TORCH_CHECK(state.is_cuda() && state.scalar_type() == at::kByte && state.numel() == ttt_lce_state_bytes(&pb),
-              "linear cross entropy: state must be the forward's");
+void check_state(const at::Tensor& state, const at::Tensor& h, const ttt_lce_problem& pb) {
+  TORCH_CHECK(state.device() == h.device() && state.scalar_type() == at::kByte && state.is_contiguous() &&
+                  state.numel() == ttt_lce_state_bytes(&pb),
+              "linear cross entropy: state must be that of a forward with need_state, on hidden's device");
 }
 
 std::tuple<at::Tensor, at::Tensor> op_linear_ce_bwd(const at::Tensor& dloss_, const at::Tensor& h_,
@@ -328,7 +332,7 @@ std::tuple<at::Tensor, at::Tensor> op_linear_ce_bwd(const at::Tensor& dloss_, co
   c10::cuda::CUDAGuard guard(h_.device());
   at::Tensor word = error_word_for(h_.get_device());
   raise_if_pending(h_.get_device(), word);
-  check_state(state, pb);
+  check_state(state, h_, pb);
   const Rows h(h_, pb.dim);
   const at::Tensor w = weight_rows(w_), dloss = lce_upstream(dloss_, h_, pb);
   at::Tensor dh = need_dh ? at::empty(h_.sizes(), h_.options()) : at::empty({0}, h_.options());
@@ -360,7 +364,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_linear_ce_bwd2(const at::Tenso
   c10::cuda::CUDAGuard guard(h_.device());
   at::Tensor word = error_word_for(h_.get_device());
   raise_if_pending(h_.get_device(), word);
-  check_state(state, pb);
+  check_state(state, h_, pb);
   const Rows h(h_, pb.dim);
   const at::Tensor w = weight_rows(w_), dloss = lce_upstream(dloss_, h_, pb);
   Rows uh;
@@ -630,7 +634,7 @@ TORCH_LIBRARY_FRAGMENT(ttt, m) {
   m.def("layer_norm_bwd2(Tensor dy, Tensor x, Tensor? w, Tensor stats, Tensor? ux, Tensor? uw, Tensor? ub) "
         " -> (Tensor gdy, Tensor gx, Tensor gw)");
   // reduction: 0 none, 1 mean, 2 sum; state (bytes) is what the gradients need of the forward
-  // (filled only with need_state).
+  // (empty without need_state).
   m.def("linear_ce(Tensor h, Tensor w, Tensor targets, Tensor? mask, int reduction, int ignore_index, bool "
         "need_state) -> (Tensor loss, Tensor state)");
   m.def("linear_ce_bwd(Tensor dloss, Tensor h, Tensor w, Tensor state, int reduction, bool need_dh, bool need_dw) -> "
