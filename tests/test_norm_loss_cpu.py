@@ -197,3 +197,59 @@ def test_buffer_sizes(lib):
             assert lib.ttt_lce_work_bytes(ctypes.byref(pb), p) <= (513 << 20) + extra + 256 * n
     assert lib.ttt_lce_work_bytes(ctypes.byref(LceProblem(1, 0, 64, 1, 1, 0, 0)), 1) == 0
     assert lib.ttt_lce_state_bytes(None) == 0
+
+
+# ---------------------------------------------------------------- forward mode
+@pytest.fixture()
+def stand_ins(lib):
+    """The raw operators on CPU tensors, so that what surrounds them can be run here."""
+    _lib.load_torch_ops()
+    with torch.library._scoped_library("ttt", "IMPL") as impl:
+        impl.impl("layer_norm", lambda x, w, b, eps, need: (
+            F.layer_norm(x, x.shape[-1:], w, b, eps), x.new_zeros(2, x.numel() // x.shape[-1] if need else 0)), "CPU")
+        impl.impl("layer_norm_bwd", lambda dy, x, w, stats, need_dx, need_dw, need_db, p_type: (
+            dy.clone(), x.new_zeros(x.shape[-1]), x.new_zeros(x.shape[-1])), "CPU")
+        impl.impl("linear_ce", lambda h, w, t, m, reduction, ignore, need: (
+            F.cross_entropy(h @ w.t(), t), h.new_zeros(0, dtype=torch.uint8)), "CPU")
+        impl.impl("linear_ce_bwd", lambda dloss, h, w, state, reduction, need_dh, need_dw: (
+            dloss * h, dloss * w), "CPU")
+        yield torch.ops.ttt
+
+
+def test_forward_mode_is_refused(stand_ins):
+    """Neither operator has a forward-mode derivative: a tensor with a tangent raises, whichever input it is,
+    and so does a tangent on the upstream gradient. Without one (or with the mode off) nothing changes."""
+    import torch.autograd.forward_ad as fwd
+
+    x, w, b = torch.randn(5, 8), torch.randn(8), torch.randn(8)
+    head, t, m = torch.randn(9, 8), torch.randint(0, 9, (5,)), torch.ones(5)
+    norm = lambda x, w, b: stand_ins.layer_norm_ad(x, w, b, 1e-5)  # noqa: E731
+    loss = lambda h, w, m: stand_ins.linear_ce_ad(h, w, t, m, 1, -100)  # noqa: E731
+    for fn, args in ((norm, (x, w, b)), (loss, (x, head, m))):
+        plain = fn(*args)
+        for i in range(3):
+            tangents = [torch.zeros_like(a) for a in args]
+            tangents[i] = torch.ones_like(args[i])
+
+            def one(a, i=i):
+                return fn(*args[:i], a, *args[i + 1:])
+
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.func.jvp(one, (args[i],), (tangents[i],))
+            with fwd.dual_level():
+                dual = fwd.make_dual(args[i], tangents[i])
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    one(dual)
+                with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+                    one(dual)
+                with fwd._set_fwd_grad_enabled(False):
+                    assert torch.equal(one(dual), plain)
+        # reverse mode is as before, and a tangent of the upstream gradient is refused
+        leaf = args[0].clone().requires_grad_(True)
+        y = fn(leaf, *args[1:])
+        torch.autograd.grad(y, leaf, torch.ones_like(y), retain_graph=True)
+        with fwd.dual_level():
+            up = fwd.make_dual(torch.ones_like(y), torch.ones_like(y))
+            for create in (False, True):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    torch.autograd.grad(y, leaf, up, retain_graph=True, create_graph=create)

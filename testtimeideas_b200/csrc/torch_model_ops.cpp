@@ -9,6 +9,7 @@
 // each is itself a Function with a closed-form backward, as the attention's is,
 // and computes only the gradients that the running backward asks for.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -409,6 +410,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_linear_ce_bwd2(const at::Tenso
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// The operators run below the autograd keys, where a forward-mode tangent would be lost: refused instead.
+void refuse_tangents(const char* op, std::initializer_list<const at::Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), op, " has no forward-mode derivative");
+}
+constexpr const char *kNormOp = "layer norm", *kLceOp = "linear cross entropy";
+
 at::Tensor defined_or(const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); }
 OptTensor opt(const at::Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 
@@ -477,6 +486,7 @@ struct LayerNormBwdFn : torch::autograd::Function<LayerNormBwdFn> {
     const variable_list v = ctx->get_saved_variables();
     variable_list g(6);
     if (!up[0].defined() && !up[1].defined() && !up[2].defined()) return g;
+    refuse_tangents(kNormOp, {&up[0], &up[1], &up[2]});
     {
       at::AutoDispatchBelowADInplaceOrView below;
       std::tie(g[0], g[1], g[2]) =
@@ -503,6 +513,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   static variable_list backward(AutogradContext* ctx, const variable_list& up) {
     variable_list g(4);
     if (!up[0].defined()) return g;
+    refuse_tangents(kNormOp, {&up[0]});
     const variable_list v = ctx->get_saved_variables();
     const int64_t p_type = ctx->saved_data["p_type"].toInt();
     // needs_input_grad counts the tensors that were given: x, then w and b where present
@@ -534,6 +545,7 @@ bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
 
 at::Tensor op_layer_norm_ad(const at::Tensor& x, const OptTensor& w_, const OptTensor& b_, double eps) {
   const at::Tensor w = defined_or(w_), b = defined_or(b_);
+  refuse_tangents(kNormOp, {&x, &w, &b});
   if (wants_grad({&x, &w, &b})) return LayerNormFn::apply(x, w_, b_, eps);
   at::AutoDispatchBelowADInplaceOrView below;
   return std::get<0>(raw_layer_norm().call(x, w_, b_, eps, false));
@@ -569,6 +581,7 @@ struct LinearCEBwdFn : torch::autograd::Function<LinearCEBwdFn> {
     const variable_list v = ctx->get_saved_variables();
     variable_list g(7);
     if (!up[0].defined() && !up[1].defined()) return g;
+    refuse_tangents(kLceOp, {&up[0], &up[1]});
     bool need[3];
     for (int i = 0; i < 3; ++i) need[i] = ctx->needs_input_grad(i);
     {
@@ -598,6 +611,7 @@ struct LinearCEFn : torch::autograd::Function<LinearCEFn> {
   static variable_list backward(AutogradContext* ctx, const variable_list& up) {
     variable_list g(6);
     if (!up[0].defined()) return g;
+    refuse_tangents(kLceOp, {&up[0]});
     const variable_list v = ctx->get_saved_variables();
     const int64_t reduction = ctx->saved_data["reduction"].toInt();
     const int64_t need = (ctx->needs_input_grad(0) ? 1 : 0) | (ctx->needs_input_grad(1) ? 2 : 0);
@@ -618,6 +632,8 @@ struct LinearCEFn : torch::autograd::Function<LinearCEFn> {
 
 at::Tensor op_linear_ce_ad(const at::Tensor& h, const at::Tensor& w, const at::Tensor& targets, const OptTensor& mask,
                            int64_t reduction, int64_t ignore_index) {
+  const at::Tensor weights = defined_or(mask);
+  refuse_tangents(kLceOp, {&h, &w, &weights});
   if (wants_grad({&h, &w})) return LinearCEFn::apply(h, w, targets, mask, reduction, ignore_index);
   at::AutoDispatchBelowADInplaceOrView below;
   return std::get<0>(raw_linear_ce().call(h, w, targets, mask, reduction, ignore_index, false));

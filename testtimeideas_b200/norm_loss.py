@@ -5,9 +5,9 @@ The meta step (``ttt_model.meta_step``) takes the gradient of a gradient through
 every op of the inner step: the norms of each block and the token loss among
 them. Both operators here follow the attention's form: an autograd Function
 whose backward is itself a Function with a closed-form backward (in C++,
-csrc/torch_model_ops.cpp); a third derivative raises. CUDA tensors run the
-kernels (C ABI in include/ttt_ops.h); CPU tensors run the PyTorch formulation of
-the same value.
+csrc/torch_model_ops.cpp); a third derivative and, on CUDA, a forward-mode one
+raise. CUDA tensors run the kernels (C ABI in include/ttt_ops.h); CPU tensors run
+the PyTorch formulation of the same value.
 """
 
 from __future__ import annotations
