@@ -253,3 +253,17 @@ def test_forward_mode_is_refused(stand_ins):
             for create in (False, True):
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     torch.autograd.grad(y, leaf, up, retain_graph=True, create_graph=create)
+
+
+def test_a_mask_that_wants_a_gradient_is_refused(stand_ins):
+    """The kernels form no gradient by the mask's weights; none was returned without a word."""
+    h, w, t = torch.randn(5, 8), torch.randn(9, 8), torch.randint(0, 9, (5,))
+    mask = torch.rand(5).requires_grad_(True)
+    for hidden in (h, h.clone().requires_grad_(True)):
+        with pytest.raises(RuntimeError, match="gradient by the mask"):
+            stand_ins.linear_ce_ad(hidden, w, t, mask, 1, -100)
+        with pytest.raises(RuntimeError, match="gradient by the mask"):
+            stand_ins.linear_ce_ad(hidden, w, t, mask * 2, 0, -100)
+        stand_ins.linear_ce_ad(hidden, w, t, mask.detach(), 1, -100)
+        with torch.no_grad():
+            stand_ins.linear_ce_ad(hidden, w, t, mask, 1, -100)

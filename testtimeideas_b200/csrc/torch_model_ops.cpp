@@ -634,6 +634,7 @@ at::Tensor op_linear_ce_ad(const at::Tensor& h, const at::Tensor& w, const at::T
                            int64_t reduction, int64_t ignore_index) {
   const at::Tensor weights = defined_or(mask);
   refuse_tangents(kLceOp, {&h, &w, &weights});
+  TORCH_CHECK(!wants_grad({&weights}), "linear cross entropy forms no gradient by the mask: detach it");
   if (wants_grad({&h, &w})) return LinearCEFn::apply(h, w, targets, mask, reduction, ignore_index);
   at::AutoDispatchBelowADInplaceOrView below;
   return std::get<0>(raw_linear_ce().call(h, w, targets, mask, reduction, ignore_index, false));

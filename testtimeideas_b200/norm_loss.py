@@ -87,7 +87,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     Positions left out are not read: what ``hidden`` holds there changes nothing,
     and their gradient is exactly 0. A target outside the vocabulary raises: at
     once on CPU, at the next call of this library (or check_device_errors) on
-    CUDA. Differentiable twice in hidden, weight and the upstream gradient."""
+    CUDA. Differentiable twice in hidden, weight and the upstream gradient; a mask that
+    requires a gradient gets one on CPU and is refused on CUDA."""
     if reduction not in _lib.LCE_REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_lib.LCE_REDUCTIONS)}, got {reduction!r}")
     if not _kernel_path(hidden):
