@@ -453,3 +453,28 @@ def test_sizes_past_the_limits_are_refused(n, d, v, grad):
     t = torch.zeros(1, dtype=torch.long, device="cuda").expand(n)
     with pytest.raises(RuntimeError, match="at most 2\\^24 rows"):
         tb.linear_cross_entropy(h, w, t)
+
+
+@pytest.mark.parametrize("grad", (False, True))
+@pytest.mark.parametrize("n,v", [(1, 700), (4, 700), (4, 5000), (64, 250), (300, 2000)])
+def test_nearly_certain_tokens(n, v, grad):
+    """Logits near 520 that are exact in fp32, with one entry 16 or 24 above the others: the losses of tokens
+    that have it as their target are 1e-4 to 1e-8, far below an ulp of the logits, and never negative.
+
+    With the maximum taken out first, what is left are the errors of l, the sum of exponentials (2^-22
+    each and for each of two rescalings, their sum at most as much again), and of its logarithm: below
+    2^-19 in all, of 1 or of the loss."""
+    g = torch.Generator().manual_seed(n + v)
+    for gap in (0.25, 0.375):
+        h = torch.randint(1, 3, (n, 32), generator=g).float()
+        w = torch.randint(-2, 3, (v, 32), generator=g).float() / 8
+        h[:, -1], w[:, -1], w[5, -1] = 64.0, 8.0, 8.0 + gap
+        h, w = (x.to(torch.bfloat16).cuda() for x in (h, w))
+        t = torch.randint(0, v, (n,), generator=g)
+        t[::2] = 5
+        t = t.cuda()
+        ref = _definition(h.double(), w.double(), t, None, "none")
+        assert 0.0 < float(ref[0]) < 1e-2
+        loss = tb.linear_cross_entropy(h.requires_grad_(grad), w, t, reduction="none").detach()
+        assert float(loss.min()) >= 0.0
+        assert float(((loss.double() - ref).abs() / ref.clamp_min(1.0)).max()) <= 2.0**-19

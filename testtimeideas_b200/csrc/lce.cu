@@ -477,9 +477,13 @@ __global__ void __launch_bounds__(32 * kShares) lce_lse_kernel(const State st, c
     l = 0.f;
 #pragma unroll
     for (int i = 0; i < kShares; ++i) l += sh[i][lane].y * exp2f(sh[i][lane].x - sub);
-    const float lse2 = m + log2f(l);
-    st.lse2[s] = lse2;
-    v = st.mw[s] * (kLn2 * lse2 - ztgt[s]);
+    const float log_l = log2f(l);
+    st.lse2[s] = m + log_l;
+    // The large terms first, in one rounding: log-sum-exp and logit, each rounded, would leave ulps of
+    // the logit in a loss near 0. m carries the rounding of its own product with log2 e, and so do the
+    // exponentials in l.
+    const float ce = kLn2 * (fmaf(-ztgt[s], kLog2e, m) + log_l);
+    v = st.mw[s] * (ce < 0.f ? 0.f : ce);  // NaN stays
     if (reduction == TTT_LCE_NONE) loss[st.idx[s]] = v;
   }
   if (reduction != TTT_LCE_NONE) total_rows(v, sums, &st.head->ticket, st.head->denom, loss);
@@ -641,19 +645,20 @@ __global__ void __launch_bounds__(32 * kScoreWarps) lce_score_kernel(const RowAr
       float top = mx[r];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        z[r][u] = v0 + u < v_end ? z[r][u] * kLog2e : -INFINITY;
+        z[r][u] = v0 + u < v_end ? z[r][u] : -INFINITY;
         top = fmaxf(top, z[r][u]);
       }
-      const float sub = top == -INFINITY ? 0.f : top;
-      sum[r] *= exp2f(mx[r] - sub);
+      // the maximum's product with log2 e is rounded alike wherever it is used
+      const float sub = top == -INFINITY ? 0.f : __fmul_rn(top, kLog2e);
+      sum[r] *= exp2f(__fmul_rn(mx[r], kLog2e) - sub);
 #pragma unroll
-      for (int u = 0; u < U; ++u) sum[r] += exp2f(z[r][u] - sub);
+      for (int u = 0; u < U; ++u) sum[r] += exp2f(fmaf(z[r][u], kLog2e, -sub));
       mx[r] = top;
     }
   }
   if (lane == 0) {
 #pragma unroll
-    for (int r = 0; r < NR; ++r) sh[warp][r] = make_float2(mx[r], sum[r]);
+    for (int r = 0; r < NR; ++r) sh[warp][r] = make_float2(__fmul_rn(mx[r], kLog2e), sum[r]);
   }
   __syncthreads();
   if (threadIdx.x < nr) {

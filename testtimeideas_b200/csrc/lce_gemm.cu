@@ -494,8 +494,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
 #pragma unroll
           for (int j = 1; j < 64; ++j) m = fmaxf(m, v[j]);
           m = fmaxf(m, mx);
-          const float sub = m == -INFINITY ? 0.f : m * kLog2e;  // nothing seen yet: all exponentials are 0
-          sum *= fast_exp2(mx * kLog2e - sub);
+          // Nothing seen yet: all exponentials are 0. The maximum's product with log2 e is rounded alike
+          // here and in what is written out, so that its rounding cancels in the loss.
+          const float sub = m == -INFINITY ? 0.f : __fmul_rn(m, kLog2e);
+          sum *= fast_exp2(__fmul_rn(mx, kLog2e) - sub);
 #pragma unroll
           for (int j = 0; j < 64; ++j) sum += fast_exp2(fmaf(v[j], kLog2e, -sub));
           mx = m;
@@ -510,7 +512,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
           if (lane == src) p.ztgt[slot] = z;
         }
         release();
-        p.part[static_cast<int64_t>(tl.n * 2 + half) * p.n_pad + slot] = make_float2(mx * kLog2e, sum);
+        p.part[static_cast<int64_t>(tl.n * 2 + half) * p.n_pad + slot] = make_float2(__fmul_rn(mx, kLog2e), sum);
       } else if constexpr (KIND == kLceDualStats) {
         const int target = p.tgt[slot] - p.col0;
         const float lse2 = p.lse2[slot];
