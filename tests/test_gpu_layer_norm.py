@@ -124,6 +124,22 @@ def test_optional_parameters(weight, bias):
     _check(inp, **over)
 
 
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("d", (96, 301, 2050))
+def test_fp32_bias_alone(dtype, d):
+    """A bias in fp32 beside 16-bit x and no weight: the gradients take its upstream gradient as it is. ub
+    nearly cancels the rest of gdy here (one row), so that rounding it first would show: what is left
+    is 1e-2 of it, and carries a few fp32 roundings of terms near 4 (2e-6) and its own."""
+    inp = {**_inputs(1, d, dtype, torch.float32, seed=d), "w": None, "uw": None}
+    _check(inp)
+    with_zero = {k: None if v is None else v.double() for k, v in inp.items()}
+    with_zero["ub"] = torch.zeros_like(with_zero["ub"])
+    rest = _all(_definition, **with_zero)["gdy"][0]
+    small = 1e-2 * torch.randn(d, generator=torch.Generator().manual_seed(d), dtype=torch.float64)
+    got = _check(inp, ub=(small - rest).float())
+    assert float(got["gdy"].abs().max()) < 0.1
+
+
 @pytest.mark.parametrize("dtype", (torch.float16, torch.float32))
 def test_layouts(dtype):
     """Row slices, misaligned starts, a broadcast row, transposed storage, broadcast upstream gradients."""

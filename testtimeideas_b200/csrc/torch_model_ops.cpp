@@ -177,12 +177,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_layer_norm_bwd2(const at::Tens
                                                                   const OptTensor& w_, const at::Tensor& stats,
                                                                   const OptTensor& ux_, const OptTensor& uw_,
                                                                   const OptTensor& ub_) {
-  const ttt_norm_problem pb = norm_problem(x_, w_, std::nullopt, 0.0);
+  ttt_norm_problem pb = norm_problem(x_, w_, std::nullopt, 0.0);
   c10::cuda::CUDAGuard guard(x_.device());
   at::Tensor word = error_word_for(x_.get_device());
   raise_if_pending(x_.get_device(), word);
   check_stats(stats, x_, pb.rows);
-  const auto pt = w_.has_value() ? w_->scalar_type() : x_.scalar_type();
+  // without a weight the parameters' type is that of what comes for the bias
+  auto pt = w_.has_value() ? w_->scalar_type() : x_.scalar_type();
+  for (const OptTensor* u : {&uw_, &ub_})
+    if (!w_.has_value() && u->has_value() && (*u)->scalar_type() == at::kFloat) pt = at::kFloat;
+  pb.p_dtype = type_code(pt);
   const Rows x(x_, pb.dim), dy = grad_rows(dy_, x_, pb.dim, "dy");
   const at::Tensor w = vec(w_);
   const Rows ux = ux_.has_value() ? grad_rows(*ux_, x_, pb.dim, "ux") : Rows();
@@ -195,7 +199,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_layer_norm_bwd2(const at::Tens
     up[i] = u->to(pt).contiguous();
   }
   at::Tensor gx = at::empty(x_.sizes(), x_.options()), gdy = at::empty(x_.sizes(), x_.options());
-  at::Tensor gw = at::empty({w_.has_value() ? pb.dim : 0}, x_.options().dtype(pt));
+  at::Tensor gw = at::empty({w_.has_value() ? pb.dim : 0}, x_.options().dtype(w_.has_value() ? pt : x_.scalar_type()));
   at::Tensor work = w_.has_value() ? scratch(ttt_norm_work_bytes(&pb), x_) : at::Tensor();
   ttt_norm_bwd2_args a{};
   a.pb = pb;
