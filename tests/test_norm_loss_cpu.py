@@ -64,6 +64,27 @@ def test_linear_cross_entropy_left_out_rows_and_second_gradients():
         tb.linear_cross_entropy(h, w, t, m, reduction="max")
 
 
+def test_linear_cross_entropy_sums_16_bit_losses_in_32():
+    """Equal logits: every loss is log(8) rounded to bf16, and so is their mean under any mask. 70000
+    positions: neither the sum of their losses nor their count is a number of fp16."""
+    w, t = torch.zeros(8, 4, dtype=torch.bfloat16), torch.zeros(1300, dtype=torch.long)
+    h = torch.ones(1300, 4, dtype=torch.bfloat16)
+    one = tb.linear_cross_entropy(h[:1], w, t[:1])
+    assert one.dtype == torch.bfloat16 and abs(float(one) - 2.0794) < 0.005
+    for kept in (1001, 1005, 1011, 1300):
+        for weight in (1.0, 1 / 3):
+            m = torch.zeros(1300)
+            m[:kept] = weight
+            assert torch.equal(tb.linear_cross_entropy(h, w, t, m), one)
+    n = 70000
+    h, w, t = torch.ones(n, 2).half(), torch.zeros(8, 2).half().requires_grad_(True), torch.zeros(n, dtype=torch.long)
+    for m in (None, torch.ones(n)):
+        loss = tb.linear_cross_entropy(h, w, t, m)
+        assert loss.dtype == torch.float16 and abs(float(loss.detach()) - 2.0794) < 0.005
+        dw, = torch.autograd.grad(loss, w)
+        assert (dw[0].float() + 0.875).abs().max() < 0.01 and (dw[1:].float() - 0.125).abs().max() < 0.01
+
+
 def test_layer_norm_module_keeps_the_state_dict():
     ref, m = torch.nn.LayerNorm(24).double(), tb.LayerNorm(24).double()
     with torch.no_grad():

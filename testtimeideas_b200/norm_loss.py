@@ -51,8 +51,10 @@ class LayerNorm(nn.LayerNorm):
 
 # ---------------------------------------------------------------- linear cross entropy
 def _linear_ce_math(h, w, targets, mask, reduction, ignore_index):
-    """The same value in PyTorch (CPU tensors)."""
-    weight = torch.ones_like(targets, dtype=h.dtype) if mask is None else mask.to(h.dtype)
+    """The same value in PyTorch (CPU tensors); weights and sums in 32 bits or more."""
+    dtype = h.dtype
+    acc = torch.promote_types(dtype, torch.float32)
+    weight = torch.ones_like(targets, dtype=acc) if mask is None else mask.to(acc)
     keep = (weight != 0) & (targets != ignore_index)
     if bool(((targets < 0) | (targets >= w.shape[0]))[keep].any()):
         raise ValueError(f"linear cross entropy: a target is outside the vocabulary of {w.shape[0]}")
@@ -60,12 +62,12 @@ def _linear_ce_math(h, w, targets, mask, reduction, ignore_index):
     t = torch.where(keep, targets, torch.zeros_like(targets))
     z = torch.matmul(h, w.transpose(0, 1))
     ce = torch.logsumexp(z, -1) - z.gather(-1, t[..., None])[..., 0]
-    ce = torch.where(keep, ce * weight, torch.zeros_like(ce))
-    if reduction == "none":
-        return ce
-    if reduction == "sum":
-        return ce.sum()
-    return ce.sum() / (max(targets.numel(), 1) if mask is None else weight.sum().clamp_min(1.0))
+    ce = torch.where(keep, ce.to(acc) * weight, torch.zeros_like(weight))
+    if reduction == "mean":
+        ce = ce.sum() / (max(targets.numel(), 1) if mask is None else weight.sum().clamp_min(1.0))
+    elif reduction == "sum":
+        ce = ce.sum()
+    return ce.to(dtype)
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
