@@ -26,6 +26,16 @@ def _kernel_path(x: torch.Tensor) -> bool:
     return x.is_cuda
 
 
+def _autocast_to(dtype: Optional[torch.dtype], *tensors):
+    """The tensors as autocast hands them to an op it runs in `dtype` (None: its own 16-bit type);
+    unchanged outside autocast, and where they are not fp16, bf16 or fp32."""
+    if not torch.is_autocast_enabled("cuda"):
+        return tensors
+    to = dtype or torch.get_autocast_dtype("cuda")
+    low = (torch.float16, torch.bfloat16, torch.float32)
+    return tuple(t.to(to) if t is not None and t.dtype in low else t for t in tensors)
+
+
 # ---------------------------------------------------------------- layer norm
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
@@ -34,10 +44,11 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     x: [..., dim] in fp16, bf16 or fp32, any strides (a layout that is not rows
     of unit stride is copied); weight, bias: [dim] in x's dtype or fp32, either
     may be None. On CUDA dim is at most 16384; statistics and sums are fp32.
+    Under autocast it runs in fp32, as F.layer_norm does.
     Differentiable twice in x, weight and the upstream gradient."""
     if not _kernel_path(x):
         return F.layer_norm(x, x.shape[-1:], weight, bias, eps)
-    return _lib.layer_norm_ad(x, weight, bias, eps)
+    return _lib.layer_norm_ad(*_autocast_to(torch.float32, x, weight, bias), eps)
 
 
 class LayerNorm(nn.LayerNorm):
@@ -75,7 +86,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
                          ignore_index: int = -100) -> torch.Tensor:
     """Token cross entropy of the logits ``hidden @ weight.T``, which are never stored.
 
-    hidden: [..., dim]; weight: [vocab, dim] (both fp16 or both bf16 on CUDA);
+    hidden: [..., dim]; weight: [vocab, dim] (both fp16 or both bf16 on CUDA; autocast
+    casts both to its type, as F.linear's operands);
     targets: integers, hidden's leading shape; mask: the targets' shape, bool or
     weights m (a position with m = 0 is left out). The position's loss is m times
     its cross entropy, 0 where the target is ``ignore_index``; the result is fp32
@@ -95,4 +107,5 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
         raise ValueError(f"reduction must be one of {sorted(_lib.LCE_REDUCTIONS)}, got {reduction!r}")
     if not _kernel_path(hidden):
         return _linear_ce_math(hidden, weight, targets, mask, reduction, ignore_index)
+    hidden, weight = _autocast_to(None, hidden, weight)
     return _lib.linear_ce_ad(hidden, weight, targets, mask, reduction, ignore_index)
