@@ -137,11 +137,9 @@ typedef struct {
 int ttt_lce_fwd(const ttt_lce_fwd_args* a, void* stream);
 
 /* With c_i = dloss m_i / N (dloss_i m_i for TTT_LCE_NONE): G = c (P - onehot(t)),
- * dh = G w, dw = G^T h. */
+ * dh = G w, dw = G^T h. h itself is not asked for: `state` holds its participating rows. */
 typedef struct {
   ttt_lce_problem pb;
-  const void* h;
-  int64_t h_stride;
   const void* w;
   int64_t w_stride;
   const void* state;
@@ -159,8 +157,6 @@ int ttt_lce_bwd(const ttt_lce_bwd_args* a, void* stream);
  * gh = D w + G uw, gw = D^T h + G^T uh, d/dc_i = rho_i - A_{i t_i}. */
 typedef struct {
   ttt_lce_problem pb;
-  const void* h;
-  int64_t h_stride;
   const void* w;
   int64_t w_stride;
   const void* uh; /* [n, dim], any row stride; NULL: zeros */

@@ -187,3 +187,22 @@ def test_gradients_refuse_what_is_not_the_forwards():
             ops.layer_norm_bwd(x["h"], x["h"], None, bad, True, False, False, torch.bfloat16)
         with pytest.raises(RuntimeError, match="stats must be"):
             ops.layer_norm_bwd2(x["h"], x["h"], None, bad, x["h"], None, None)
+
+
+def test_gradients_do_not_copy_hidden():
+    """The gradients read the rows that the forward gathered; a transposed hidden costs them no copy."""
+    x, ops = _inputs(n=4096, d=512, v=600, seed=8), torch.ops.ttt
+    loss, state = ops.linear_ce(x["h"], x["w"], x["t"], None, 1, -100, True)
+    one = torch.ones_like(loss)
+    peaks, outs = [], []
+    for h in (x["h"], x["h"].t().contiguous().t()):
+        for call in (lambda: ops.linear_ce_bwd(one, h, x["w"], state, 1, True, True),
+                     lambda: ops.linear_ce_bwd2(one, h, x["w"], state, 1, x["h"], x["w"], True, True, True)):
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_allocated()
+            outs.append(call())
+            torch.cuda.synchronize()
+            peaks.append(torch.cuda.max_memory_allocated() - before)
+    assert peaks[:2] == peaks[2:]
+    assert all(torch.equal(a, b) for i in (0, 1) for a, b in zip(outs[i], outs[i + 2]))

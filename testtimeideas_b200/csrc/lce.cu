@@ -989,7 +989,6 @@ int ttt_lce_bwd(const ttt_lce_bwd_args* a, void* stream) {
   if (a->dh != nullptr && !aligned(a->dh, 16)) return TTT_ERR_ALIGN;
   if (pb.n == 0)
     return a->dw != nullptr ? zero(a->dw, pb.vocab * pb.dim * 2, static_cast<cudaStream_t>(stream)) : TTT_OK;
-  if (a->h == nullptr) return TTT_ERR_NULL;
   if (a->work == nullptr) return TTT_ERR_SCRATCH;
   if (!aligned(a->work, 256) || !aligned(a->state, 256)) return TTT_ERR_ALIGN;
   Pass p(pb, 1, a->state, a->work, a->dloss, a->err, stream);
@@ -1016,7 +1015,6 @@ int ttt_lce_bwd2(const ttt_lce_bwd2_args* a, void* stream) {
     if (a->gdloss != nullptr && gd > 0) TTT_TRY(zero(a->gdloss, gd * 4, s));
     return TTT_OK;
   }
-  if (a->h == nullptr) return TTT_ERR_NULL;
   if (a->work == nullptr) return TTT_ERR_SCRATCH;
   if (!aligned(a->work, 256) || !aligned(a->state, 256)) return TTT_ERR_ALIGN;
   Pass p(pb, 2, a->state, a->work, a->dloss, a->err, stream);

@@ -338,15 +338,12 @@ std::tuple<at::Tensor, at::Tensor> op_linear_ce_bwd(const at::Tensor& dloss_, co
   at::Tensor word = error_word_for(h_.get_device());
   raise_if_pending(h_.get_device(), word);
   check_state(state, h_, pb);
-  const Rows h(h_, pb.dim);
   const at::Tensor w = weight_rows(w_), dloss = lce_upstream(dloss_, h_, pb);
   at::Tensor dh = need_dh ? at::empty(h_.sizes(), h_.options()) : at::empty({0}, h_.options());
   at::Tensor dw = need_dw ? at::empty(w_.sizes(), w_.options()) : at::empty({0}, w_.options());
   at::Tensor work = lce_work(pb, 1, h_);
   ttt_lce_bwd_args a{};
   a.pb = pb;
-  a.h = h.p;
-  a.h_stride = h.stride;
   a.w = w.data_ptr();
   a.w_stride = w.stride(0);
   a.state = state.data_ptr();
@@ -370,7 +367,6 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_linear_ce_bwd2(const at::Tenso
   at::Tensor word = error_word_for(h_.get_device());
   raise_if_pending(h_.get_device(), word);
   check_state(state, h_, pb);
-  const Rows h(h_, pb.dim);
   const at::Tensor w = weight_rows(w_), dloss = lce_upstream(dloss_, h_, pb);
   Rows uh;
   at::Tensor uw;
@@ -390,8 +386,6 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> op_linear_ce_bwd2(const at::Tenso
   at::Tensor work = lce_work(pb, 2, h_);
   ttt_lce_bwd2_args a{};
   a.pb = pb;
-  a.h = h.p;
-  a.h_stride = h.stride;
   a.w = w.data_ptr();
   a.w_stride = w.stride(0);
   a.uh = uh.p;
@@ -655,7 +649,7 @@ TORCH_LIBRARY_FRAGMENT(ttt, m) {
   m.def("layer_norm_bwd2(Tensor dy, Tensor x, Tensor? w, Tensor stats, Tensor? ux, Tensor? uw, Tensor? ub) "
         " -> (Tensor gdy, Tensor gx, Tensor gw)");
   // reduction: 0 none, 1 mean, 2 sum; state (bytes) is what the gradients need of the forward
-  // (empty without need_state).
+  // (empty without need_state); of h itself they take the shape and the type.
   m.def("linear_ce(Tensor h, Tensor w, Tensor targets, Tensor? mask, int reduction, int ignore_index, bool "
         "need_state) -> (Tensor loss, Tensor state)");
   m.def("linear_ce_bwd(Tensor dloss, Tensor h, Tensor w, Tensor state, int reduction, bool need_dh, bool need_dw) -> "
