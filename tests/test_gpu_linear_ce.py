@@ -350,6 +350,24 @@ def test_gradient_by_the_upstream_is_the_loss_direction():
     assert got["gd"].shape == (40,)
 
 
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("n,d,v", [(40, 64, 100), (300, 136, 1500)])
+def test_gradient_by_the_upstream_along_the_gradient(n, d, v, dtype):
+    """With uh = dh of dloss = 1 the gradient by dloss_i is |dh_i|^2. dh is within 4u of its largest entry of
+    what the second gradient forms in fp32, and that is within 1e-5 of the terms' scale (twice the largest A)."""
+    inp = _inputs(n, d, v, dtype, seed=n)
+    h, dloss = inp["h"].requires_grad_(True), torch.ones(n, device="cuda", requires_grad=True)
+    loss = tb.linear_cross_entropy(h, inp["w"], inp["t"], reduction="none")
+    dh, = torch.autograd.grad(loss, h, dloss, create_graph=True)
+    uh = dh.detach()
+    gd, = torch.autograd.grad(dh, dloss, uh)
+    x = uh.double()
+    scale = 2 * float((x @ inp["w"].double().t()).abs().max())
+    bound = 4 * U[dtype] * float(x.abs().max()) * x.abs().sum(1) + 1e-5 * scale
+    assert bool(((gd.double() - x.square().sum(1)).abs() <= bound).all())
+    assert float(bound.max()) < 0.2 * float(x.square().sum(1).median())
+
+
 def test_only_one_gradient_wanted():
     inp = _inputs(70, 64, 300, torch.bfloat16, seed=55)
     h, w = inp["h"].clone().requires_grad_(True), inp["w"].clone().requires_grad_(True)
