@@ -496,3 +496,24 @@ def test_nearly_certain_tokens(n, v, grad):
         loss = tb.linear_cross_entropy(h.requires_grad_(grad), w, t, reduction="none").detach()
         assert float(loss.min()) >= 0.0
         assert float(((loss.double() - ref).abs() / ref.clamp_min(1.0)).max()) <= 2.0**-19
+
+
+@pytest.mark.parametrize("up", (float("inf"), float("nan")))
+@pytest.mark.parametrize("reduction", ("mean", "sum", "none"))
+def test_rows_left_out_stay_zero_when_the_upstream_is_not_finite(reduction, up):
+    """An overflowed loss scale: the rows that take part lose their gradients, those left out keep exact
+    zeros; with none that takes part the weight gradients are zeros too."""
+    n = 150
+    inp = _inputs(n, 72, 300, torch.float16, seed=67)
+    m = _mask(n, "weights", 68)
+    inp["t"][1::9] = -100
+    out = (m == 0) | (inp["t"] == -100)
+    fn = lambda m: lambda h, w: tb.linear_cross_entropy(h, w, inp["t"], m, reduction=reduction)  # noqa: E731
+    dl = torch.full((n,) if reduction == "none" else (), up, device="cuda")
+    got = _all(fn(m), inp["h"], inp["w"], dl, inp["uh"], inp["uw"])
+    for k in ("dh", "gh"):
+        assert not got[k][out].any(), k
+        assert not got[k][~out].isfinite().all(), k
+    none = _all(fn(torch.zeros(n, device="cuda")), inp["h"], inp["w"], dl, inp["uh"], inp["uw"])
+    for k in ("dh", "gh", "dw", "gw", "gd"):
+        assert not none[k].any(), k

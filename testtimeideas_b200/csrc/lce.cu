@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(256) lce_scatter_kernel(const int* slot, const
   const int64_t i = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / width;
   if (i >= n) return;
   const int s = slot[i];
-  const float mul = coef.out();
+  const float mul = s >= 0 ? coef.out() : 0.f;  // an infinite one leaves the other rows' zeros alone
   uint16_t* dst = dh + i * dim;
 #pragma unroll 4
   for (int c = (threadIdx.x % width) * 4; c < dim; c += width * 4) {

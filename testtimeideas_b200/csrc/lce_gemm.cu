@@ -612,13 +612,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
             tmem_wait_ld();
             reg_fence(v);
             if (q == C::HALF / 64 - 1) release();
-          } else {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] *= mul;
+          } else {  // no row takes part: zeros, whatever the upstream value is
 #pragma unroll
             for (int j = 0; j < 64; ++j) v[j] = 0.f;
           }
           const int cq = c0 + q * 64;
-#pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] *= mul;
           if (cq >= p.dim || row0 >= p.cols) continue;
           if (boxes) {
             store_panel<BF16, C::BOXES>(panel, turn, &p.dw_out, lane, cq, row0, v);
