@@ -517,3 +517,27 @@ def test_rows_left_out_stay_zero_when_the_upstream_is_not_finite(reduction, up):
     none = _all(fn(torch.zeros(n, device="cuda")), inp["h"], inp["w"], dl, inp["uh"], inp["uw"])
     for k in ("dh", "gh", "dw", "gw", "gd"):
         assert not none[k].any(), k
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("n,v", [(1, 700), (5, 3000), (300, 2000)])
+def test_gradients_of_nearly_certain_tokens(n, v, dtype):
+    """The logits of the test above, every target the likely entry: G there is p - 1, 1e-2 to 1e-4, and column 0
+    of the hidden gradient is that entry alone (w is 0 in it except for a 1 in the target's row). It is rounded
+    twice (2u); p is within 2^-19 as l is there."""
+    g = torch.Generator().manual_seed(n + v)
+    h = torch.randint(1, 3, (n, 32), generator=g).float()
+    w = torch.randint(-2, 3, (v, 32), generator=g).float() / 8
+    h[:, -1], w[:, -1], w[5, -1] = 64.0, 8.0, 8.25
+    h[:, 0], w[:, 0], w[5, 0] = 0.0, 0.0, 1.0
+    h, w = (x.to(dtype).cuda().requires_grad_(True) for x in (h, w))
+    t = torch.full((n,), 5, device="cuda")
+    p = torch.softmax(h.detach().double() @ w.detach().double().t(), 1)[:, 5]
+    assert 1e-5 < float((1 - p).min()) and float((1 - p).max()) < 0.05
+    up = 1024.0
+    dh, = torch.autograd.grad(tb.linear_cross_entropy(h, w, t, reduction="sum"), h, torch.full((), up, device="cuda"))
+    err = (dh[:, 0].double() - up * (p - 1)).abs()
+    assert bool((err <= up * (2 * U[dtype] * (1 - p) + 2.0**-19)).all())
+    # one entry of the vocabulary: p is 1, and what 2^-19 of it leaves is all there is
+    dh, = torch.autograd.grad(tb.linear_cross_entropy(h, w[:1], t * 0, reduction="sum"), h)
+    assert float(dh.abs().max()) <= 2.0**-19 * float(w[:1].detach().abs().max())

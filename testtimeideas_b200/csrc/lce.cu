@@ -4,7 +4,7 @@
 // The participating rows are listed first (slots), and h is gathered into a
 // compact copy that the state keeps, so masked rows cost no products and whatever
 // they hold stays out of every sum. Then
-//   forward   statistics of z, combined per row into the base-2 log-sum-exp
+//   forward   statistics of z, combined per row into maximum and sum of exponentials
 //   gradient  per piece of the vocabulary: G in 16 bits; then in one launch G w,
 //             added to fp32 partial rows, and G^T h, rounded into the piece's rows
 //             of dw; at the end the partial rows are added in order and scattered
@@ -62,7 +62,10 @@ struct State {
   int* idx;      // [n_pad] source row of a slot, -1 past the last
   int* tgt;      // [n_pad] target of a slot, -1 past the last
   float* mw;     // [n_pad] mask weight of a slot, 0 past the last
-  float* lse2;   // [n_pad] base-2 log-sum-exp of a slot, +inf past the last
+  // The row's log-sum-exp in two parts, p = exp2(z log2 e - top2) / l: one rounded number of the
+  // logits' size would leave its ulps in p - 1.
+  float* top2;   // [n_pad] base-2 maximum of a slot, +inf past the last
+  float* inv_l;  // [n_pad] 1 / l, the sum of exponentials below it, 0 past the last
   int* slot;     // [n] slot of a source row, -1 if it takes no part
   uint16_t* hc;  // [n_pad][dim_pad] rows of h by slot, zeros past the last
 };
@@ -74,7 +77,8 @@ int64_t state_layout(const ttt_lce_problem& pb, void* base, State* s) {
   t.idx = a.take<int>(n_pad);
   t.tgt = a.take<int>(n_pad);
   t.mw = a.take<float>(n_pad);
-  t.lse2 = a.take<float>(n_pad);
+  t.top2 = a.take<float>(n_pad);
+  t.inv_l = a.take<float>(n_pad);
   t.slot = a.take<int>(pb.n);
   t.hc = a.take<uint16_t>(n_pad * up(pb.dim, 8));
   if (s != nullptr) *s = t;
@@ -287,7 +291,10 @@ __device__ __forceinline__ void copy_rows(const RowArgs& a, const int64_t (&row)
 __device__ __forceinline__ void clear_slot(const RowArgs& a, int64_t s, int lane) {
   for (int c = lane * 8; c < a.dim_pad; c += 256)
     *reinterpret_cast<uint4*>(a.dst + s * a.dim_pad + c) = make_uint4(0, 0, 0, 0);
-  if (lane == 0) a.st.idx[s] = -1, a.st.tgt[s] = -1, a.st.mw[s] = 0.f, a.st.lse2[s] = INFINITY;
+  if (lane == 0) {
+    a.st.idx[s] = -1, a.st.tgt[s] = -1, a.st.mw[s] = 0.f;
+    a.st.top2[s] = INFINITY, a.st.inv_l[s] = 0.f;
+  }
 }
 
 // Lists the participating rows and gathers h. Block b owns a range of a.list_rows rows,
@@ -439,7 +446,7 @@ __device__ __forceinline__ void total_rows(float v, float* sums, unsigned* ticke
 }
 
 // Merges the half tiles' (max, sum) of a row: 32 rows and 32 shares of the tiles per
-// block, shares in order. Writes lse2 and the row's weighted loss.
+// block, shares in order. Writes top2, inv_l and the row's weighted loss.
 constexpr int kShares = 32;
 __global__ void __launch_bounds__(32 * kShares) lce_lse_kernel(const State st, const float2* part, const float* ztgt,
                                                                int parts, int n_pad, int reduction, float* sums,
@@ -477,12 +484,12 @@ __global__ void __launch_bounds__(32 * kShares) lce_lse_kernel(const State st, c
     l = 0.f;
 #pragma unroll
     for (int i = 0; i < kShares; ++i) l += sh[i][lane].y * exp2f(sh[i][lane].x - sub);
-    const float log_l = log2f(l);
-    st.lse2[s] = m + log_l;
+    st.top2[s] = m;
+    st.inv_l[s] = 1.f / l;
     // The large terms first, in one rounding: log-sum-exp and logit, each rounded, would leave ulps of
     // the logit in a loss near 0. m carries the rounding of its own product with log2 e, and so do the
     // exponentials in l.
-    const float ce = kLn2 * (fmaf(-ztgt[s], kLog2e, m) + log_l);
+    const float ce = kLn2 * (fmaf(-ztgt[s], kLog2e, m) + log2f(l));
     v = st.mw[s] * (ce < 0.f ? 0.f : ce);  // NaN stays
     if (reduction == TTT_LCE_NONE) loss[st.idx[s]] = v;
   }
@@ -832,7 +839,7 @@ struct Pass {
     ttt::LceGemm g;
     std::memset(&g, 0, sizeof(g));
     g.head = st.head, g.coef = coef;
-    g.tgt = st.tgt, g.lse2 = st.lse2, g.rho = w.rho;
+    g.tgt = st.tgt, g.top2 = st.top2, g.inv_l = st.inv_l, g.rho = w.rho;
     g.part = w.part, g.ztgt = w.ztgt, g.ticket = w.counters;
     g.n_pad = static_cast<int>(q.n_pad), g.dim = q.dim, g.dim_pad = q.dim_pad;
     g.col0 = static_cast<int>(col0), g.cols = static_cast<int>(cols);

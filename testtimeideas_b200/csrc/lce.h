@@ -72,7 +72,7 @@ struct LceGemm {
   LceCoef coef;
   // rows of the state / work arrays, indexed by row slot
   const int* tgt;
-  const float* lse2;
+  const float *top2, *inv_l;
   const float* rho;
   float2* part;      // statistics kinds: [2 * n_tiles][n_pad]
   float* ztgt;       // statistics kinds: value at the target

@@ -515,7 +515,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
         p.part[static_cast<int64_t>(tl.n * 2 + half) * p.n_pad + slot] = make_float2(__fmul_rn(mx, kLog2e), sum);
       } else if constexpr (KIND == kLceDualStats) {
         const int target = p.tgt[slot] - p.col0;
-        const float lse2 = p.lse2[slot];
+        const float top2 = p.top2[slot], inv_l = p.inv_l[slot];
         float z[64], v[64];
         tmem_ld_nw<64>(acc, z);
         tmem_ld_nw<64>(acc + C::BN, v);
@@ -525,11 +525,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
         float sum = 0.f, big = 0.f;
 #pragma unroll
         for (int j = 0; j < 64; ++j) {
-          float x = fast_exp2(fmaf(z[j], kLog2e, -lse2)) * v[j];
+          float x = fast_exp2(fmaf(z[j], kLog2e, -top2)) * v[j];
           if (c0 + j >= p.cols) x = 0.f;
           sum += x;
           big = fmaxf(big, fabsf(x));
         }
+        sum *= inv_l;
+        big *= inv_l;
         unsigned hit = __ballot_sync(0xffffffffu, target >= c0 && target < min(c0 + C::HALF, p.cols));
         while (hit != 0) {
           const int src = __ffs(hit) - 1;
@@ -542,7 +544,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
         p.part[static_cast<int64_t>(tl.n * 2 + half) * p.n_pad + slot] = make_float2(sum, big);
       } else if constexpr (C::GRAD) {
         const int target = p.tgt[slot] - p.col0;
-        const float lse2 = p.lse2[slot], coef = slot < n_active ? p.coef.row(slot) * mul : 0.f;
+        const float top2 = p.top2[slot], coef = slot < n_active ? p.coef.row(slot) * mul : 0.f;
+        const float coef_l = coef * p.inv_l[slot];  // c p = coef_l * exp2(z log2 e - top2)
         const float rho = C::DUAL ? p.rho[slot] : 0.f;
         const int row0 = tl.m * C::BM + static_cast<int>(rank) * C::ROWS_A + quarter * 32;
 #pragma unroll 1
@@ -553,7 +556,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
           reg_fence(v);
           const int cq = c0 + q * 64;
 #pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] = fast_exp2(fmaf(v[j], kLog2e, -lse2));
+          for (int j = 0; j < 64; ++j) v[j] = fast_exp2(fmaf(v[j], kLog2e, -top2));
           if constexpr (C::DUAL) {
             float d[64];
             tmem_ld_nw<64>(acc + C::BN, d);
@@ -561,19 +564,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LceCfg<KIND>::NTHREA
             reg_fence(d);
             release();
 #pragma unroll
-            for (int j = 0; j < 64; ++j) d[j] = coef * v[j] * (d[j] - rho);
+            for (int j = 0; j < 64; ++j) d[j] = coef_l * v[j] * (d[j] - rho);
             store_panel<BF16, C::BOXES>(panel, turn, &p.out[1], lane, cq, row0, d);
           } else if (q == C::HALF / 64 - 1) {
             release();
           }
+#pragma unroll
+          for (int j = 0; j < 64; ++j) v[j] *= coef_l;
           const bool here = target >= cq && target < cq + 64;
           if (__any_sync(0xffffffffu, here)) {
             const int tj = here ? target - cq : -1;
 #pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] -= j == tj ? 1.f : 0.f;
+            for (int j = 0; j < 64; ++j) v[j] -= j == tj ? coef : 0.f;
           }
-#pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] *= coef;
           store_panel<BF16, C::BOXES>(panel, turn, &p.out[0], lane, cq, row0, v);
         }
       } else if (!tl.dw) {
