@@ -124,8 +124,10 @@ int64_t makespan(int64_t pairs, int64_t n_long, int64_t len, int64_t n_short, in
 // them let the pairs end together and fill the GPU with few tokens, but each costs a
 // pass over fp32 partial rows. The count with the least time is taken, with a step at
 // 0.3 us (512 cycles), a tile's start and end at eight steps, and the partial rows
-// written and read at 6.5 TB/s. At 8192 x 768 x 32000 the second gradient's pieces (96
-// tiles of 512 steps against 189 of 264) take 1552 steps uncut and 1408 in three shares.
+// written and read at 6.5 TB/s. The model counts 64-wide steps; the kernel cuts the shares at
+// its 128-wide stages, so a modelled length is off by up to one of those. At 8192 x 768 x 32000
+// the second gradient's pieces (96 tiles of 512 steps against 189 of 264) take 1552 steps uncut
+// and 1408 in three shares.
 int plan_splits(const Plan& q, int segs, int64_t pairs) {
   const int64_t cols = std::min(q.piece, q.vocab);
   const int64_t dt = up(q.dim, ttt::kLceBN) / ttt::kLceBN, kt = up(cols, 64) / 64;
