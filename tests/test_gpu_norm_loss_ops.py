@@ -206,3 +206,14 @@ def test_gradients_do_not_copy_hidden():
             peaks.append(torch.cuda.max_memory_allocated() - before)
     assert peaks[:2] == peaks[2:]
     assert all(torch.equal(a, b) for i in (0, 1) for a, b in zip(outs[i], outs[i + 2]))
+
+
+def test_gradients_refuse_a_state_of_other_rows():
+    x, ops = _inputs(n=6, d=64, v=90), torch.ops.ttt
+    loss, state = ops.linear_ce(x["h"][:5], x["w"], x["t"][:5], None, 1, -100, True)
+    for n in (4, 6):
+        h = x["h"][:n]
+        with pytest.raises(RuntimeError, match="state must be"):
+            ops.linear_ce_bwd(torch.ones_like(loss), h, x["w"], state, 1, True, True)
+        with pytest.raises(RuntimeError, match="state must be"):
+            ops.linear_ce_bwd2(torch.ones_like(loss), h, x["w"], state, 1, h, x["w"], True, True, True)

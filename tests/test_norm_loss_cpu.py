@@ -288,3 +288,11 @@ def test_a_mask_that_wants_a_gradient_is_refused(stand_ins):
         stand_ins.linear_ce_ad(hidden, w, t, mask.detach(), 1, -100)
         with torch.no_grad():
             stand_ins.linear_ce_ad(hidden, w, t, mask, 1, -100)
+
+
+def test_state_sizes_tell_row_counts_apart(lib):
+    """The gradients know a state by its size, and index with the rows it lists."""
+    lib.ttt_lce_state_bytes.restype = ctypes.c_int64
+    for d in (8, 72, 768):
+        sizes = [lib.ttt_lce_state_bytes(ctypes.byref(LceProblem(n, 100, d, 1, 1, 0, -100))) for n in range(600)]
+        assert len(set(sizes)) == 600 and sizes == [_lib._lce_state_bytes(n, d) for n in range(600)]

@@ -552,11 +552,11 @@ LCE_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
 def _lce_state_bytes(n: int, dim: int) -> int:
-    """ttt_lce_state_bytes: the head, five arrays of n rows padded to 256, one of n, and the
-    gathered rows of h, each in 256-byte parts."""
+    """ttt_lce_state_bytes: the head, five arrays of n rows padded to 256 and the gathered rows
+    of h, each in 256-byte parts, and one array of n."""
     up = lambda b: (b + 255) // 256 * 256  # noqa: E731
     rows = up(n)
-    return 256 + 5 * up(rows * 4) + up(n * 4) + up(rows * ((dim + 7) // 8 * 8) * 2)
+    return 256 + 5 * up(rows * 4) + up(rows * ((dim + 7) // 8 * 8) * 2) + n * 4
 
 
 def linear_ce_ad(h, w, targets, mask, reduction: str, ignore_index: int):

@@ -66,9 +66,10 @@ struct State {
   // logits' size would leave its ulps in p - 1.
   float* top2;   // [n_pad] base-2 maximum of a slot, +inf past the last
   float* inv_l;  // [n_pad] 1 / l, the sum of exponentials below it, 0 past the last
-  int* slot;     // [n] slot of a source row, -1 if it takes no part
   uint16_t* hc;  // [n_pad][dim_pad] rows of h by slot, zeros past the last
+  int* slot;     // [n] slot of a source row, -1 if it takes no part
 };
+// The size ends with the last of `slot`, so that a state of one row count does not pass for another's.
 int64_t state_layout(const ttt_lce_problem& pb, void* base, State* s) {
   Arena a(base);
   const int64_t n_pad = up(pb.n, ttt::kLceBM);
@@ -79,10 +80,11 @@ int64_t state_layout(const ttt_lce_problem& pb, void* base, State* s) {
   t.mw = a.take<float>(n_pad);
   t.top2 = a.take<float>(n_pad);
   t.inv_l = a.take<float>(n_pad);
-  t.slot = a.take<int>(pb.n);
   t.hc = a.take<uint16_t>(n_pad * up(pb.dim, 8));
+  const int64_t slots_at = a.used;
+  t.slot = a.take<int>(pb.n);
   if (s != nullptr) *s = t;
-  return a.used;
+  return slots_at + pb.n * static_cast<int64_t>(sizeof(int));
 }
 
 int device_sms() {
